@@ -94,6 +94,32 @@ class TrainConfigC(C.Structure):
     ]
 
 
+class KVCacheC(C.Structure):
+    """glc_kv_cache (include/gollama_cuda.h)."""
+
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("num_pages", C.c_int),
+        ("page_size", C.c_int),
+        ("num_kv_heads", C.c_int),
+        ("head_dim", C.c_int),
+    ]
+
+
+class KVBatchC(C.Structure):
+    """glc_kv_batch (include/gollama_cuda.h)."""
+
+    _fields_ = [
+        ("page_table", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("starts", C.c_void_p),
+        ("num_seqs", C.c_int),
+        ("max_pages", C.c_int),
+        ("num_rows", C.c_int),
+    ]
+
+
 def _nccl_hint() -> None:
     """Point the library at the NCCL that PyTorch bundles, when installed, so
     one process never holds two NCCL builds under the same soname."""

@@ -3,12 +3,18 @@
 #include <cstring>
 
 #include "glc_internal.h"
+#include "sm100.cuh"
 
 using glc::Context;
 
 static inline Context* C_(glc_ctx* c) { return reinterpret_cast<Context*>(c); }
 
 namespace glc {
+
+const char* device_error_text(int code) {
+  return code == GLC_DEV_BAD_ARGUMENT ? "an index or a length in device memory is out of range"
+                                      : "a bounded wait in a kernel ran out";
+}
 
 int Context::workspace(size_t bytes, void** out) {
   if (bytes > ws_bytes) {
@@ -74,6 +80,8 @@ int glc_init(int device, glc_ctx** out) {
       cudaMalloc(&c->d_err, sizeof(int)) != cudaSuccess || cudaMemset(c->d_err, 0, sizeof(int)) != cudaSuccess ||
       cudaMalloc(&c->dyn_ctr, sizeof(int) * Context::kDynCounters) != cudaSuccess ||
       cudaMemset(c->dyn_ctr, 0, sizeof(int) * Context::kDynCounters) != cudaSuccess ||
+      cudaMalloc(&c->kv_count, sizeof(int) * Context::kKvCounters) != cudaSuccess ||
+      cudaMemset(c->kv_count, 0, sizeof(int) * Context::kKvCounters) != cudaSuccess ||
       cudaEventCreate(&c->timer_start) != cudaSuccess || cudaEventCreate(&c->timer_stop) != cudaSuccess) {
     delete c;
     return GLC_ERR_CUDA;
@@ -103,6 +111,7 @@ int glc_destroy(glc_ctx* ctx) {
   if (c->ws) cudaFree(c->ws);
   if (c->d_err) cudaFree(c->d_err);
   if (c->dyn_ctr) cudaFree(c->dyn_ctr);
+  if (c->kv_count) cudaFree(c->kv_count);
   if (c->timer_start) cudaEventDestroy(c->timer_start);
   if (c->timer_stop) cudaEventDestroy(c->timer_stop);
   for (auto& r : c->prof) {
@@ -147,7 +156,7 @@ int glc_sync(glc_ctx* ctx) {
   if (err != 0) {
     cudaMemset(c->d_err, 0, sizeof(int));
     char msg[128];
-    std::snprintf(msg, sizeof msg, "device error %d (a bounded wait in a kernel ran out)", err);
+    std::snprintf(msg, sizeof msg, "device error %d (%s)", err, glc::device_error_text(err));
     return c->fail(GLC_ERR_DEVICE, msg);
   }
   return GLC_OK;

@@ -48,6 +48,10 @@ struct Context {
   static constexpr int kDynCounters = 1024;
   int* dyn_ctr = nullptr;
   unsigned long long dyn_next = 0;
+  // arrival counters of the attention over the 4-bit cache, one per CTA: zero
+  // between calls (the last CTA to arrive clears its counter)
+  static constexpr int kKvCounters = 1024;
+  int* kv_count = nullptr;
   // device tile lists of grouped CTA-pair GEMM launches, by (tiles and
   // k-blocks of each problem, clusters); built once per shape
   std::vector<std::pair<std::array<long long, 5>, int*>> gemm_sched;
@@ -112,6 +116,9 @@ struct Context {
   // Returns a device scratch buffer of at least `bytes` (stream-ordered use only).
   int workspace(size_t bytes, void** out);
 };
+
+// What a code in the device error word means.
+const char* device_error_text(int code);
 
 // An NVTX range for the lifetime of the object when the context traces
 // (NVTX v3 is header-only: without a tool attached the calls return at once).

@@ -1,0 +1,270 @@
+// The paged 4-bit key/value cache: storing new tokens (with the rotation of
+// keys and queries) and reading tokens back.
+//
+// Both are one pass over their operands and bound by memory: a stored token
+// moves (num_heads + 2 num_kv_heads) * head_dim floats in, num_heads *
+// head_dim floats and 2 num_kv_heads * head_dim * 9/16 bytes out.
+#include <cfloat>
+
+#include "kv_cache.cuh"
+
+namespace glc {
+namespace {
+
+// A thread holds 4 consecutive elements (two rotation pairs) of one head of
+// one row; 8 neighbouring lanes hold the 32 that share a scale, so the largest
+// magnitude is three shuffles and no shared memory is used.  blockIdx.x covers
+// the heads of a row (queries, keys, values, in that order), blockIdx.y
+// strides over the rows.
+__global__ void __launch_bounds__(256)
+    kv_append_kernel(KvPools c, KvSeqs s, const float* __restrict__ q, size_t q_ld, float* __restrict__ q_out,
+                     size_t q_out_ld, int heads, const float* __restrict__ k, size_t k_ld,
+                     const float* __restrict__ v, size_t v_ld, const float* __restrict__ cos_t,
+                     const float* __restrict__ sin_t, int table_rows, int* __restrict__ err) {
+  GLC_PDL_ENTRY();
+  const int quads = c.head_dim >> 2;
+  const int u = blockIdx.x * blockDim.x + threadIdx.x;
+  // a warp whose first unit is past the row has none inside (units come in
+  // whole groups of 8 lanes); the groups past the end stay for the shuffles
+  if ((u & ~31) >= (heads + 2 * c.kv_heads) * quads) return;
+  const int head = u / quads, at = u - head * quads;
+  const bool is_q = head < heads, is_k = !is_q && head < heads + c.kv_heads;
+  const bool some = head < heads + 2 * c.kv_heads;
+  const int h = is_q ? head : is_k ? head - heads : head - heads - c.kv_heads;
+  const int half = c.head_dim >> 1;
+  const int lane = threadIdx.x & 31;
+  for (int t = blockIdx.y; t < s.rows; t += gridDim.y) {
+    int seq, pos;
+    if (!kv_row(s, c.page, t, err, &seq, &pos)) continue;  // the same for the whole block
+    if (cos_t && pos >= table_rows) {
+      if (threadIdx.x == 0) kv_bad(err);
+      continue;
+    }
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (some) {
+      const float* src = is_q ? q + t * q_ld : is_k ? k + t * k_ld : v + t * v_ld;
+      const float4 y = reinterpret_cast<const float4*>(src + static_cast<size_t>(h) * c.head_dim)[at];
+      x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+      if (cos_t && (is_q || is_k)) {
+        // glc_rope's arithmetic: every product and sum rounded on its own
+        const float2 co = reinterpret_cast<const float2*>(cos_t + static_cast<size_t>(pos) * half)[at];
+        const float2 si = reinterpret_cast<const float2*>(sin_t + static_cast<size_t>(pos) * half)[at];
+        const float a0 = __fsub_rn(__fmul_rn(x[0], co.x), __fmul_rn(x[1], si.x));
+        const float b0 = __fadd_rn(__fmul_rn(x[0], si.x), __fmul_rn(x[1], co.x));
+        const float a1 = __fsub_rn(__fmul_rn(x[2], co.y), __fmul_rn(x[3], si.y));
+        const float b1 = __fadd_rn(__fmul_rn(x[2], si.y), __fmul_rn(x[3], co.y));
+        x[0] = a0, x[1] = b0, x[2] = a1, x[3] = b1;
+      }
+      if (is_q)
+        reinterpret_cast<float4*>(q_out + t * q_out_ld + static_cast<size_t>(h) * c.head_dim)[at] =
+            make_float4(x[0], x[1], x[2], x[3]);
+    }
+    // the element of largest magnitude among the 32, the first of equals, and
+    // whether all are finite; no early exit, so every lane takes the shuffles
+    float m = x[0];
+    bool fine = fabsf(x[0]) <= FLT_MAX;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      if (fabsf(x[i]) > fabsf(m)) m = x[i];
+      fine = fine && fabsf(x[i]) <= FLT_MAX;
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      const float pm = __shfl_xor_sync(~0u, m, o);
+      if (fabsf(pm) > fabsf(m) || (fabsf(pm) == fabsf(m) && (lane & o))) m = pm;
+    }
+    const unsigned all_fine = __ballot_sync(~0u, fine);
+    if (!some || is_q) continue;
+    const int index = pos / c.page, slot = pos - index * c.page;
+    const int page = kv_page(s, c.num_pages, seq, index, err);
+    if (page < 0) continue;
+    const bool nan = ((all_fine >> (lane & 24)) & 0xffu) != 0xffu;
+    const __half d16 = nan ? __ushort_as_half(0x7e00)
+                           : __float2half_rn(fminf(fmaxf(__fmul_rn(m, -0.125f), -65504.f), 65504.f));
+    const float d = __half2float(d16);
+    unsigned bits = 0x8888u;
+    if (!nan && d != 0.f) {
+      // the whole number nearest to the exact x / d: a first guess by the
+      // reciprocal, then its residual x - n d, which is exact (n d has 15 bits,
+      // and the difference lies on x's grid and below d), against d / 2
+      const float r = __frcp_rn(d), edge = 0.5f * fabsf(d);
+      bits = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float n = rintf(__fmul_rn(x[i], r));
+        n = fminf(fmaxf(n, -16.f), 16.f);
+        const float rest = fmaf(-n, d, x[i]);
+        const float step = (rest < 0.f) == (d < 0.f) ? 1.f : -1.f;
+        if (fabsf(rest) > edge || (fabsf(rest) == edge && (static_cast<int>(n) & 1))) n += step;
+        n = fminf(fmaxf(n, -8.f), 7.f);
+        bits |= static_cast<unsigned>(static_cast<int>(n) + 8) << (4 * i);
+      }
+    }
+    uint8_t* to = (is_k ? c.k : c.v) + (static_cast<size_t>(page) * c.kv_heads + h) * c.chunk;
+    reinterpret_cast<uint16_t*>(to + static_cast<size_t>(slot) * half)[at] = static_cast<uint16_t>(bits);
+    if ((lane & 7) == 0)
+      reinterpret_cast<__half*>(to + c.scales_at)[slot * (c.head_dim / KV_GROUP) + (at >> 3)] = d16;
+  }
+}
+
+// A thread reads 8 codes (4 bytes) and their scale and writes 8 floats.
+__global__ void __launch_bounds__(256)
+    kv_read_kernel(KvPools c, KvSeqs s, float* __restrict__ k, size_t k_ld, float* __restrict__ v, size_t v_ld,
+                   int* __restrict__ err) {
+  GLC_PDL_ENTRY();
+  const int eighths = c.head_dim >> 3;
+  int u = blockIdx.x * blockDim.x + threadIdx.x;
+  const int one = c.kv_heads * eighths;
+  // with one of k and v missing, the units are the other's alone
+  if (u >= one * ((k ? 1 : 0) + (v ? 1 : 0))) return;
+  const bool is_k = k && u < one;
+  if (k && !is_k) u -= one;
+  const int h = u / eighths, at = u - h * eighths;
+  for (int t = blockIdx.y; t < s.rows; t += gridDim.y) {
+    int seq, pos;
+    if (!kv_row(s, c.page, t, err, &seq, &pos)) continue;
+    const int index = pos / c.page, slot = pos - index * c.page;
+    const int page = kv_page(s, c.num_pages, seq, index, err);
+    if (page < 0) continue;
+    const uint8_t* from = (is_k ? c.k : c.v) + (static_cast<size_t>(page) * c.kv_heads + h) * c.chunk;
+    const unsigned w = reinterpret_cast<const unsigned*>(from + static_cast<size_t>(slot) * (c.head_dim >> 1))[at];
+    const float d = __half2float(
+        reinterpret_cast<const __half*>(from + c.scales_at)[slot * (c.head_dim / KV_GROUP) + (at >> 2)]);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(d, static_cast<float>(static_cast<int>((w >> (4 * i)) & 15u) - 8));
+    float4* to = reinterpret_cast<float4*>((is_k ? k + t * k_ld : v + t * v_ld) + static_cast<size_t>(h) * c.head_dim) +
+                 2 * at;
+    to[0] = make_float4(x[0], x[1], x[2], x[3]);
+    to[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// A block per row stripe: as many as fill the device a few times over.
+dim3 row_grid(const Context* ctx, int units, int rows) {
+  const int bx = (units + 255) / 256;
+  int by = (ctx->num_sms * 16 + bx - 1) / bx;
+  if (by > rows) by = rows;
+  if (by > 65535) by = 65535;
+  return dim3(bx, by);
+}
+
+int cache_check(const char* what, const glc_kv_cache* c, std::string* msg) {
+  auto no = [&](const char* why) {
+    *msg = std::string(what) + ": " + why;
+    return GLC_ERR_INVALID;
+  };
+  if (!c) return no("no cache given");
+  if (c->num_pages <= 0 || c->num_kv_heads <= 0) return no("num_pages and num_kv_heads must be positive");
+  if (c->page_size <= 0 || c->page_size % 16 || c->page_size > 65536)
+    return no("page_size must be a multiple of 16, at most 65536");
+  if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128) {
+    *msg = std::string(what) + ": head_dim must be 32, 64, 96 or 128";
+    return GLC_ERR_UNSUPPORTED;
+  }
+  return GLC_OK;
+}
+
+}  // namespace
+
+int kv_check(Context* ctx, const char* what, const glc_kv_cache* cache, const glc_kv_batch* batch) {
+  std::string msg;
+  const int rc = cache_check(what, cache, &msg);
+  if (rc) return ctx->fail(rc, msg);
+  auto no = [&](const char* why) { return ctx->fail(GLC_ERR_INVALID, std::string(what) + ": " + why); };
+  if (!cache->k || !cache->v || !aligned16(cache->k) || !aligned16(cache->v))
+    return no("the cache's pools must be 16-byte aligned device memory");
+  if (!batch) return no("no batch given");
+  if (batch->num_seqs < 0 || batch->num_rows < 0 || batch->max_pages <= 0) return no("bad batch sizes");
+  if (batch->num_seqs > 0 && (!batch->page_table || !batch->lens)) return no("page_table and lens must be given");
+  if (!batch->starts && batch->num_rows < batch->num_seqs)
+    return no("without starts, num_rows must be at least num_seqs");
+  if (static_cast<long long>(batch->max_pages) * cache->page_size > 0x7fffffff)
+    return no("max_pages * page_size must stay below 2^31");
+  return GLC_OK;
+}
+
+}  // namespace glc
+
+using glc::Context;
+
+extern "C" {
+
+int glc_kv_cache_bytes(const glc_kv_cache* cache, size_t* bytes) {
+  std::string msg;
+  if (!bytes) return GLC_ERR_INVALID;
+  const int rc = glc::cache_check("kv_cache_bytes", cache, &msg);
+  if (rc) {
+    glc::host_error() = msg;
+    return rc;
+  }
+  *bytes = static_cast<size_t>(cache->num_pages) * cache->num_kv_heads * glc::kv_pools(*cache).chunk;
+  return GLC_OK;
+}
+
+int glc_kv_append(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* batch, const float* q, int q_ld,
+                  float* q_out, int q_out_ld, int num_heads, const float* k, int k_ld, const float* v, int v_ld,
+                  const float* cos_t, const float* sin_t, int table_rows) {
+  if (!ctx) return GLC_ERR_INVALID;
+  Context* c = reinterpret_cast<Context*>(ctx);
+  int rc = glc::kv_check(c, "kv_append", cache, batch);
+  if (rc) return rc;
+  auto no = [&](const char* why) { return c->fail(GLC_ERR_INVALID, std::string("kv_append: ") + why); };
+  const long long kv_width = static_cast<long long>(cache->num_kv_heads) * cache->head_dim;
+  const long long q_width = static_cast<long long>(num_heads) * cache->head_dim;
+  if ((q == nullptr) != (q_out == nullptr)) return no("q and q_out must both be given, or neither");
+  if (q && num_heads <= 0) return no("num_heads must be positive");
+  if ((cos_t == nullptr) != (sin_t == nullptr)) return no("cos_t and sin_t must both be given, or neither");
+  if (cos_t && table_rows <= 0) return no("table_rows must be positive");
+  if (!k || !v) return no("k and v must be given");
+  if ((q && (q_ld < q_width || q_out_ld < q_width || ((q_ld | q_out_ld) & 3))) || k_ld < kv_width ||
+      v_ld < kv_width || ((k_ld | v_ld) & 3))
+    return no("row strides must be multiples of 4 and at least the row's width");
+  if (!glc::aligned16(q) || !glc::aligned16(q_out) || !glc::aligned16(k) || !glc::aligned16(v) ||
+      !glc::aligned16(cos_t) || !glc::aligned16(sin_t))
+    return no("pointers must be 16-byte aligned");
+  if (q_width + 2 * kv_width > (1 << 26)) return no("the rows are too wide");
+  if (batch->num_rows == 0 || batch->num_seqs == 0) return GLC_OK;
+  glc::DeviceScope on(c);
+  const int heads = q ? num_heads : 0;
+  const int units = (heads + 2 * cache->num_kv_heads) * (cache->head_dim / 4);
+  const double moved = static_cast<double>(batch->num_rows) *
+                       (8.0 * (q ? q_width : 0) + (8.0 + 9.0 / 8.0) * kv_width);
+  glc::ProfScope prof(c, glc::PROF_OTHER, moved, c->stream);
+  glc::launch_pdl(c, glc::kv_append_kernel, glc::row_grid(c, units, batch->num_rows), 256, 0, c->stream,
+                  glc::kv_pools(*cache), glc::kv_seqs(*batch), q, static_cast<size_t>(q_ld), q_out,
+                  static_cast<size_t>(q_out_ld), heads, k, static_cast<size_t>(k_ld), v, static_cast<size_t>(v_ld),
+                  cos_t, sin_t, table_rows, c->d_err);
+  GLC_LAUNCH_CHECK(c, "kv_append");
+  return GLC_OK;
+}
+
+int glc_kv_read(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* batch, float* k, int k_ld, float* v,
+                int v_ld) {
+  if (!ctx) return GLC_ERR_INVALID;
+  Context* c = reinterpret_cast<Context*>(ctx);
+  int rc = glc::kv_check(c, "kv_read", cache, batch);
+  if (rc) return rc;
+  auto no = [&](const char* why) { return c->fail(GLC_ERR_INVALID, std::string("kv_read: ") + why); };
+  const long long width = static_cast<long long>(cache->num_kv_heads) * cache->head_dim;
+  if (!k && !v) return no("k or v must be given");
+  if ((k && (k_ld < width || (k_ld & 3))) || (v && (v_ld < width || (v_ld & 3))))
+    return no("row strides must be multiples of 4 and at least the row's width");
+  if (!glc::aligned16(k) || !glc::aligned16(v)) return no("pointers must be 16-byte aligned");
+  if (width > (1 << 26)) return no("the rows are too wide");
+  if (batch->num_rows == 0 || batch->num_seqs == 0) return GLC_OK;
+  glc::DeviceScope on(c);
+  const int sides = (k ? 1 : 0) + (v ? 1 : 0);
+  const int units = sides * cache->num_kv_heads * (cache->head_dim / 8);
+  glc::ProfScope prof(c, glc::PROF_OTHER, static_cast<double>(batch->num_rows) * sides * width * (4.0 + 9.0 / 16.0),
+                      c->stream);
+  glc::launch_pdl(c, glc::kv_read_kernel, glc::row_grid(c, units, batch->num_rows), 256, 0, c->stream,
+                  glc::kv_pools(*cache), glc::kv_seqs(*batch), k, static_cast<size_t>(k_ld), v,
+                  static_cast<size_t>(v_ld), c->d_err);
+  GLC_LAUNCH_CHECK(c, "kv_read");
+  return GLC_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,260 @@
+// Where a token of the paged 4-bit key/value cache lies, which position of which
+// sequence a row of the operands is, and how the attention over the cache cuts
+// its work: the index arithmetic of kv_cache.cu and attention_kv.cu, for the
+// device and, so that it can be checked without one, for the host.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+
+#include "../../include/gollama_cuda.h"
+
+#if defined(__CUDACC__)
+#define KV_HD __host__ __device__ __forceinline__
+#else
+#define KV_HD inline
+#endif
+
+namespace glc {
+
+constexpr int KV_GROUP = 32;         // elements that share a scale
+constexpr int KV_BAD_ARGUMENT = 110; // GLC_DEV_BAD_ARGUMENT
+
+// glc_kv_cache with the sizes that follow from it.
+struct KvPools {
+  uint8_t* k;
+  uint8_t* v;
+  int num_pages, page, kv_heads, head_dim;
+  size_t chunk;   // bytes of one page of one head
+  int scales_at;  // of them, where the scales begin
+};
+struct KvSeqs {
+  const int* table;
+  const int* lens;
+  const int* starts;
+  int seqs, max_pages, rows;
+};
+
+inline KvPools kv_pools(const glc_kv_cache& c) {
+  KvPools p;
+  p.k = static_cast<uint8_t*>(c.k);
+  p.v = static_cast<uint8_t*>(c.v);
+  p.num_pages = c.num_pages;
+  p.page = c.page_size;
+  p.kv_heads = c.num_kv_heads;
+  p.head_dim = c.head_dim;
+  p.chunk = static_cast<size_t>(c.page_size) * (c.head_dim / 16) * 9;
+  p.scales_at = c.page_size * (c.head_dim / 2);
+  return p;
+}
+inline KvSeqs kv_seqs(const glc_kv_batch& b) {
+  return {b.page_table, b.lens, b.starts, b.num_seqs, b.max_pages, b.num_rows};
+}
+
+KV_HD void kv_bad(int* err) {
+#if defined(__CUDA_ARCH__)
+  atomicCAS(err, 0, KV_BAD_ARGUMENT);
+#else
+  if (*err == 0) *err = KV_BAD_ARGUMENT;
+#endif
+}
+
+// The rows [first, first + n) of sequence b that hold its new tokens, and its
+// length, held to what the operands and the table have; the error word is set
+// where they go beyond it.
+struct KvSpan {
+  int first, n, len;
+};
+KV_HD KvSpan kv_span(const KvSeqs& s, int page, int b, int* err) {
+  KvSpan r;
+  r.len = s.lens[b];
+  const int most = s.max_pages * page;  // below 2^31, checked by the host
+  if (r.len < 0 || r.len > most) {
+    kv_bad(err);
+    r.len = r.len < 0 ? 0 : most;
+  }
+  r.first = b;
+  r.n = 1;
+  if (s.starts) {
+    r.first = s.starts[b];
+    const int end = s.starts[b + 1];
+    if (r.first < 0 || end < r.first || end > s.rows) {
+      kv_bad(err);
+      r.first = 0;
+      r.n = 0;
+    } else {
+      r.n = end - r.first;
+    }
+  }
+  return r;
+}
+
+// Sequence and position of row t: false where the row belongs to no sequence
+// or its position is negative.  With starts, the last sequence that begins at
+// or before t.
+KV_HD bool kv_row(const KvSeqs& s, int page, int t, int* err, int* seq, int* pos) {
+  int b = t;
+  if (s.starts) {
+    int lo = 0, hi = s.seqs;  // starts[lo] <= t < starts[hi], when it holds at all
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s.starts[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+  } else if (t >= s.seqs) {
+    return false;
+  }
+  const KvSpan r = kv_span(s, page, b, err);
+  const int i = t - r.first;
+  if (i < 0 || i >= r.n) return false;
+  *seq = b;
+  *pos = r.len - r.n + i;
+  return *pos >= 0;
+}
+
+// Page `index` of sequence b; -1 (and the error word) where the table has none.
+KV_HD int kv_page(const KvSeqs& s, int num_pages, int b, int index, int* err) {
+  const int p = s.table[static_cast<size_t>(b) * s.max_pages + index];
+  if (p < 0 || p >= num_pages) {
+    kv_bad(err);
+    return -1;
+  }
+  return p;
+}
+
+// ---------------------------------------------------------------- attention
+
+constexpr int KV_RT = 8;   // query rows of an item
+constexpr int KV_WK = 32;  // keys of a warp's tile
+
+// The items of one KV head of a sequence.  A tile of KV_RT query rows holds the
+// heads of `toks` whole tokens, or, where a group has more heads than that, up
+// to KV_RT heads of one token (`parts` tiles per token).  Tile i sees the keys
+// of its last token, in units of `unit` keys, one at least (an item without
+// keys still writes its rows).
+struct KvRows {
+  int first, n, len, toks, parts, tiles;
+};
+KV_HD KvRows kv_rows(const KvSeqs& s, int page, int group, int b, int* err) {
+  const KvSpan r = kv_span(s, page, b, err);
+  KvRows w;
+  w.first = r.first;
+  w.n = r.n;
+  w.len = r.len;
+  w.toks = group < KV_RT ? KV_RT / group : 1;
+  w.parts = (group + KV_RT - 1) / KV_RT;
+  w.tiles = (r.n + w.toks - 1) / w.toks * w.parts;
+  return w;
+}
+// Keys seen by the last token of the run of tokens `run`.
+KV_HD int kv_run_keys(const KvRows& w, int run) {
+  const int last = (run + 1) * w.toks < w.n ? (run + 1) * w.toks : w.n;
+  const int keys = w.len - w.n + last;
+  return keys < 0 ? 0 : keys;
+}
+KV_HD int kv_run_units(const KvRows& w, int run, int unit) {
+  const int u = (kv_run_keys(w, run) + unit - 1) / unit;
+  return u < 1 ? 1 : u;
+}
+// One past the last run with as many units as `run` has: the runs' keys grow by
+// `toks` each, so equals are counted by a division, not one by one.
+KV_HD int kv_run_equals(const KvRows& w, int run, int units, int unit) {
+  const long long room = static_cast<long long>(units) * unit - (w.len - w.n);  // new tokens that fit
+  if (room >= w.n) return w.tiles / w.parts;
+  const int end = static_cast<int>(room / w.toks);
+  return end > run ? end : run + 1;
+}
+KV_HD long long kv_head_units(const KvRows& w, int unit) {
+  const int runs = w.tiles / w.parts;
+  long long sum = 0;
+  for (int i = 0; i < runs;) {
+    const int u = kv_run_units(w, i, unit), next = kv_run_equals(w, i, u, unit);
+    sum += static_cast<long long>(u) * (next - i) * w.parts;
+    i = next;
+  }
+  return sum;
+}
+// The tile in which unit `at` of a head lies: its first unit and its units.
+KV_HD int kv_find_tile(const KvRows& w, int unit, long long at, long long* first, int* units) {
+  const int runs = w.tiles / w.parts;
+  long long sum = 0;
+  for (int i = 0; i < runs;) {
+    const int u = kv_run_units(w, i, unit), next = kv_run_equals(w, i, u, unit);
+    const long long all = static_cast<long long>(u) * (next - i) * w.parts;
+    if (at < sum + all) {
+      const int skip = static_cast<int>((at - sum) / u);
+      *first = sum + static_cast<long long>(skip) * u;
+      *units = u;
+      return i * w.parts + skip;
+    }
+    sum += all;
+    i = next;
+  }
+  *first = sum;
+  *units = 1;
+  return 0;
+}
+
+// Of `total` units, CTA c of `ctas` (at most total) has [c total / ctas,
+// (c + 1) total / ctas): the CTA that has a unit.
+KV_HD int kv_cta_of(long long unit, long long total, long long ctas) {
+  return static_cast<int>(((unit + 1) * ctas - 1) / total);
+}
+
+// A tile of KV_WK keys in shared memory: codes of the keys, codes of the
+// values, scales of the keys, scales of the values.
+template <int HD>
+struct KvTile {
+  static constexpr int NB = HD / KV_GROUP;       // scales of a token, and 16-byte pieces of its codes
+  static constexpr int ROW = HD / 2;             // bytes of its codes
+  static constexpr int CODES = KV_WK * ROW;
+  static constexpr int SCALES = KV_WK * NB * 2;
+  static constexpr int BYTES = 2 * (CODES + SCALES);
+  static constexpr int CODE_PIECES = KV_WK * NB;  // of one side
+  static constexpr int SCALE_PIECES = 8 * NB;     // of both sides
+
+  // Byte of piece `ch` of the token in column `col` of the products.  The 16-byte
+  // pieces are swizzled so that a piece of 8 columns falls in 8 different quads of banks.
+  static KV_HD int code_at(int col, int ch) {
+    return col * ROW + 16 * (HD == 128 ? ch ^ ((col >> 1) & 3) : HD == 64 ? ch ^ ((col >> 2) & 1) : ch);
+  }
+  // Column of a token: of 16 tokens, those with bit 1 clear, then those with it
+  // set, so that a lane's two columns in each of two products are 4 tokens in a row.
+  static KV_HD int column(int token) {
+    return (token & 16) | ((token & 2) << 2) | ((token >> 1) & 6) | (token & 1);
+  }
+  // Piece id of the codes of a side: its token and where it comes from (relative
+  // to its token's codes) and goes to.
+  static KV_HD void code_piece(int id, int* token, int* from, int* to) {
+    const int tk = id / NB, ch = id - tk * NB;
+    *token = tk;
+    *from = 16 * ch;
+    *to = code_at(column(tk), ch);
+  }
+  // Piece id of the scales: its side, its group of 16 tokens, where it comes
+  // from (relative to the group's scales) and goes to (in the tile).
+  static KV_HD void scale_piece(int id, int* side, int* grp, int* from, int* to) {
+    *side = id / (4 * NB);
+    const int i = id - *side * 4 * NB;
+    *grp = i / (2 * NB);
+    *from = 16 * (i - *grp * 2 * NB);
+    *to = 2 * CODES + *side * SCALES + 16 * i;
+  }
+};
+
+// The page (index in the sequence) and the slot in it, both in groups of 16
+// tokens, of a group that walks a sequence in equal steps.
+struct KvWalk {
+  int index, slot;
+  KV_HD void start(int key, int page16) {
+    index = (key >> 4) / page16;
+    slot = (key >> 4) - index * page16;
+  }
+  KV_HD void advance(int step_index, int step_slot, int page16) {
+    index += step_index;
+    slot += step_slot;
+    if (slot >= page16) slot -= page16, ++index;
+  }
+};
+
+}  // namespace glc

@@ -1102,7 +1102,7 @@ int Trainer::train_step(const int64_t* in_dev, const int64_t* tg_dev, int B, int
     cudaMemcpy(&err, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost);
     if (err) {
       cudaMemset(ctx->d_err, 0, sizeof(int));
-      return ctx->fail(GLC_ERR_DEVICE, "train_step: a kernel's bounded wait ran out (device error " + std::to_string(err) + ")");
+      return ctx->fail(GLC_ERR_DEVICE, "train_step: device error " + std::to_string(err) + " (" + device_error_text(err) + ")");
     }
     std::memcpy(&last_norm, reinterpret_cast<char*>(loss_host) + 8, sizeof(double));
     if (loss_out) *loss_out = loss_host[0];

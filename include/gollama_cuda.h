@@ -360,6 +360,109 @@ GLC_API int glc_exp32(glc_ctx* ctx, const float* x, float* y, size_t n);
 /* addInplace (pkg/tensor/grad.go:200-204): dst += src. */
 GLC_API int glc_add_inplace(glc_ctx* ctx, float* dst, const float* src, size_t n);
 
+/* ------------------------------------------------------------------ generation
+ * What a decoding step needs beside the ops above: a paged key/value cache
+ * held in 4 bits, the attention of new tokens over it, and the choice of the
+ * next token.
+ *
+ * The cache is two device pools, keys and values, of num_pages pages of
+ * page_size tokens each.  Page p holds one chunk per KV head, and chunk
+ * (p, h) starts at byte (p * num_kv_heads + h) * page_size * head_dim * 9/16:
+ * first the codes of its tokens, head_dim/2 bytes each (element 2i in the low
+ * half of byte i, element 2i + 1 in the high half, as GLC_QTYPE_Q4_0 has
+ * them), then their scales, head_dim/32 IEEE halves each.  An element is
+ * scale * (code - 8): the arithmetic and the 4.5 bits per element of Q4_0,
+ * with codes and scales in arrays of their own so that both are read in
+ * aligned 16-byte pieces. */
+typedef struct glc_kv_cache {
+  void* k;          /* device, 16-byte aligned, glc_kv_cache_bytes each */
+  void* v;
+  int num_pages;
+  int page_size;    /* tokens per page: a multiple of 16, at most 65536 */
+  int num_kv_heads;
+  int head_dim;     /* 32, 64, 96 or 128 */
+} glc_kv_cache;
+
+/* The sequences of one call, in device memory (int32).  Sequence b has
+ * lens[b] tokens in the cache, the new ones included; its tokens p * page_size
+ * to (p + 1) * page_size - 1 are in page page_table[b * max_pages + p].  Its
+ * new tokens are its last ones: rows starts[b] to starts[b + 1] - 1 of the
+ * row-major operands hold them in order, so row starts[b] + i has position
+ * lens[b] - (starts[b + 1] - starts[b]) + i.  starts == NULL: one new token
+ * each, row b.  A new token with a negative position (lens[b] == 0 marks an
+ * idle slot of a batch) is not stored, and rows outside every sequence are
+ * left as they were.  Two new tokens must not share a slot of a page;
+ * sequences may share pages that no call writes.
+ *
+ * Values that only the device sees are checked there: a page index outside
+ * the pools, a length beyond max_pages * page_size, rows outside
+ * [0, num_rows) or a position beyond the rotation tables is neither read nor
+ * written, and the next glc_sync returns GLC_ERR_DEVICE. */
+typedef struct glc_kv_batch {
+  const int* page_table; /* [num_seqs][max_pages] */
+  const int* lens;       /* [num_seqs] */
+  const int* starts;     /* [num_seqs + 1], ascending, or NULL */
+  int num_seqs;
+  int max_pages;
+  int num_rows;          /* rows of the operands */
+} glc_kv_batch;
+
+/* Bytes of each of the two pools (host only; no reference counterpart: the
+ * reference's cache is float32 slices, pkg/model/attention.go:61-96). */
+GLC_API int glc_kv_cache_bytes(const glc_kv_cache* cache, size_t* bytes);
+/* Stores the new tokens' keys and values, rotating the keys on the way, and
+ * rotates the queries: the RoPE and cache update of Attention.Forward
+ * (pkg/model/attention.go:61-96, pkg/model/rope.go:96-126).
+ * q, q_out: [num_rows][num_heads * head_dim] (both NULL: no queries; q_out may
+ * equal q); k, v: [num_rows][num_kv_heads * head_dim].  *_ld are row strides
+ * in floats (multiples of 4), so the operands may be columns of one fused
+ * projection; pointers are 16-byte aligned.  cos_t/sin_t: [table_rows]
+ * [head_dim/2] of glc_rope_table on the device (both NULL: no rotation; q is
+ * copied).  The rotation is glc_rope's, bit for bit.  Of 32 elements x, e the
+ * one of largest magnitude (the first of equals): scale = half(e / -8), held
+ * to +-65504, and code = 8 + the whole number nearest to x / scale (ties to
+ * even) held to [-8, 7]; a scale of zero has codes 8; an infinity or a NaN
+ * among them makes the scale NaN, and all 32 read as NaN. */
+GLC_API int glc_kv_append(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* batch, const float* q, int q_ld,
+                          float* q_out, int q_out_ld, int num_heads, const float* k, int k_ld, const float* v,
+                          int v_ld, const float* cos_t, const float* sin_t, int table_rows);
+/* Reads the batch's new tokens back as the numbers they are stored as (with
+ * starts at every lens[b] rows: whole sequences), into k and v
+ * [num_rows][num_kv_heads * head_dim] (either may be NULL).  The inverse of
+ * glc_kv_append, with DequantizeQ4_0's arithmetic (pkg/quant/dequant.go:99-119). */
+GLC_API int glc_kv_read(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* batch, float* k, int k_ld,
+                        float* v, int v_ld);
+/* Attention of the new tokens over the cache (computeAttention,
+ * pkg/model/attention.go:113-206): o = softmax(q . k / sqrt(head_dim)) v over
+ * positions 0 to the token's own, query head h on KV head
+ * h / (num_heads / num_kv_heads).  q, o: [num_rows][num_heads * head_dim] with
+ * row strides in floats (multiples of 4); lse (nullable): [num_rows]
+ * [num_heads], the natural logarithm of the softmax's sum.  A token with no
+ * visible position (lens[b] == 0) gets o = 0 and lse = -infinity.  The
+ * products use the cache's exact values and q and the probabilities to 22
+ * bits, the sums are float32.  Deterministic.  Uses the context workspace. */
+GLC_API int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* batch, const float* q,
+                             int q_ld, int num_heads, float* o, int o_ld, float* lse);
+/* Draws one token per row of logits [rows][ld], the first vocab columns
+ * (Sampler, pkg/model/sampler.go, with the random numbers given): tokens in
+ * falling order of their logits (equal ones by index), the first top_k of
+ * them, of those the shortest prefix that holds top_p of their probability,
+ * of those the ones with at least min_p times the largest probability, where
+ * probabilities are proportional to exp(logit / temperature); then, in index
+ * order, the first token whose running sum of probability exceeds uniform *
+ * the kept sum.  Settings are one value per row in device memory; uniform in
+ * [0, 1).  A temperature that is not positive takes the largest logit; top_k
+ * <= 0, top_p >= 1 and min_p <= 0 keep all; top_p <= 0 and min_p >= 1 keep
+ * the first, and the equals of the first; any of top_k, top_p and min_p may be NULL.  A NaN
+ * counts as -infinity; -infinity is never drawn; where a row has nothing else
+ * its token is -1 and its logp -infinity.  logp (nullable): the natural
+ * logarithm of the drawn token's share of the kept probability.  Weights are
+ * whole numbers of 2^-42 of the largest, so that sums do not depend on their
+ * order.  vocab at most 393216. */
+GLC_API int glc_sample(glc_ctx* ctx, const float* logits, int ld, int rows, int vocab, const float* temperature,
+                       const int* top_k, const float* top_p, const float* min_p, const float* uniform,
+                       int64_t* tokens, float* logp);
+
 /* ------------------------------------------------------------------ model / trainer */
 #define GLC_SEMANTICS_REFERENCE 0 /* pkg/train exactly, quirks included */
 #define GLC_SEMANTICS_LLAMA 1     /* RoPE, GQA, attention backward, full RMSNorm backward, CE-seeded backward */

@@ -1,0 +1,207 @@
+// Test harness: the index arithmetic of the paged 4-bit cache and of the
+// attention over it (gollama_b200/csrc/kv_plan.h) walked on the host as the
+// kernels walk it, and a context without a device for the tests of refused
+// arguments.  Built by tests/test_kv_plan.py; never linked into the library.
+#include <algorithm>
+#include <cstring>
+#include <map>
+#include <set>
+#include <vector>
+
+#include "../../gollama_b200/csrc/glc_internal.h"
+#include "../../gollama_b200/csrc/kv_plan.h"
+
+using namespace glc;
+
+// A context whose calls can be refused (they return before they touch a
+// device); it is never destroyed through the library.
+extern "C" void* test_context() {
+  auto* c = new Context();
+  c->num_sms = 148;
+  return c;
+}
+extern "C" void test_context_free(void* c) { delete static_cast<Context*>(c); }
+
+namespace {
+
+// 0, or a number that names what went wrong
+template <int HD>
+int walk(const KvPools& c, const KvSeqs& s, int group, int warps, int grid, int* err) {
+  using Tile = KvTile<HD>;
+  const int unit = warps * KV_WK;
+  long long total = 0;
+  for (int b = 0; b < s.seqs; ++b) total += kv_head_units(kv_rows(s, c.page, group, b, err), unit) * c.kv_heads;
+  const long long ctas = std::min<long long>(total, grid);
+  const size_t pool = static_cast<size_t>(c.num_pages) * c.kv_heads * c.chunk;
+  // (sequence, head, tile) -> per key how often it was read; and who wrote it
+  std::map<std::vector<int>, std::vector<int>> seen;
+  std::map<std::vector<int>, std::vector<std::pair<int, int>>> parts;  // (cta, slot) of an item's parts
+  std::map<int, int> arrivals, needed;
+  std::set<std::vector<int>> whole;
+  for (int cta = 0; cta < ctas; ++cta) {
+    const long long begin = total * cta / ctas, end = total * (cta + 1) / ctas;
+    if (begin >= end) return 1;
+    for (long long x = begin; x < end; ++x)
+      if (kv_cta_of(x, total, ctas) != cta) return 2;
+    long long at_b = 0, units_b = 0;
+    int b = 0;
+    for (; b < s.seqs; ++b) {
+      units_b = kv_head_units(kv_rows(s, c.page, group, b, err), unit) * c.kv_heads;
+      if (begin < at_b + units_b) break;
+      at_b += units_b;
+    }
+    if (b == s.seqs) return 3;
+    KvRows w = kv_rows(s, c.page, group, b, err);
+    const long long per_head = units_b / c.kv_heads;
+    int h = static_cast<int>((begin - at_b) / per_head);
+    long long item_at;
+    int units;
+    int tile = kv_find_tile(w, unit, begin - at_b - h * per_head, &item_at, &units);
+    item_at += at_b + h * per_head;
+    const int page16 = c.page >> 4, step_pages = (unit / 16) / page16, step_slot = (unit / 16) % page16;
+    for (long long at = begin; at < end;) {
+      const long long item_end = item_at + units, seg_end = std::min(item_end, end);
+      if (at < item_at || at >= item_end) return 4;
+      const int run_at = tile / w.parts, part_at = tile - run_at * w.parts;
+      const int keys = kv_run_keys(w, run_at);
+      const int key0 = static_cast<int>(at - item_at) * unit;
+      const int key1 = std::min(static_cast<int>(seg_end - item_at) * unit, keys);
+      const int tok0 = run_at * w.toks, head0 = part_at * KV_RT;
+      const int width = group < KV_RT ? group : std::min(group - head0, KV_RT);
+      const int rows = std::min(w.n - tok0, w.toks) * width;
+      if (rows < 1 || rows > KV_RT || head0 + width > group) return 5;
+      auto& count = seen[{b, h, tile}];
+      count.resize(keys);
+      for (int warp = 0; warp < warps; ++warp) {
+        KvWalk g[2];
+        int next = key0 + warp * KV_WK;
+        for (int i = 0; i < 2; ++i) g[i].start(next + 16 * i, page16);
+        for (int key = next; key < key1; key += unit) {
+          std::set<int> to_all;
+          size_t base[2] = {0, 0};
+          bool ok[2];
+          for (int i = 0; i < 2; ++i) {
+            const int k = key + 16 * i;
+            ok[i] = false;
+            if (k < key1) {
+              if (g[i].index != k / c.page || g[i].slot != k % c.page / 16) return 6;
+              if (g[i].index >= s.max_pages) return 7;
+              const int p = kv_page(s, c.num_pages, b, g[i].index, err);
+              ok[i] = p >= 0;
+              base[i] = (ok[i] ? static_cast<size_t>(p) * c.kv_heads * c.chunk : 0) + h * c.chunk;
+            }
+          }
+          for (int id = 0; id < Tile::CODE_PIECES; ++id) {
+            int tk, from, to;
+            Tile::code_piece(id, &tk, &from, &to);
+            const int i = tk >> 4;
+            if (to < 0 || to + 16 > Tile::CODES || to % 16 || !to_all.insert(to).second) return 8;
+            if (Tile::column(tk) / 16 != i) return 9;
+            if (!ok[i] || key + tk >= key1) continue;
+            const size_t src = base[i] + static_cast<size_t>(g[i].slot * 16 + (tk & 15)) * Tile::ROW + from;
+            if (src + 16 > pool || src % 16) return 10;
+            if ((src - base[i]) + 16 > static_cast<size_t>(c.scales_at)) return 11;
+            if (from == 0) ++count[key + tk];
+          }
+          for (int id = 0; id < Tile::SCALE_PIECES; ++id) {
+            int side, grp, from, to;
+            Tile::scale_piece(id, &side, &grp, &from, &to);
+            if (to < 2 * Tile::CODES || to + 16 > Tile::BYTES || !to_all.insert(to).second) return 12;
+            if (!ok[grp]) continue;
+            const size_t src = base[grp] + c.scales_at + static_cast<size_t>(g[grp].slot) * 32 * Tile::NB + from;
+            if (src + 16 > base[grp] + c.chunk || src + 16 > pool || src % 16) return 13;
+          }
+          for (int i = 0; i < 2; ++i) g[i].advance(step_pages, step_slot, page16);
+        }
+      }
+      if (at == item_at && seg_end == item_end) {
+        if (!whole.insert({b, h, tile}).second) return 14;
+      } else {
+        const int first = kv_cta_of(item_at, total, ctas), last = kv_cta_of(item_end - 1, total, ctas);
+        parts[{b, h, tile}].push_back({cta, at == item_at ? 1 : 0});
+        if ((cta == first) != (at == item_at) || cta < first || cta > last) return 15;
+        ++arrivals[first];
+        needed[first] = last - first + 1;
+      }
+      at = seg_end;
+      if (at < end) {
+        item_at = item_end;
+        if (++tile == w.tiles) {
+          tile = 0;
+          if (++h == c.kv_heads) {
+            h = 0;
+            do {
+              if (++b >= s.seqs) return 16;
+              w = kv_rows(s, c.page, group, b, err);
+            } while (w.tiles == 0);
+          }
+        }
+        units = kv_run_units(w, tile / w.parts, unit);
+      }
+    }
+  }
+  for (auto& a : arrivals)
+    if (a.second != needed[a.first]) return 17;
+  for (auto& p : parts) {
+    if (whole.count(p.first)) return 18;
+    std::set<std::pair<int, int>> distinct(p.second.begin(), p.second.end());
+    if (distinct.size() != p.second.size()) return 19;
+  }
+  // every item once, every key of it that has a page once
+  for (int b = 0; b < s.seqs; ++b) {
+    const KvRows w = kv_rows(s, c.page, group, b, err);
+    int covered = 0;
+    for (int h = 0; h < c.kv_heads; ++h)
+      for (int tile = 0; tile < w.tiles; ++tile) {
+        const std::vector<int> id{b, h, tile};
+        if (!whole.count(id) && !parts.count(id)) return 20;
+        const auto& count = seen[id];
+        for (size_t k = 0; k < count.size(); ++k) {
+          const int p = s.table[static_cast<size_t>(b) * s.max_pages + k / c.page];
+          if (count[k] != (p >= 0 && p < c.num_pages ? 1 : 0)) return 21;
+        }
+      }
+    for (int i = 0; i < w.tiles; i += w.parts) covered += std::min(w.toks, w.n - i / w.parts * w.toks);
+    if (covered != w.n) return 22;
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int kv_walk(const glc_kv_cache* cache, const glc_kv_batch* batch, int group, int grid, int* err) {
+  const KvPools c = kv_pools(*cache);
+  const KvSeqs s = kv_seqs(*batch);
+  switch (c.head_dim) {
+    case 32: return walk<32>(c, s, group, 16, grid, err);
+    case 64: return walk<64>(c, s, group, 16, grid, err);
+    case 96: return walk<96>(c, s, group, 12, grid, err);
+    case 128: return walk<128>(c, s, group, 12, grid, err);
+  }
+  return -1;
+}
+
+// Rows of kv_append and kv_read: sequence and position of each (-1: none).
+extern "C" void kv_rows_of(const glc_kv_cache* cache, const glc_kv_batch* batch, int* seq, int* pos, int* err) {
+  const KvSeqs s = kv_seqs(*batch);
+  for (int t = 0; t < s.rows; ++t) {
+    seq[t] = -1;
+    pos[t] = -1;
+    int b, p;
+    if (kv_row(s, cache->page_size, t, err, &b, &p)) {
+      seq[t] = b;
+      pos[t] = p;
+    }
+  }
+}
+
+// Quads of banks that 8 columns of a piece fall in (8: no conflict).
+extern "C" int kv_bank_quads(int hd, int col0, int ch) {
+  std::set<int> quads;
+  for (int i = 0; i < 8; ++i) {
+    const int at = hd == 32 ? KvTile<32>::code_at(col0 + i, ch) : hd == 64 ? KvTile<64>::code_at(col0 + i, ch)
+                   : hd == 96 ? KvTile<96>::code_at(col0 + i, ch) : KvTile<128>::code_at(col0 + i, ch);
+    quads.insert(at / 16 % 8);
+  }
+  return static_cast<int>(quads.size());
+}
