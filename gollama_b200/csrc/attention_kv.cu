@@ -6,22 +6,25 @@
 //   s_j = q . k_j * log2(e) / sqrt(hd),  m' = max(m, max s_j),
 //   p_j = 2^(s_j - m'),  l = l 2^(m - m') + sum p_j,  o = o 2^(m - m') + sum p_j v_j.
 //
-// A code of the cache is a whole number below 16, so as the low mantissa bits
-// of a half it is exact (n 2^-24; in the next nibble n 2^-20), and one AND
-// makes two matrix operands of it: nothing is dequantized.  The other operand
-// is float32 split into two halves (hi + lo, 22 bits), which share the 16 rows
-// of one m16n8k16 product: rows 0-7 hold hi and rows 8-15 lo of 8 query rows.
-// The scales enter in float32: a key's after the product over its 32 elements
-// (one product pair per block of 32), a value's before it, on the
-// probabilities.  The "- 8" is a constant per query and block (the initial
-// value of q . n) and a sum of the scaled probabilities per block of values.
+// Codes become matrix operands without being scaled: two of them OR'ed into the
+// mantissas of two halves are 1024 + n (or 1024 + 16 n), and one packed addition
+// (or fused multiply-add) makes n - 8 of them, exactly.  (The bare bits would be
+// the subnormal half n 2^-24, one instruction less, but the products align
+// subnormal operands by their exponent field and lose 7 bits of the sum: errors
+// of 1e-5 instead of 5e-7 were measured.)  Keys and values are the 16-row
+// operand of m16n8k16 products, 8 query rows the other, which is float32 split
+// into two halves (hi + lo, 22 bits) and goes through in two products with one
+// accumulator.  The scales enter outside the products: a key's in float32 after
+// the product over its 32 elements, a value's before it, on the probabilities'
+// halves (hi' = hi d, lo' = lo d + the exact rest fma(hi, d, -hi')).
 //
-// Query rows are (new token, head of the KV head's group), RT = 8 at a time.
-// A work item is a sequence, a KV head and such a tile of rows; its keys are
-// cut into units, the units of all items laid end to end and dealt out evenly
-// to one CTA per SM, so that lengths may differ and a single long sequence
-// fills the device.  Items cut between CTAs leave partial (m, l, o); the CTA
-// that arrives last joins them in the order of their keys.
+// A work item is a sequence, a KV head and 8 query rows ((new token, head of
+// the KV head's group) pairs); its keys are cut into units, the units of all
+// items laid end to end and dealt out evenly over the CTAs, so that lengths
+// may differ and a single long sequence fills the device.  Each warp walks its
+// own tiles of 32 keys with its own ring of asynchronous copies; the warps of
+// a CTA join at the end of an item.  Items cut between CTAs leave partial
+// (m, l, o); the CTA that arrives last joins them in the order of their keys.
 #include <cfloat>
 
 #include "kv_cache.cuh"
@@ -29,8 +32,7 @@
 namespace glc {
 namespace {
 
-constexpr int RT = KV_RT, WK = KV_WK;
-constexpr int STAGES = 3; // tiles of a warp's ring
+constexpr int WK = KV_WK;
 
 struct AttnKv {
   KvPools c;
@@ -47,18 +49,24 @@ struct AttnKv {
   int* err;
 };
 
-template <int HD>
+template <int HD, int W>
 struct Shape {
   using Tile = KvTile<HD>;
   static constexpr int NB = Tile::NB;
-  static constexpr int WARPS = HD >= 96 ? 12 : 16;
-  static constexpr int FSCALES = 2 * NB * WK * 4;  // a tile's scales as floats
-  static constexpr int RING = WARPS * (STAGES * Tile::BYTES + FSCALES);
-  // the warps' (o, m, l) at the end of an item, in the ring's place
-  static constexpr int JOIN = WARPS * RT * (HD + 2) * 4;
-  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+  static constexpr int RT = 8;  // query rows of an item
+  static constexpr int STAGES = HD >= 96 ? 2 : 3;
+  static constexpr int PER_SM = 16 / W;  // CTAs: 16 warps of 128 registers
+  static constexpr int KS = NB == 3 ? 4 : NB;  // floats of a key's scales
+  static constexpr int SCALES = WK * KS * 4 + NB * WK * 2;  // a tile's scales as the products take them
+  static constexpr int WARP = STAGES * Tile::BYTES + SCALES;
+  static constexpr int JOIN = W * RT * (HD + 2) * 4;  // the warps' (o, m, l), in the rings' place
+  static constexpr int SMEM = W * WARP > JOIN ? W * WARP : JOIN;
+  static_assert(WARP % 16 == 0, "rings start on 16 bytes");
 };
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool some) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16 : 0) : "memory");
 }
@@ -77,32 +85,46 @@ __device__ __forceinline__ void ldsm4t(uint32_t* r, uint32_t at) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(at));
 }
-__device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// d = a b + c
+__device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1, const float* c) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 halves(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 // (x0, x1) as halves hi + lo: 22 bits where lo is a normal half
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t* hi, uint32_t* lo) {
-  const __half2 h = __floats2half2_rn(x0, x1);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
-  *hi = *reinterpret_cast<const uint32_t*>(&h);
-  *lo = *reinterpret_cast<const uint32_t*>(&l);
+__device__ __forceinline__ void split2(float x0, float x1, __half2* hi, __half2* lo) {
+  *hi = __floats2half2_rn(x0, x1);
+  const float2 f = __half22float2(*hi);
+  *lo = __floats2half2_rn(x0 - f.x, x1 - f.y);
+}
+// codes less 8 of the low nibbles of x's halves, and of the next ones
+__device__ __forceinline__ uint32_t codes0(uint32_t x) {
+  return bits(__hadd2(halves((x & 0x000f000fu) | 0x64006400u), halves(0xe408e408u)));  // - 1032
+}
+__device__ __forceinline__ uint32_t codes1(uint32_t x) {
+  return bits(__hfma2(halves((x & 0x00f000f0u) | 0x64006400u), halves(0x2c002c00u), halves(0xd480d480u)));  // / 16 - 72
 }
 
-template <int HD>
-__global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(const AttnKv a) {
+template <int HD, int W>
+__global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_kernel(const AttnKv a) {
   GLC_PDL_ENTRY();
-  using S = Shape<HD>;
+  using S = Shape<HD, W>;
   using Tile = KvTile<HD>;
-  constexpr int NB = S::NB, W = S::WARPS, UNIT = W * WK;
+  constexpr int NB = S::NB, RT = S::RT, STAGES = S::STAGES, UNIT = W * WK;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long sum_s[W];
   __shared__ long long at_s[2];
@@ -117,7 +139,7 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
   const int b0 = tid * run < a.s.seqs ? tid * run : a.s.seqs;
   const int b1 = b0 + run < a.s.seqs ? b0 + run : a.s.seqs;
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += kv_head_units(kv_rows(a.s, a.c.page, a.group, b, a.err), UNIT) * a.c.kv_heads;
+  for (int b = b0; b < b1; ++b) mine += kv_head_units(kv_rows(a.s, a.c.page, a.group, RT, b, a.err), UNIT) * a.c.kv_heads;
   long long upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -139,7 +161,7 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
   if (upto - mine <= begin && begin < upto) {
     long long at = upto - mine;
     for (int b = b0; b < b1; ++b) {
-      const long long u = kv_head_units(kv_rows(a.s, a.c.page, a.group, b, a.err), UNIT) * a.c.kv_heads;
+      const long long u = kv_head_units(kv_rows(a.s, a.c.page, a.group, RT, b, a.err), UNIT) * a.c.kv_heads;
       if (begin < at + u) {
         seq_s = b;
         at_s[0] = at;
@@ -152,7 +174,7 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
   __syncthreads();
   int b = seq_s;
   if (b < 0) return;
-  KvRows w = kv_rows(a.s, a.c.page, a.group, b, a.err);
+  KvRows w = kv_rows(a.s, a.c.page, a.group, RT, b, a.err);
   long long per_head = at_s[1] / a.c.kv_heads;
   int h = static_cast<int>((begin - at_s[0]) / per_head);
   int units = 1;
@@ -160,8 +182,9 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
   int tile = kv_find_tile(w, UNIT, begin - at_s[0] - h * per_head, &item_at, &units);
   item_at += at_s[0] + h * per_head;
 
-  uint8_t* ring = smem + warp * (STAGES * Tile::BYTES);
-  float* fsc = reinterpret_cast<float*>(smem + W * STAGES * Tile::BYTES + warp * S::FSCALES);
+  uint8_t* ring = smem + warp * S::WARP;
+  float* kscale = reinterpret_cast<float*>(ring + STAGES * Tile::BYTES);            // [key][KS]
+  __half* vscale = reinterpret_cast<__half*>(ring + STAGES * Tile::BYTES + WK * S::KS * 4);  // [block][t][8 keys][pair]
   const uint32_t ring_u = smem_u32(ring);
   const int page16 = a.c.page >> 4;
   // a warp's tiles lie UNIT keys apart
@@ -177,68 +200,12 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
     int key1 = static_cast<int>(seg_end - item_at) * UNIT;
     if (key1 > keys) key1 = keys;
 
-    // the tile's first token and head, its rows, and this thread's row g (the
-    // rows past the last repeat row 0 and are not written)
+    // the tile's first token and head, and its rows (those past the last repeat
+    // row 0 and are not written)
     const int tok0 = run_at * w.toks, head0 = part_at * RT;
     const int width = a.group < RT ? a.group : a.group - head0 < RT ? a.group - head0 : RT;  // heads of a token
     const int rows = (w.n - tok0 < w.toks ? w.n - tok0 : w.toks) * width;
-    const int my_row = g < rows ? g : 0, my_tok = tok0 + my_row / width, my_head = head0 + my_row % width;
-    const int last_key = w.len - w.n + my_tok;  // the last key this row sees
-    const float* qp =
-        a.q + static_cast<size_t>(w.first + my_tok) * a.q_ld + static_cast<size_t>(h * a.group + my_head) * HD;
-    uint32_t qf[NB][2][4];
-    float base[NB][2];  // -8 times the sum of q over a block, of hi and of lo
-    float rs;           // what a product is short of s: the row's power of two, units of the codes, scale2
-    {
-      float x[NB][8], top = 0.f;
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const float4 u = *reinterpret_cast<const float4*>(qp + 32 * i + 8 * t);
-        const float4 v = *reinterpret_cast<const float4*>(qp + 32 * i + 8 * t + 4);
-        x[i][0] = u.x, x[i][1] = u.y, x[i][2] = u.z, x[i][3] = u.w;
-        x[i][4] = v.x, x[i][5] = v.y, x[i][6] = v.z, x[i][7] = v.w;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i][j]));
-      }
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-      // the row's largest magnitude goes to [2^13, 2^14); subnormal rows stay as they are
-      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-      e = e < -100 ? -100 : e > 126 ? 126 : e;
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
-      rs = a.scale2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * 2048.f;  // 2^(e - 13 + 24)
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        // code pairs (0,4), (2,6) of 8 count n 2^-24, pairs (1,5), (3,7) n 2^-20
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] *= up * (j & 1 ? 0.0625f : 1.f);
-        split2(x[i][0], x[i][4], &qf[i][0][0], &qf[i][0][1]);
-        split2(x[i][1], x[i][5], &qf[i][0][2], &qf[i][0][3]);
-        split2(x[i][2], x[i][6], &qf[i][1][0], &qf[i][1][1]);
-        split2(x[i][3], x[i][7], &qf[i][1][2], &qf[i][1][3]);
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816(d, qf[i][0], 0x80088008u, 0x80808080u);
-        mma16816(d, qf[i][1], 0x80088008u, 0x80808080u);
-        base[i][0] = d[0];
-        base[i][1] = d[2];
-      }
-    }
-
-    float acc[NB][4][4];
-    float vsum[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      vsum[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    // probabilities times value scales are held at 2^vexp times their size, so
-    // that the largest lies in the halves' range and lo is a normal half
-    int vexp = 0;
-    uint32_t vtop = 0;  // largest scale (bits) that vexp allows
+    auto row_token = [&](int r) { return tok0 + (r < rows ? r : 0) / width; };
 
     // the two groups of 16 tokens of the warp's next tile, and their pages
     KvWalk walk[2];
@@ -259,23 +226,29 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
         const bool ok0 = page[0] >= 0, ok1 = page[1] >= 0;
         const size_t f0 = (ok0 ? page[0] * page_bytes : 0) + head_at;
         const size_t f1 = (ok1 ? page[1] * page_bytes : 0) + head_at;
+        const bool full = next + WK <= key1 && ok0 && ok1;
 #pragma unroll
         for (int j = 0; j < Tile::CODE_PIECES / 32; ++j) {
-          int token, from, at;
-          Tile::code_piece(lane + 32 * j, &token, &from, &at);
+          int token, from, at_;
+          Tile::code_piece(lane + 32 * j, &token, &from, &at_);
           const bool hi = token >= 16;
           const size_t src =
               (hi ? f1 : f0) + static_cast<size_t>((hi ? walk[1].slot : walk[0].slot) * 16 + (token & 15)) * Tile::ROW + from;
-          const bool some = (hi ? ok1 : ok0) && next + token < key1;
-          copy16(to + at, a.c.k + src, some);
-          copy16(to + Tile::CODES + at, a.c.v + src, some);
+          if (full) {
+            copy16(to + at_, a.c.k + src);
+            copy16(to + Tile::CODES + at_, a.c.v + src);
+          } else {
+            const bool some = (hi ? ok1 : ok0) && next + token < key1;
+            copy16(to + at_, a.c.k + src, some);
+            copy16(to + Tile::CODES + at_, a.c.v + src, some);
+          }
         }
         if (lane < Tile::SCALE_PIECES) {
-          int side, grp, from, at;
-          Tile::scale_piece(lane, &side, &grp, &from, &at);
+          int side, grp, from, at_;
+          Tile::scale_piece(lane, &side, &grp, &from, &at_);
           const size_t src = (grp ? f1 : f0) + a.c.scales_at +
                              static_cast<size_t>(grp ? walk[1].slot : walk[0].slot) * (32 * NB) + from;
-          copy16(to + at, (side ? a.c.v : a.c.k) + src, grp ? ok1 : ok0);
+          copy16(to + at_, (side ? a.c.v : a.c.k) + src, grp ? ok1 : ok0);
         }
         next += UNIT;
 #pragma unroll
@@ -289,159 +262,245 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
+    // ---- the queries as operands: lane (g, t) holds elements 8t .. 8t + 7 of
+    // each block of row g, and of columns 2t and 2t + 1 what goes by query
+    uint32_t qf[NB][2][4];  // per block and half of it: hi, hi, lo, lo
+    float rs[2];            // what a product is short of s: the row's power of two and scale2
+    int last_key[2];        // the last key the row sees
+    {
+      const int my_row = g < rows ? g : 0, my_tok = tok0 + my_row / width, my_head = head0 + my_row % width;
+      const float* qp =
+          a.q + static_cast<size_t>(w.first + my_tok) * a.q_ld + static_cast<size_t>(h * a.group + my_head) * HD;
+      float x[NB][8], top = 0.f;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const float4 u = *reinterpret_cast<const float4*>(qp + 32 * i + 8 * t);
+        const float4 v = *reinterpret_cast<const float4*>(qp + 32 * i + 8 * t + 4);
+        x[i][0] = u.x, x[i][1] = u.y, x[i][2] = u.z, x[i][3] = u.w;
+        x[i][4] = v.x, x[i][5] = v.y, x[i][6] = v.z, x[i][7] = v.w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i][j]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+      // the row's largest magnitude goes to [2^13, 2^14)
+      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+      e = e < -100 ? -100 : e > 126 ? 126 : e;
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
+      const float my_rs = a.scale2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * 0.0001220703125f;  // 2^(e - 13)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        rs[i] = __shfl_sync(~0u, my_rs, 4 * (2 * t + i));
+        last_key[i] = w.len - w.n + row_token(2 * t + i);
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] *= up;
+        // in the order in which the codes of 8 elements come apart: (0,4), (1,5); (2,6), (3,7)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          __half2 h0, l0, h1, l1;
+          split2(x[i][2 * j], x[i][2 * j + 4], &h0, &l0);
+          split2(x[i][2 * j + 1], x[i][2 * j + 5], &h1, &l1);
+          qf[i][j][0] = bits(h0), qf[i][j][1] = bits(h1), qf[i][j][2] = bits(l0), qf[i][j][3] = bits(l1);
+        }
+      }
+    }
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+
+    // rows: elements 4g + e of a block, columns: queries; [..][j][0..1] is e = 2j, [2..3] e = 2j + 1
+    float acc[NB][2][4];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[i][j][x] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    // probabilities are held at 2^PEXP and value scales at 2^vexp times their
+    // size: their products stay below 2^15, and lo and lo' are normal halves
+    // where they matter
+    constexpr int PEXP = 8;
+    int vexp = 0;
+    uint32_t vtop = 0;  // largest scale (bits) that vexp allows
+
     int stage = 0;
     for (int key = key0 + warp * WK; key < key1; key += UNIT) {
       copies_wait<STAGES - 2>();
       __syncwarp();  // the tile is there for all lanes, and all are done with the last one's stage
       fetch(stage == 0 ? STAGES - 1 : stage - 1);
       const uint32_t from = ring_u + stage * Tile::BYTES;
+      bool odd_scale;  // some value scale is infinite or not a number
       {
-        // lane = key: its scales as floats, zero behind the last key
+        // lane = key: its scales, zero behind the last key
         const __half* ks = reinterpret_cast<const __half*>(ring + stage * Tile::BYTES + 2 * Tile::CODES) + lane * NB;
         const __half* vs = ks + WK * NB;
         const bool some = key + lane < key1;
         uint32_t big = 0;
-        float kf[NB], vf[NB];
+        __half vh[NB];
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          const uint32_t vb = some ? __half_as_ushort(vs[i]) : 0u;
-          kf[i] = some ? __half2float(ks[i]) : 0.f;
-          vf[i] = __half2float(__ushort_as_half(static_cast<unsigned short>(vb)));
-          const uint32_t mag = vb & 0x7fffu;
+          kscale[lane * S::KS + i] = some ? __half2float(ks[i]) : 0.f;
+          vh[i] = some ? vs[i] : __ushort_as_half(0);
+          const uint32_t mag = __half_as_ushort(vh[i]) & 0x7fffu;
           big = big > mag ? big : mag;
         }
         big = __reduce_max_sync(~0u, big);
+        odd_scale = big > 0x7bffu;
         if (big > vtop) {  // the same for the whole warp
-          if (big > 0x7bffu) big = 0x7bffu;
-          // the largest scale to [2^12, 2^13): room for scales four times as large
+          if (odd_scale) big = 0x7bffu;
+          // the largest scale to [2^4, 2^5): room for scales four times as large
           const int e = big < 0x400u ? -15 : static_cast<int>(big >> 10) - 15;
-          const int now = 12 - e;
+          const int now = 4 - e;
           const float by = vtop ? __uint_as_float(static_cast<uint32_t>(127 + now - vexp) << 23) : 0.f;
 #pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            vsum[i] *= by;
+          for (int i = 0; i < NB; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
               for (int x = 0; x < 4; ++x) acc[i][j][x] *= by;
-          }
           vexp = now;
           vtop = e + 3 > 15 ? 0x7fffu : (static_cast<uint32_t>(e + 3 + 15) << 10) - 1;
         }
         const float up = __uint_as_float(static_cast<uint32_t>(127 + vexp) << 23);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          fsc[i * WK + lane] = kf[i];
-          fsc[(NB + i) * WK + lane] = vf[i] * up;
-        }
+        for (int i = 0; i < NB; ++i)
+          vscale[((i * 4 + ((lane >> 1) & 3)) * 4 + (lane >> 3)) * 2 + (lane & 1)] =
+              __float2half_rn(__half2float(vh[i]) * up);
       }
       __syncwarp();
 
-      // ---- s: tiles of 8 keys; column pair t of tiles 2j and 2j + 1 is keys 16 j + 4 t .. + 3
-      float s[4][2];
+      // ---- s of keys 16 j + g (x = 0, 1: queries 2t, 2t + 1) and 16 j + 8 + g (x = 2, 3)
+      float s[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) s[2 * j + i][0] = s[2 * j + i][1] = 0.f;
-        constexpr int PAIRS = (NB * 2 + 3) / 4;  // ldmatrix x4 per 16 keys
+        constexpr int PAIRS = (NB * 2 + 3) / 4;  // ldmatrix x4 per 16 keys: (8 keys, block) matrices
         uint32_t kw[PAIRS][4];
 #pragma unroll
         for (int p = 0; p < PAIRS; ++p) {
-          // matrix mi: tile (of 8 keys) and block of 32 elements
           const int mi = p * 4 + (lane >> 3);
           const int tl = mi / NB < 2 ? mi / NB : 0, bl = mi / NB < 2 ? mi % NB : 0;
-          const int row = 16 * j + 8 * tl + (lane & 7);
-          ldsm4(kw[p], from + Tile::code_at(row, bl));
+          ldsm4(kw[p], from + Tile::code_at(16 * j + 8 * tl + (lane & 7), bl));
+        }
+        float d0[4], d1[4];
+        if constexpr (NB >= 3) {
+          *reinterpret_cast<float4*>(d0) = *reinterpret_cast<const float4*>(kscale + (16 * j + g) * 4);
+          *reinterpret_cast<float4*>(d1) = *reinterpret_cast<const float4*>(kscale + (16 * j + 8 + g) * 4);
+        } else if constexpr (NB == 2) {
+          *reinterpret_cast<float2*>(d0) = *reinterpret_cast<const float2*>(kscale + (16 * j + g) * 2);
+          *reinterpret_cast<float2*>(d1) = *reinterpret_cast<const float2*>(kscale + (16 * j + 8 + g) * 2);
+        } else {
+          d0[0] = kscale[16 * j + g];
+          d1[0] = kscale[16 * j + 8 + g];
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          const float4 d = *reinterpret_cast<const float4*>(fsc + i * WK + 16 * j + 4 * t);
+          const uint32_t x = kw[i >> 2][i & 3], y = kw[(NB + i) >> 2][(NB + i) & 3], xs = x >> 8, ys = y >> 8;
+          const uint32_t a0 = codes0(x), a1 = codes0(y), a2 = codes1(x), a3 = codes1(y);
+          const uint32_t e0 = codes0(xs), e1 = codes0(ys), e2 = codes1(xs), e3 = codes1(ys);
+          float c[4];
+          mma16816(c, a0, a1, a2, a3, qf[i][0][0], qf[i][0][1], zero);
+          mma16816(c, a0, a1, a2, a3, qf[i][0][2], qf[i][0][3], c);
+          mma16816(c, e0, e1, e2, e3, qf[i][1][0], qf[i][1][1], c);
+          mma16816(c, e0, e1, e2, e3, qf[i][1][2], qf[i][1][3], c);
 #pragma unroll
-          for (int tl = 0; tl < 2; ++tl) {
-            const int mi = tl * NB + i;
-            const uint32_t x = kw[mi >> 2][mi & 3], y = x >> 8;
-            float c[4] = {base[i][0], base[i][0], base[i][1], base[i][1]};
-            mma16816(c, qf[i][0], x & 0x000f000fu, x & 0x00f000f0u);
-            mma16816(c, qf[i][1], y & 0x000f000fu, y & 0x00f000f0u);
-            s[2 * j + tl][0] = fmaf(tl ? d.z : d.x, c[0] + c[2], s[2 * j + tl][0]);
-            s[2 * j + tl][1] = fmaf(tl ? d.w : d.y, c[1] + c[3], s[2 * j + tl][1]);
-          }
+          for (int z = 0; z < 4; ++z) s[j][z] = i ? fmaf(z < 2 ? d0[i] : d1[i], c[z], s[j][z]) : (z < 2 ? d0[0] : d1[0]) * c[z];
         }
       }
 
-      // ---- the running softmax of row g
+      // ---- the running softmax of queries 2t and 2t + 1
       const bool edge = key + WK > key1 || key + WK - 1 > w.len - w.n + tok0;
-      float top = -INFINITY;
+      if (edge) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          s[i][x] *= rs;
-          if (edge) {
-            const int k = key + 16 * (i >> 1) + 4 * t + 2 * (i & 1) + x;
-            if (k > last_key || k >= key1) s[i][x] = -INFINITY;
+          for (int z = 0; z < 4; ++z) {
+            const int k = key + 16 * j + (z >> 1) * 8 + g;
+            if (k > last_key[z & 1] || k >= key1) s[j][z] = -INFINITY;
           }
-          top = fmaxf(top, s[i][x]);
-        }
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-      if (__any_sync(~0u, top > m)) {
-        const float now = fmaxf(m, top);
-        const float by = now == -INFINITY ? 0.f : exp2_fast(m - now);
-        m = now;
-        l *= by;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          vsum[i] *= by;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) acc[i][j][x] *= by;
-        }
       }
-      const float ms = m == -INFINITY ? 0.f : m;
+      float top[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(fmaxf(s[0][i], s[0][i + 2]), fmaxf(s[1][i], s[1][i + 2]));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 4));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 8));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 16)) * rs[i];
+      }
+      if (__any_sync(~0u, top[0] > m[0] || top[1] > m[1])) {
+        float by[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          s[i][x] = exp2_fast(s[i][x] - ms);
-          l += s[i][x];
+        for (int i = 0; i < 2; ++i) {
+          const float now = fmaxf(m[i], top[i]);
+          by[i] = now == -INFINITY ? 0.f : exp2_fast(m[i] - now);
+          m[i] = now;
+          l[i] *= by[i];
         }
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[i][j][x] *= by[x & 1];
+      }
+      const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0] - PEXP, m[1] == -INFINITY ? 0.f : m[1] - PEXP};
+      // probabilities as halves, turned so that lane (g, t) has query g and keys 2t, 2t + 1 of each 8
+      __half2 hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float p0 = exp2_fast(fmaf(s[j][2 * i], rs[0], -ms[0]));
+          const float p1 = exp2_fast(fmaf(s[j][2 * i + 1], rs[1], -ms[1]));
+          l[0] += p0;
+          l[1] += p1;
+          __half2 ph, pl;
+          split2(p0, p1, &ph, &pl);
+          hi[2 * j + i] = halves(transposed(bits(ph)));
+          lo[2 * j + i] = halves(transposed(bits(pl)));
+        }
+      uint32_t seen = 0xffu;  // bit 2i + x: key 8i + 2t + x counts for query g
+      if (odd_scale && edge) {
+        const int last = w.len - w.n + row_token(g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (key + 8 * (i >> 1) + 2 * t + (i & 1) > last) seen &= ~(1u << i);
+      }
 
-      // ---- o: 16 keys at a time
+      // ---- o
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int i = 0; i < NB; ++i) {
+        uint32_t vw[4];  // codes of element pairs, 8 keys each
+        ldsm4t(vw, from + Tile::CODES + Tile::code_at(lane, i));
+        const uint4 d4 = *reinterpret_cast<const uint4*>(vscale + (i * 4 + t) * 8);
+        const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w};
+        uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int i = 0; i < NB; i += 2) {
-          uint32_t vw[4];
-          {
-            const int mi = lane >> 3, bl = NB == 1 ? 0 : (i + (mi >> 1) < NB ? i + (mi >> 1) : i);
-            const int row = 16 * j + 8 * (mi & 1) + (lane & 7);
-            ldsm4t(vw, from + Tile::CODES + Tile::code_at(row, bl));
+        for (int x = 0; x < 4; ++x) {
+          const __half2 d = halves(dw[x]);
+          const __half2 big = __hmul2(hi[x], d);
+          const __half2 rest = __hfma2(lo[x], d, __hfma2(hi[x], d, __hneg2(big)));
+          ph[x] = bits(big);
+          pl[x] = bits(rest);
+        }
+        if (seen != 0xffu) {  // a key that a row does not see counts nothing, whatever its scale is
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t keep = ((seen >> (2 * x)) & 1u ? 0x0000ffffu : 0u) | ((seen >> (2 * x + 1)) & 1u ? 0xffff0000u : 0u);
+            ph[x] &= keep;
+            pl[x] &= keep;
           }
+        }
 #pragma unroll
-          for (int ii = 0; ii < 2; ++ii) {
-            if (i + ii >= NB) break;
-            const float4 d = *reinterpret_cast<const float4*>(fsc + (NB + i + ii) * WK + 16 * j + 4 * t);
-            float x0 = s[2 * j][0] * d.x, x1 = s[2 * j][1] * d.y;
-            float x2 = s[2 * j + 1][0] * d.z, x3 = s[2 * j + 1][1] * d.w;
-            if (edge) {  // a key that this row does not see counts nothing, whatever its scale is
-              const int k = key + 16 * j + 4 * t;
-              if (k > last_key) x0 = 0.f;
-              if (k + 1 > last_key) x1 = 0.f;
-              if (k + 2 > last_key) x2 = 0.f;
-              if (k + 3 > last_key) x3 = 0.f;
-            }
-            vsum[i + ii] += (x0 + x1) + (x2 + x3);
-            uint32_t pf[4];
-            split2(x0, x1, &pf[0], &pf[1]);
-            split2(x2, x3, &pf[2], &pf[3]);
-            const uint32_t u = vw[2 * ii], v = vw[2 * ii + 1], uy = u >> 8, vy = v >> 8;
-            mma16816(acc[i + ii][0], pf, u & 0x000f000fu, v & 0x000f000fu);
-            mma16816(acc[i + ii][1], pf, u & 0x00f000f0u, v & 0x00f000f0u);
-            mma16816(acc[i + ii][2], pf, uy & 0x000f000fu, vy & 0x000f000fu);
-            mma16816(acc[i + ii][3], pf, uy & 0x00f000f0u, vy & 0x00f000f0u);
-          }
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t u = vw[2 * j], v = vw[2 * j + 1], us = u >> 8, vs = v >> 8;
+          const uint32_t a0 = codes0(u), a1 = codes1(u), a2 = codes0(v), a3 = codes1(v);
+          mma16816(acc[i][0], a0, a1, a2, a3, ph[2 * j], ph[2 * j + 1], acc[i][0]);
+          mma16816(acc[i][0], a0, a1, a2, a3, pl[2 * j], pl[2 * j + 1], acc[i][0]);
+          const uint32_t c0 = codes0(us), c1 = codes1(us), c2 = codes0(vs), c3 = codes1(vs);
+          mma16816(acc[i][1], c0, c1, c2, c3, ph[2 * j], ph[2 * j + 1], acc[i][1]);
+          mma16816(acc[i][1], c0, c1, c2, c3, pl[2 * j], pl[2 * j + 1], acc[i][1]);
         }
       }
       stage = stage == STAGES - 1 ? 0 : stage + 1;
@@ -449,37 +508,42 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
     copies_wait<0>();
 
     // ---- the warps' parts of the segment joined through shared memory
-    l += __shfl_xor_sync(~0u, l, 1);
-    l += __shfl_xor_sync(~0u, l, 2);
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - vexp) << 23);
-    __syncthreads();  // the ring is free
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[i] += __shfl_xor_sync(~0u, l[i], o);
+      l[i] *= 1.f / (1 << PEXP);
+    }
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - PEXP - vexp) << 23);
+    __syncthreads();  // the rings are free
     float* jo = reinterpret_cast<float*>(smem) + warp * RT * HD;
     float* jm = reinterpret_cast<float*>(smem) + W * RT * HD;  // [W][RT] m, then l
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      vsum[i] += __shfl_xor_sync(~0u, vsum[i], 1);
-      vsum[i] += __shfl_xor_sync(~0u, vsum[i], 2);
-      // columns 4 (2t) + j and 4 (2t + 1) + j of the block
-      float x[8];
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float unit = j & 1 ? 1048576.f : 16777216.f;
-        x[j] = ((acc[i][j][0] + acc[i][j][2]) * unit - 8.f * vsum[i]) * down;
-        x[4 + j] = ((acc[i][j][1] + acc[i][j][3]) * unit - 8.f * vsum[i]) * down;
+      for (int x = 0; x < 2; ++x)
+        *reinterpret_cast<float4*>(jo + (2 * t + x) * HD + 32 * i + 4 * g) =
+            make_float4(acc[i][0][x] * down, acc[i][0][2 + x] * down, acc[i][1][x] * down,
+                        acc[i][1][2 + x] * down);
+    if (g == 0) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        jm[warp * RT + 2 * t + x] = m[x];
+        jm[W * RT + warp * RT + 2 * t + x] = l[x];
       }
-      float4* to = reinterpret_cast<float4*>(jo + g * HD + 32 * i + 8 * t);
-      to[0] = make_float4(x[0], x[1], x[2], x[3]);
-      to[1] = make_float4(x[4], x[5], x[6], x[7]);
-    }
-    if (t == 0) {
-      jm[warp * RT + g] = m;
-      jm[W * RT + warp * RT + g] = l;
     }
     __syncthreads();
     const bool whole = at == item_at && seg_end == item_end;
-    const int first_cta = kv_cta_of(item_at, total, ctas);
-    const int last_cta = kv_cta_of(item_end - 1, total, ctas);
     float* part = a.part + static_cast<size_t>(2 * blockIdx.x + (at == item_at ? 1 : 0)) * RT * (HD + 2);
+    auto write = [&](int r, int c4, float M, float L, float4 o) {
+      const int tk = tok0 + r / width, hh = h * a.group + head0 + r % width;
+      const float inv = M == -INFINITY ? 0.f : 1.f / L;
+      reinterpret_cast<float4*>(a.o + static_cast<size_t>(w.first + tk) * a.o_ld + static_cast<size_t>(hh) * HD)[c4] =
+          make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+      if (a.lse && c4 == 0)
+        a.lse[static_cast<size_t>(w.first + tk) * a.c.kv_heads * a.group + hh] =
+            M == -INFINITY ? -INFINITY : M * 0.69314718055994531f + logf(L);
+    };
     for (int i = tid; i < RT * HD / 4; i += W * 32) {
       const int r = i / (HD / 4), c4 = i - r * (HD / 4);
       float M = -INFINITY, L = 0.f;
@@ -498,15 +562,7 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
         o.w = fmaf(y.w, by, o.w);
       }
       if (whole) {
-        if (r < rows) {
-          const int tk = tok0 + r / width, hh = h * a.group + head0 + r % width;
-          const float inv = M == -INFINITY ? 0.f : 1.f / L;
-          reinterpret_cast<float4*>(a.o + static_cast<size_t>(w.first + tk) * a.o_ld + static_cast<size_t>(hh) * HD)[c4] =
-              make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-          if (a.lse && c4 == 0)
-            a.lse[static_cast<size_t>(w.first + tk) * a.c.kv_heads * a.group + hh] =
-                M == -INFINITY ? -INFINITY : M * 0.69314718055994531f + logf(L);
-        }
+        if (r < rows) write(r, c4, M, L, o);
       } else {
         reinterpret_cast<float4*>(part)[i] = o;
         if (c4 == 0) {
@@ -517,19 +573,18 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
     }
     if (!whole) {
       // ---- the last of the item's CTAs to arrive joins the parts
+      const int first_cta = kv_cta_of(item_at, total, ctas), last_cta = kv_cta_of(item_end - 1, total, ctas);
       __threadfence();
       __syncthreads();
       if (tid == 0) {
-        const int need = last_cta - first_cta + 1;
-        last_s = atomicAdd(a.count + first_cta, 1) == need - 1;
+        last_s = atomicAdd(a.count + first_cta, 1) == last_cta - first_cta;
         if (last_s) a.count[first_cta] = 0;
       }
       __syncthreads();
       if (last_s) {
         __threadfence();
-        for (int i = tid; i < RT * HD / 4; i += W * 32) {
+        for (int i = tid; i < rows * HD / 4; i += W * 32) {
           const int r = i / (HD / 4), c4 = i - r * (HD / 4);
-          if (r >= rows) continue;
           float M = -INFINITY, L = 0.f;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -546,17 +601,11 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
             o.z = fmaf(y.z, by, o.z * old);
             o.w = fmaf(y.w, by, o.w * old);
           }
-          const int tk = tok0 + r / width, hh = h * a.group + head0 + r % width;
-          const float inv = M == -INFINITY ? 0.f : 1.f / L;
-          reinterpret_cast<float4*>(a.o + static_cast<size_t>(w.first + tk) * a.o_ld + static_cast<size_t>(hh) * HD)[c4] =
-              make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-          if (a.lse && c4 == 0)
-            a.lse[static_cast<size_t>(w.first + tk) * a.c.kv_heads * a.group + hh] =
-                M == -INFINITY ? -INFINITY : M * 0.69314718055994531f + logf(L);
+          write(r, c4, M, L, o);
         }
       }
     }
-    __syncthreads();  // the shared memory is the ring again
+    __syncthreads();  // the shared memory is the rings again
 
     // ---- the next item: the next tile of rows, head, sequence that has any
     at = seg_end;
@@ -568,7 +617,7 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
           h = 0;
           do {  // units remain, so a sequence with rows does (were the lengths left alone meanwhile)
             if (++b >= a.s.seqs) return;
-            w = kv_rows(a.s, a.c.page, a.group, b, a.err);
+            w = kv_rows(a.s, a.c.page, a.group, RT, b, a.err);
           } while (w.tiles == 0);
         }
       }
@@ -577,18 +626,35 @@ __global__ void __launch_bounds__(Shape<HD>::WARPS * 32, 1) attention_kv_kernel(
   }
 }
 
-template <int HD>
-int launch(Context* ctx, const AttnKv& a, int ctas, cudaStream_t s) {
+template <int HD, int W>
+int launch(Context* ctx, const AttnKv& a, cudaStream_t s) {
+  using S = Shape<HD, W>;
   static thread_local int ready = -1;  // device on which the attribute is set
   if (ready != ctx->device) {
-    const cudaError_t e = cudaFuncSetAttribute(attention_kv_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               Shape<HD>::SMEM);
+    const cudaError_t e =
+        cudaFuncSetAttribute(attention_kv_kernel<HD, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return ctx->fail_cuda(e, "attention_kv: shared memory");
     ready = ctx->device;
   }
-  glc::launch_pdl(ctx, attention_kv_kernel<HD>, dim3(ctas), dim3(Shape<HD>::WARPS * 32), Shape<HD>::SMEM, s, a);
+  const int ctas = ctx->num_sms * S::PER_SM;
+  if (ctas > Context::kKvCounters) return ctx->fail(GLC_ERR_UNSUPPORTED, "attention_kv: more SMs than counters");
+  void* ws = nullptr;
+  const int rc = ctx->workspace(sizeof(float) * 2 * ctas * S::RT * (HD + 2), &ws);
+  if (rc) return rc;
+  AttnKv b = a;
+  b.part = static_cast<float*>(ws);
+  glc::launch_pdl(ctx, attention_kv_kernel<HD, W>, dim3(ctas), dim3(W * 32), S::SMEM, s, b);
   GLC_LAUNCH_CHECK(ctx, "attention_kv");
   return GLC_OK;
+}
+
+template <int HD>
+int launch_for(Context* ctx, const AttnKv& a, cudaStream_t s) {
+  // Few items are cut between many CTAs, and few large CTAs leave fewer parts to
+  // join; of many items a CTA has several, and small CTAs overlap one's joins
+  // with another's copies.
+  const long long items = static_cast<long long>(a.s.rows) * ((a.group + 7) / 8) * a.c.kv_heads;
+  return items >= ctx->num_sms / 2 ? launch<HD, 4>(ctx, a, s) : launch<HD, 16>(ctx, a, s);
 }
 
 }  // namespace
@@ -614,11 +680,6 @@ extern "C" int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const g
   if (static_cast<long long>(batch->num_rows) * group > 0x40000000) return no("too many query rows");
   if (batch->num_rows == 0 || batch->num_seqs == 0) return GLC_OK;
   glc::DeviceScope on(c);
-  const int ctas = c->num_sms;
-  const int hd = cache->head_dim;
-  void* ws = nullptr;
-  rc = c->workspace(sizeof(float) * 2 * ctas * glc::RT * (hd + 2), &ws);
-  if (rc) return rc;
   glc::AttnKv a;
   a.c = glc::kv_pools(*cache);
   a.s = glc::kv_seqs(*batch);
@@ -628,16 +689,16 @@ extern "C" int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const g
   a.o_ld = o_ld;
   a.lse = lse;
   a.group = group;
-  a.scale2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(hd)));
-  a.part = static_cast<float*>(ws);
+  a.scale2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(cache->head_dim)));
+  a.part = nullptr;
   a.count = c->kv_count;
   a.err = c->d_err;
   // the cache's share of the traffic depends on lengths that the host does not have
   glc::ProfScope prof(c, glc::PROF_OTHER, 8.0 * batch->num_rows * width, c->stream);
-  switch (hd) {
-    case 32: return glc::launch<32>(c, a, ctas, c->stream);
-    case 64: return glc::launch<64>(c, a, ctas, c->stream);
-    case 96: return glc::launch<96>(c, a, ctas, c->stream);
-    default: return glc::launch<128>(c, a, ctas, c->stream);
+  switch (cache->head_dim) {
+    case 32: return glc::launch_for<32>(c, a, c->stream);
+    case 64: return glc::launch_for<64>(c, a, c->stream);
+    case 96: return glc::launch_for<96>(c, a, c->stream);
+    default: return glc::launch_for<128>(c, a, c->stream);
   }
 }

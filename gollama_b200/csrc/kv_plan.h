@@ -124,25 +124,24 @@ KV_HD int kv_page(const KvSeqs& s, int num_pages, int b, int index, int* err) {
 
 // ---------------------------------------------------------------- attention
 
-constexpr int KV_RT = 8;   // query rows of an item
 constexpr int KV_WK = 32;  // keys of a warp's tile
 
-// The items of one KV head of a sequence.  A tile of KV_RT query rows holds the
+// The items of one KV head of a sequence.  A tile of `rt` query rows holds the
 // heads of `toks` whole tokens, or, where a group has more heads than that, up
-// to KV_RT heads of one token (`parts` tiles per token).  Tile i sees the keys
-// of its last token, in units of `unit` keys, one at least (an item without
-// keys still writes its rows).
+// to rt heads of one token (`parts` tiles per token).  Tile i sees the keys of
+// its last token, in units of `unit` keys, one at least (an item without keys
+// still writes its rows).
 struct KvRows {
   int first, n, len, toks, parts, tiles;
 };
-KV_HD KvRows kv_rows(const KvSeqs& s, int page, int group, int b, int* err) {
+KV_HD KvRows kv_rows(const KvSeqs& s, int page, int group, int rt, int b, int* err) {
   const KvSpan r = kv_span(s, page, b, err);
   KvRows w;
   w.first = r.first;
   w.n = r.n;
   w.len = r.len;
-  w.toks = group < KV_RT ? KV_RT / group : 1;
-  w.parts = (group + KV_RT - 1) / KV_RT;
+  w.toks = group < rt ? rt / group : 1;
+  w.parts = (group + rt - 1) / rt;
   w.tiles = (r.n + w.toks - 1) / w.toks * w.parts;
   return w;
 }
@@ -213,15 +212,10 @@ struct KvTile {
   static constexpr int CODE_PIECES = KV_WK * NB;  // of one side
   static constexpr int SCALE_PIECES = 8 * NB;     // of both sides
 
-  // Byte of piece `ch` of the token in column `col` of the products.  The 16-byte
-  // pieces are swizzled so that a piece of 8 columns falls in 8 different quads of banks.
-  static KV_HD int code_at(int col, int ch) {
-    return col * ROW + 16 * (HD == 128 ? ch ^ ((col >> 1) & 3) : HD == 64 ? ch ^ ((col >> 2) & 1) : ch);
-  }
-  // Column of a token: of 16 tokens, those with bit 1 clear, then those with it
-  // set, so that a lane's two columns in each of two products are 4 tokens in a row.
-  static KV_HD int column(int token) {
-    return (token & 16) | ((token & 2) << 2) | ((token >> 1) & 6) | (token & 1);
+  // Byte of piece `ch` of a token.  The 16-byte pieces are swizzled so that a
+  // piece of 8 tokens falls in 8 different quads of banks.
+  static KV_HD int code_at(int token, int ch) {
+    return token * ROW + 16 * (HD == 128 ? ch ^ ((token >> 1) & 3) : HD == 64 ? ch ^ ((token >> 2) & 1) : ch);
   }
   // Piece id of the codes of a side: its token and where it comes from (relative
   // to its token's codes) and goes to.
@@ -229,7 +223,7 @@ struct KvTile {
     const int tk = id / NB, ch = id - tk * NB;
     *token = tk;
     *from = 16 * ch;
-    *to = code_at(column(tk), ch);
+    *to = code_at(tk, ch);
   }
   // Piece id of the scales: its side, its group of 16 tokens, where it comes
   // from (relative to the group's scales) and goes to (in the tile).

@@ -26,11 +26,11 @@ namespace {
 
 // 0, or a number that names what went wrong
 template <int HD>
-int walk(const KvPools& c, const KvSeqs& s, int group, int warps, int grid, int* err) {
+int walk(const KvPools& c, const KvSeqs& s, int group, int rt, int warps, int grid, int* err) {
   using Tile = KvTile<HD>;
   const int unit = warps * KV_WK;
   long long total = 0;
-  for (int b = 0; b < s.seqs; ++b) total += kv_head_units(kv_rows(s, c.page, group, b, err), unit) * c.kv_heads;
+  for (int b = 0; b < s.seqs; ++b) total += kv_head_units(kv_rows(s, c.page, group, rt, b, err), unit) * c.kv_heads;
   const long long ctas = std::min<long long>(total, grid);
   const size_t pool = static_cast<size_t>(c.num_pages) * c.kv_heads * c.chunk;
   // (sequence, head, tile) -> per key how often it was read; and who wrote it
@@ -46,12 +46,12 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int warps, int grid, int*
     long long at_b = 0, units_b = 0;
     int b = 0;
     for (; b < s.seqs; ++b) {
-      units_b = kv_head_units(kv_rows(s, c.page, group, b, err), unit) * c.kv_heads;
+      units_b = kv_head_units(kv_rows(s, c.page, group, rt, b, err), unit) * c.kv_heads;
       if (begin < at_b + units_b) break;
       at_b += units_b;
     }
     if (b == s.seqs) return 3;
-    KvRows w = kv_rows(s, c.page, group, b, err);
+    KvRows w = kv_rows(s, c.page, group, rt, b, err);
     const long long per_head = units_b / c.kv_heads;
     int h = static_cast<int>((begin - at_b) / per_head);
     long long item_at;
@@ -66,10 +66,10 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int warps, int grid, int*
       const int keys = kv_run_keys(w, run_at);
       const int key0 = static_cast<int>(at - item_at) * unit;
       const int key1 = std::min(static_cast<int>(seg_end - item_at) * unit, keys);
-      const int tok0 = run_at * w.toks, head0 = part_at * KV_RT;
-      const int width = group < KV_RT ? group : std::min(group - head0, KV_RT);
+      const int tok0 = run_at * w.toks, head0 = part_at * rt;
+      const int width = group < rt ? group : std::min(group - head0, rt);
       const int rows = std::min(w.n - tok0, w.toks) * width;
-      if (rows < 1 || rows > KV_RT || head0 + width > group) return 5;
+      if (rows < 1 || rows > rt || head0 + width > group) return 5;
       auto& count = seen[{b, h, tile}];
       count.resize(keys);
       for (int warp = 0; warp < warps; ++warp) {
@@ -96,7 +96,6 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int warps, int grid, int*
             Tile::code_piece(id, &tk, &from, &to);
             const int i = tk >> 4;
             if (to < 0 || to + 16 > Tile::CODES || to % 16 || !to_all.insert(to).second) return 8;
-            if (Tile::column(tk) / 16 != i) return 9;
             if (!ok[i] || key + tk >= key1) continue;
             const size_t src = base[i] + static_cast<size_t>(g[i].slot * 16 + (tk & 15)) * Tile::ROW + from;
             if (src + 16 > pool || src % 16) return 10;
@@ -132,7 +131,7 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int warps, int grid, int*
             h = 0;
             do {
               if (++b >= s.seqs) return 16;
-              w = kv_rows(s, c.page, group, b, err);
+              w = kv_rows(s, c.page, group, rt, b, err);
             } while (w.tiles == 0);
           }
         }
@@ -149,7 +148,7 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int warps, int grid, int*
   }
   // every item once, every key of it that has a page once
   for (int b = 0; b < s.seqs; ++b) {
-    const KvRows w = kv_rows(s, c.page, group, b, err);
+    const KvRows w = kv_rows(s, c.page, group, rt, b, err);
     int covered = 0;
     for (int h = 0; h < c.kv_heads; ++h)
       for (int tile = 0; tile < w.tiles; ++tile) {
@@ -169,14 +168,15 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int warps, int grid, int*
 
 }  // namespace
 
-extern "C" int kv_walk(const glc_kv_cache* cache, const glc_kv_batch* batch, int group, int grid, int* err) {
+extern "C" int kv_walk(const glc_kv_cache* cache, const glc_kv_batch* batch, int group, int rt, int warps, int grid,
+                       int* err) {
   const KvPools c = kv_pools(*cache);
   const KvSeqs s = kv_seqs(*batch);
   switch (c.head_dim) {
-    case 32: return walk<32>(c, s, group, 16, grid, err);
-    case 64: return walk<64>(c, s, group, 16, grid, err);
-    case 96: return walk<96>(c, s, group, 12, grid, err);
-    case 128: return walk<128>(c, s, group, 12, grid, err);
+    case 32: return walk<32>(c, s, group, rt, warps, grid, err);
+    case 64: return walk<64>(c, s, group, rt, warps, grid, err);
+    case 96: return walk<96>(c, s, group, rt, warps, grid, err);
+    case 128: return walk<128>(c, s, group, rt, warps, grid, err);
   }
   return -1;
 }
@@ -195,12 +195,12 @@ extern "C" void kv_rows_of(const glc_kv_cache* cache, const glc_kv_batch* batch,
   }
 }
 
-// Quads of banks that 8 columns of a piece fall in (8: no conflict).
-extern "C" int kv_bank_quads(int hd, int col0, int ch) {
+// Quads of banks that a piece of 8 tokens falls in (8: no conflict).
+extern "C" int kv_bank_quads(int hd, int token0, int ch) {
   std::set<int> quads;
   for (int i = 0; i < 8; ++i) {
-    const int at = hd == 32 ? KvTile<32>::code_at(col0 + i, ch) : hd == 64 ? KvTile<64>::code_at(col0 + i, ch)
-                   : hd == 96 ? KvTile<96>::code_at(col0 + i, ch) : KvTile<128>::code_at(col0 + i, ch);
+    const int at = hd == 32 ? KvTile<32>::code_at(token0 + i, ch) : hd == 64 ? KvTile<64>::code_at(token0 + i, ch)
+                   : hd == 96 ? KvTile<96>::code_at(token0 + i, ch) : KvTile<128>::code_at(token0 + i, ch);
     quads.insert(at / 16 % 8);
   }
   return static_cast<int>(quads.size());

@@ -43,9 +43,9 @@ def batch_of(table, lens, starts=None, rows=None):
     return b
 
 
-def walk(host, cache, batch, group, grid):
+def walk(host, cache, batch, group, grid, rt=8, warps=16):
     err = C.c_int(0)
-    return host.kv_walk(C.byref(cache), C.byref(batch), group, grid, C.byref(err)), err.value
+    return host.kv_walk(C.byref(cache), C.byref(batch), group, rt, warps, grid, C.byref(err)), err.value
 
 
 def table_for(lens, page, pages, seed):
@@ -62,8 +62,8 @@ def table_for(lens, page, pages, seed):
 def test_every_key_is_read_once_by_every_item(host, hd, page, group, lens, news):
     starts = None if news is None else np.concatenate([[0], np.cumsum(news)])
     batch = batch_of(table_for(lens, page, 40, 1), lens, starts)
-    for grid in (1, 3, 148):
-        assert walk(host, cache_of(40, page, 2, hd), batch, group, grid) == (0, 0), grid
+    for grid, rt, warps in ((1, 8, 4), (3, 8, 16), (148, 8, 16), (592, 8, 4), (148, 16, 8), (444, 32, 4)):
+        assert walk(host, cache_of(40, page, 2, hd), batch, group, grid, rt, warps) == (0, 0), grid
 
 
 def test_walk_of_random_batches(host):
@@ -76,7 +76,7 @@ def test_walk_of_random_batches(host):
         lens = [x + int(r.integers(0, 900)) for x in news]
         page, hd, group = int(r.choice([16, 32, 80])), int(r.choice([32, 64, 96, 128])), int(r.integers(1, 18))
         batch = batch_of(table_for(lens, page, 64, i), lens, np.concatenate([[0], np.cumsum(news)]))
-        assert walk(host, cache_of(64, page, int(r.integers(1, 4)), hd), batch, group, int(r.integers(1, 200))) == (0, 0), i
+        assert walk(host, cache_of(64, page, int(r.integers(1, 4)), hd), batch, group, int(r.integers(1, 200)), int(r.choice([8, 16, 32])), int(r.choice([4, 8, 12, 16]))) == (0, 0), i
 
 
 def test_bad_pages_lengths_and_rows_are_neither_read_nor_silent(host):
@@ -113,8 +113,8 @@ def test_rows_find_their_sequence_and_position(host):
 
 
 @pytest.mark.parametrize("hd", [32, 64, 96, 128])
-def test_columns_of_a_piece_fall_in_different_banks(host, hd):
-    assert all(host.kv_bank_quads(hd, col, ch) == 8 for col in (0, 8, 16, 24) for ch in range(hd // 32))
+def test_a_piece_of_8_tokens_falls_in_different_banks(host, hd):
+    assert all(host.kv_bank_quads(hd, token, ch) == 8 for token in (0, 8, 16, 24) for ch in range(hd // 32))
 
 
 # ------------------------------------------------------------------ refusals
