@@ -47,6 +47,7 @@ struct AttnKv {
   float* part;   // [2 * CTAs][RT * (HD + 2)]
   int* count;    // arrivals, by the CTA in which the item starts; zero between calls
   int* err;
+  uint32_t k1024, less72;  // pairs of halves: 1024, -72
 };
 
 template <int HD, int W>
@@ -64,11 +65,9 @@ struct Shape {
   static_assert(WARP % 16 == 0, "rings start on 16 bytes");
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool some) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16 : 0) : "memory");
+// 16 bytes, `size` of them from src and zeros after
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int size) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
 }
 __device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -93,7 +92,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 // d = a b + c
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1, const float* c) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
@@ -103,21 +102,76 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-__device__ __forceinline__ __half2 halves(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+// Pairs of halves as 32-bit words throughout.
+__device__ __forceinline__ uint32_t add2(uint32_t x, uint32_t y) {
+  uint32_t z;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+  return z;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t x, uint32_t y) {
+  uint32_t z;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+  return z;
+}
+__device__ __forceinline__ uint32_t fma2(uint32_t x, uint32_t y, uint32_t w) {
+  uint32_t z;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(z) : "r"(x), "r"(y), "r"(w));
+  return z;
+}
+__device__ __forceinline__ uint32_t neg2(uint32_t x) {
+  uint32_t z;
+  asm("neg.f16x2 %0, %1;" : "=r"(z) : "r"(x));
+  return z;
+}
 // (x0, x1) as halves hi + lo: 22 bits where lo is a normal half
-__device__ __forceinline__ void split2(float x0, float x1, __half2* hi, __half2* lo) {
-  *hi = __floats2half2_rn(x0, x1);
-  const float2 f = __half22float2(*hi);
-  *lo = __floats2half2_rn(x0 - f.x, x1 - f.y);
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t* hi, uint32_t* lo) {
+  float f0, f1;
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "cvt.rn.f16x2.f32 %0, %4, %3;\n\t"
+      "mov.b32 {a, b}, %0;\n\t"
+      "cvt.f32.f16 %1, a;\n\t"
+      "cvt.f32.f16 %2, b;\n\t}"
+      : "=r"(*hi), "=f"(f0), "=f"(f1)
+      : "f"(x0), "f"(x1));
+  asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(*lo) : "f"(x0 - f0), "f"(x1 - f1));
 }
-// codes less 8 of the low nibbles of x's halves, and of the next ones
-__device__ __forceinline__ uint32_t codes0(uint32_t x) {
-  return bits(__hadd2(halves((x & 0x000f000fu) | 0x64006400u), halves(0xe408e408u)));  // - 1032
+// Codes less 8 of the low nibbles of x's halves, and of the next ones.  The
+// constants that an instruction has no second immediate for are kernel
+// parameters, so that they stay in registers.
+__device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t y) {
+  uint32_t z;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(z) : "r"(x), "r"(mask), "r"(y));  // (x & mask) | y
+  return z;
 }
-__device__ __forceinline__ uint32_t codes1(uint32_t x) {
-  return bits(__hfma2(halves((x & 0x00f000f0u) | 0x64006400u), halves(0x2c002c00u), halves(0xd480d480u)));  // / 16 - 72
+__device__ __forceinline__ float half_float(uint32_t x) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(x)));
 }
+// N halves of shared memory, in pairs
+template <int N>
+__device__ __forceinline__ void load_halves(uint32_t at, uint32_t* x) {
+  if constexpr (N == 4) {
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(at));
+  } else if constexpr (N == 2) {
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x[0]) : "r"(at));
+  } else {
+#pragma unroll
+    for (int i = 0; i < (N + 1) / 2; ++i) {
+      unsigned short a, b = 0;
+      asm volatile("ld.shared.b16 %0, [%1];" : "=h"(a) : "r"(at + 4 * i));
+      if (2 * i + 1 < N) asm volatile("ld.shared.b16 %0, [%1];" : "=h"(b) : "r"(at + 4 * i + 2));
+      x[i] = a | static_cast<uint32_t>(b) << 16;
+    }
+  }
+}
+struct Unpack {
+  uint32_t k1024, less72;
+  __device__ __forceinline__ uint32_t low(uint32_t x) const {
+    return add2(masked_or(x, 0x000f000fu, k1024), 0xe408e408u);  // - 1032
+  }
+  __device__ __forceinline__ uint32_t next(uint32_t x) const {
+    return fma2(masked_or(x, 0x00f000f0u, k1024), 0x2c002c00u, less72);  // / 16 - 72
+  }
+};
 
 template <int HD, int W>
 __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_kernel(const AttnKv a) {
@@ -126,136 +180,141 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
   using Tile = KvTile<HD>;
   constexpr int NB = S::NB, RT = S::RT, STAGES = S::STAGES, UNIT = W * WK;
   extern __shared__ __align__(128) uint8_t smem[];
+  // the share and where in it the CTA is, by thread 0
+  struct Place {
+    long long at, end, item_at, total, ctas;
+    int b, h, tile, units;
+    KvRows w;
+  };
+  __shared__ Place place;
   __shared__ long long sum_s[W];
-  __shared__ long long at_s[2];
-  __shared__ int seq_s, last_s;
+  __shared__ int last_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
 
   // ---- the share of this CTA: thread i counts the units of its run of
   // sequences, a scan over the threads finds the run that the share begins in
-  if (tid == 0) seq_s = -1;
-  const int run = (a.s.seqs + W * 32 - 1) / (W * 32);
-  const int b0 = tid * run < a.s.seqs ? tid * run : a.s.seqs;
-  const int b1 = b0 + run < a.s.seqs ? b0 + run : a.s.seqs;
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += kv_head_units(kv_rows(a.s, a.c.page, a.group, RT, b, a.err), UNIT) * a.c.kv_heads;
-  long long upto = mine;
+  {
+    if (tid == 0) place.b = -1;
+    const int run = (a.s.seqs + W * 32 - 1) / (W * 32);
+    const int b0 = tid * run < a.s.seqs ? tid * run : a.s.seqs;
+    const int b1 = b0 + run < a.s.seqs ? b0 + run : a.s.seqs;
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b)
+      mine += kv_head_units(kv_rows(a.s, a.c.page, a.group, RT, b, a.err), UNIT) * a.c.kv_heads;
+    long long upto = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(~0u, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) sum_s[warp] = upto;
-  __syncthreads();
-  long long total = 0, before = 0;
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    if (i < warp) before += sum_s[i];
-    total += sum_s[i];
-  }
-  upto += before;
-  const long long ctas = total < gridDim.x ? total : gridDim.x;
-  if (blockIdx.x >= ctas) return;
-  const long long begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
-  if (upto - mine <= begin && begin < upto) {
-    long long at = upto - mine;
-    for (int b = b0; b < b1; ++b) {
-      const long long u = kv_head_units(kv_rows(a.s, a.c.page, a.group, RT, b, a.err), UNIT) * a.c.kv_heads;
-      if (begin < at + u) {
-        seq_s = b;
-        at_s[0] = at;
-        at_s[1] = u;
-        break;
-      }
-      at += u;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += v;
     }
+    if (lane == 31) sum_s[warp] = upto;
+    __syncthreads();
+    long long total = 0, before = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if (i < warp) before += sum_s[i];
+      total += sum_s[i];
+    }
+    upto += before;
+    const long long ctas = total < gridDim.x ? total : gridDim.x;
+    if (blockIdx.x >= ctas) return;
+    const long long begin = total * blockIdx.x / ctas;
+    if (upto - mine <= begin && begin < upto) {
+      long long at = upto - mine;
+      for (int b = b0; b < b1; ++b) {
+        const KvRows w = kv_rows(a.s, a.c.page, a.group, RT, b, a.err);
+        const long long per_head = kv_head_units(w, UNIT), u = per_head * a.c.kv_heads;
+        if (begin < at + u) {
+          const int h = static_cast<int>((begin - at) / per_head);
+          place.at = begin;
+          place.end = total * (blockIdx.x + 1) / ctas;
+          place.total = total;
+          place.ctas = ctas;
+          place.b = b;
+          place.h = h;
+          place.tile = kv_find_tile(w, UNIT, begin - at - h * per_head, &place.item_at, &place.units);
+          place.item_at += at + h * per_head;
+          place.w = w;
+          break;
+        }
+        at += u;
+      }
+    }
+    __syncthreads();
+    if (place.b < 0) return;  // not reached, were the lengths left alone meanwhile
   }
-  __syncthreads();
-  int b = seq_s;
-  if (b < 0) return;
-  KvRows w = kv_rows(a.s, a.c.page, a.group, RT, b, a.err);
-  long long per_head = at_s[1] / a.c.kv_heads;
-  int h = static_cast<int>((begin - at_s[0]) / per_head);
-  int units = 1;
-  long long item_at;  // first unit of the item
-  int tile = kv_find_tile(w, UNIT, begin - at_s[0] - h * per_head, &item_at, &units);
-  item_at += at_s[0] + h * per_head;
 
   uint8_t* ring = smem + warp * S::WARP;
   float* kscale = reinterpret_cast<float*>(ring + STAGES * Tile::BYTES);            // [key][KS]
   __half* vscale = reinterpret_cast<__half*>(ring + STAGES * Tile::BYTES + WK * S::KS * 4);  // [block][t][8 keys][pair]
   const uint32_t ring_u = smem_u32(ring);
   const int page16 = a.c.page >> 4;
+  const uint32_t page_bytes = static_cast<uint32_t>(a.c.chunk * a.c.kv_heads);
+  // 8 lanes each copy a side of a group of 16 tokens of a tile
+  const int lane8 = lane & 7, side = lane >> 4, grp = (lane >> 3) & 1;
+  const uint32_t codes_to = ring_u + Tile::codes_of(side, grp), scales_to = ring_u + Tile::scales_of(side, grp) + lane8 * 16;
+  uint32_t swizzled[4];  // piece lane8 as the pieces lane8 + 8 j of the group's codes are swizzled
+#pragma unroll
+  for (int j = 0; j < 4; ++j) swizzled[j] = codes_to + ((lane8 * 16) ^ Tile::swizzle(j));
   // a warp's tiles lie UNIT keys apart
+  const int scales_from = a.c.scales_at;
   const int step_pages = (UNIT / 16) / page16, step_slot = (UNIT / 16) % page16;
 
-  for (long long at = begin; at < end;) {
+  const Unpack unpack{a.k1024, a.less72};
+  for (;;) {
     // ---- one item, or the part of it that lies in this share
-    const long long item_end = item_at + units;
-    const long long seg_end = item_end < end ? item_end : end;
-    const int run_at = tile / w.parts, part_at = tile - run_at * w.parts;
-    const int keys = kv_run_keys(w, run_at);
-    const int key0 = static_cast<int>(at - item_at) * UNIT;
-    int key1 = static_cast<int>(seg_end - item_at) * UNIT;
-    if (key1 > keys) key1 = keys;
-
-    // the tile's first token and head, and its rows (those past the last repeat
-    // row 0 and are not written)
-    const int tok0 = run_at * w.toks, head0 = part_at * RT;
-    const int width = a.group < RT ? a.group : a.group - head0 < RT ? a.group - head0 : RT;  // heads of a token
-    const int rows = (w.n - tok0 < w.toks ? w.n - tok0 : w.toks) * width;
-    auto row_token = [&](int r) { return tok0 + (r < rows ? r : 0) / width; };
-
-    // the two groups of 16 tokens of the warp's next tile, and their pages
-    KvWalk walk[2];
-    int page[2];
-    int next = key0 + warp * WK;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      walk[i].start(next + 16 * i, page16);
-      page[i] = next + 16 * i < key1 ? kv_page(a.s, a.c.num_pages, b, walk[i].index, a.err) : -1;
+    int key0, key1, edge_key, rows, width, tok0, head0;
+    const int* table;
+    const uint8_t* head;  // piece lane8 of the item's head in page 0 of the lane's side
+    {
+      const Place& p = place;
+      const int run_at = p.tile / p.w.parts, part_at = p.tile - run_at * p.w.parts;
+      const long long seg_end = p.item_at + p.units < p.end ? p.item_at + p.units : p.end;
+      key0 = static_cast<int>(p.at - p.item_at) * UNIT;
+      key1 = static_cast<int>(seg_end - p.item_at) * UNIT;
+      const int keys = kv_run_keys(p.w, run_at);
+      if (key1 > keys) key1 = keys;
+      table = a.s.table + static_cast<size_t>(p.b) * a.s.max_pages;
+      head = (side ? a.c.v : a.c.k) + static_cast<size_t>(p.h) * a.c.chunk + lane8 * 16;
+      // the tile's first token and head, and its rows (those past the last repeat
+      // row 0 and are not written)
+      tok0 = run_at * p.w.toks, head0 = part_at * RT;
+      width = a.group < RT ? a.group : a.group - head0 < RT ? a.group - head0 : RT;  // heads of a token
+      rows = (p.w.n - tok0 < p.w.toks ? p.w.n - tok0 : p.w.toks) * width;
+      edge_key = p.w.len - p.w.n + tok0;  // the last key that all rows see
     }
-    const size_t head_at = static_cast<size_t>(h) * a.c.chunk;
-    const size_t page_bytes = a.c.chunk * a.c.kv_heads;
+    // the last key that row r sees
+    auto row_last = [&](int r) { return edge_key + (r < rows ? r : 0) / width; };
 
-    // copies the tile at `next` to a stage and looks the following one's pages up
+    auto table_page = [&](int index) {
+      const int p = table[index];
+      if (static_cast<unsigned>(p) < static_cast<unsigned>(a.c.num_pages)) return p;
+      kv_bad(a.err);
+      return -1;
+    };
+    // the lane's group of 16 tokens in the warp's next tile, and its page
+    int next = key0 + warp * WK;
+    KvWalk walk;
+    walk.start(next + 16 * grp, page16);
+    int page = next + 16 * grp < key1 ? table_page(walk.index) : -1;
+
+    // copies the tile at `next` to a stage and looks the following one's page up.
+    // A group has whole pages of 16 slots, so the slots behind the last key are
+    // copied too: their codes are numbers, their scales are not used.
     auto fetch = [&](int stage) {
       if (next < key1) {
-        const uint32_t to = ring_u + stage * Tile::BYTES;
-        const bool ok0 = page[0] >= 0, ok1 = page[1] >= 0;
-        const size_t f0 = (ok0 ? page[0] * page_bytes : 0) + head_at;
-        const size_t f1 = (ok1 ? page[1] * page_bytes : 0) + head_at;
-        const bool full = next + WK <= key1 && ok0 && ok1;
+        const uint8_t* from = head + static_cast<uint64_t>(page < 0 ? 0 : page) * page_bytes;
+        const uint8_t* codes = from + walk.slot * (16 * Tile::ROW);
+        const uint8_t* scales = from + walk.slot * (32 * NB);
+        const int size = page < 0 ? 0 : 16;  // 0: zeros are stored, nothing is read
+        const uint32_t to = stage * Tile::BYTES;
 #pragma unroll
-        for (int j = 0; j < Tile::CODE_PIECES / 32; ++j) {
-          int token, from, at_;
-          Tile::code_piece(lane + 32 * j, &token, &from, &at_);
-          const bool hi = token >= 16;
-          const size_t src =
-              (hi ? f1 : f0) + static_cast<size_t>((hi ? walk[1].slot : walk[0].slot) * 16 + (token & 15)) * Tile::ROW + from;
-          if (full) {
-            copy16(to + at_, a.c.k + src);
-            copy16(to + Tile::CODES + at_, a.c.v + src);
-          } else {
-            const bool some = (hi ? ok1 : ok0) && next + token < key1;
-            copy16(to + at_, a.c.k + src, some);
-            copy16(to + Tile::CODES + at_, a.c.v + src, some);
-          }
-        }
-        if (lane < Tile::SCALE_PIECES) {
-          int side, grp, from, at_;
-          Tile::scale_piece(lane, &side, &grp, &from, &at_);
-          const size_t src = (grp ? f1 : f0) + a.c.scales_at +
-                             static_cast<size_t>(grp ? walk[1].slot : walk[0].slot) * (32 * NB) + from;
-          copy16(to + at_, (side ? a.c.v : a.c.k) + src, grp ? ok1 : ok0);
-        }
+        for (int j = 0; j < Tile::LANE_PIECES; ++j) copy16(swizzled[j & 3] + to + 128 * j, codes + 128 * j, size);
+        if (lane8 < Tile::GROUP_SCALES) copy16(scales_to + to, scales + scales_from, size);
         next += UNIT;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          walk[i].advance(step_pages, step_slot, page16);
-          page[i] = next + 16 * i < key1 ? kv_page(a.s, a.c.num_pages, b, walk[i].index, a.err) : -1;
-        }
+        walk.advance(step_pages, step_slot, page16);
+        page = next + 16 * grp < key1 ? table_page(walk.index) : -1;
       }
       copies_close();
     };
@@ -270,7 +329,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
     {
       const int my_row = g < rows ? g : 0, my_tok = tok0 + my_row / width, my_head = head0 + my_row % width;
       const float* qp =
-          a.q + static_cast<size_t>(w.first + my_tok) * a.q_ld + static_cast<size_t>(h * a.group + my_head) * HD;
+          a.q + static_cast<size_t>(place.w.first + my_tok) * a.q_ld + static_cast<size_t>(place.h * a.group + my_head) * HD;
       float x[NB][8], top = 0.f;
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
@@ -291,7 +350,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         rs[i] = __shfl_sync(~0u, my_rs, 4 * (2 * t + i));
-        last_key[i] = w.len - w.n + row_token(2 * t + i);
+        last_key[i] = row_last(2 * t + i);
       }
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
@@ -300,10 +359,8 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
         // in the order in which the codes of 8 elements come apart: (0,4), (1,5); (2,6), (3,7)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          __half2 h0, l0, h1, l1;
-          split2(x[i][2 * j], x[i][2 * j + 4], &h0, &l0);
-          split2(x[i][2 * j + 1], x[i][2 * j + 5], &h1, &l1);
-          qf[i][j][0] = bits(h0), qf[i][j][1] = bits(h1), qf[i][j][2] = bits(l0), qf[i][j][3] = bits(l1);
+          split2(x[i][2 * j], x[i][2 * j + 4], &qf[i][j][0], &qf[i][j][2]);
+          split2(x[i][2 * j + 1], x[i][2 * j + 5], &qf[i][j][1], &qf[i][j][3]);
         }
       }
     }
@@ -318,12 +375,15 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
 #pragma unroll
         for (int x = 0; x < 4; ++x) acc[i][j][x] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    // probabilities are held at 2^PEXP and value scales at 2^vexp times their
-    // size: their products stay below 2^15, and lo and lo' are normal halves
-    // where they matter
-    constexpr int PEXP = 8;
+    // m is raised only when a score passes it by more than 2^SLACK, so that the
+    // sums are seldom rescaled; probabilities are held at 2^PEXP and value scales
+    // at 2^vexp times their size: their products stay below 2^15, and lo and lo'
+    // are normal halves where they matter
+    constexpr float SLACK = 4.f;
+    constexpr int PEXP = 4;
     int vexp = 0;
     uint32_t vtop = 0;  // largest scale (bits) that vexp allows
+    uint32_t up1 = 0x3c003c00u, up2 = 0x3c003c00u;  // 2^vexp, in pairs of halves
 
     int stage = 0;
     for (int key = key0 + warp * WK; key < key1; key += UNIT) {
@@ -334,18 +394,25 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
       bool odd_scale;  // some value scale is infinite or not a number
       {
         // lane = key: its scales, zero behind the last key
-        const __half* ks = reinterpret_cast<const __half*>(ring + stage * Tile::BYTES + 2 * Tile::CODES) + lane * NB;
-        const __half* vs = ks + WK * NB;
-        const bool some = key + lane < key1;
+        const uint32_t at = from + 2 * Tile::CODES + lane * (2 * NB);
+        uint32_t kd[(NB + 1) / 2], vd[(NB + 1) / 2];  // pairs of blocks
+        load_halves<NB>(at, kd);
+        load_halves<NB>(at + Tile::SCALES, vd);
+        if (key + WK > key1 && key + lane >= key1) {
+#pragma unroll
+          for (int i = 0; i < (NB + 1) / 2; ++i) kd[i] = vd[i] = 0;
+        }
+        float kf[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t big = 0;
-        __half vh[NB];
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          kscale[lane * S::KS + i] = some ? __half2float(ks[i]) : 0.f;
-          vh[i] = some ? vs[i] : __ushort_as_half(0);
-          const uint32_t mag = __half_as_ushort(vh[i]) & 0x7fffu;
+          kf[i] = half_float(i & 1 ? kd[i / 2] >> 16 : kd[i / 2]);
+          const uint32_t mag = (i & 1 ? vd[i / 2] >> 16 : vd[i / 2]) & 0x7fffu;
           big = big > mag ? big : mag;
         }
+        if constexpr (S::KS == 4) *reinterpret_cast<float4*>(kscale + lane * 4) = make_float4(kf[0], kf[1], kf[2], kf[3]);
+        else if constexpr (S::KS == 2) *reinterpret_cast<float2*>(kscale + lane * 2) = make_float2(kf[0], kf[1]);
+        else kscale[lane] = kf[0];
         big = __reduce_max_sync(~0u, big);
         odd_scale = big > 0x7bffu;
         if (big > vtop) {  // the same for the whole warp
@@ -362,12 +429,18 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
               for (int x = 0; x < 4; ++x) acc[i][j][x] *= by;
           vexp = now;
           vtop = e + 3 > 15 ? 0x7fffu : (static_cast<uint32_t>(e + 3 + 15) << 10) - 1;
+          // 2^vexp as two halves, since 2^19 is none
+          const int first = vexp > 15 ? 15 : vexp, second = vexp - first;
+          up1 = static_cast<uint32_t>(15 + first) * 0x04000400u;
+          up2 = static_cast<uint32_t>(15 + second) * 0x04000400u;
         }
-        const float up = __uint_as_float(static_cast<uint32_t>(127 + vexp) << 23);
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
-          vscale[((i * 4 + ((lane >> 1) & 3)) * 4 + (lane >> 3)) * 2 + (lane & 1)] =
-              __float2half_rn(__half2float(vh[i]) * up);
+        for (int i = 0; i < (NB + 1) / 2; ++i) {
+          const uint32_t d = mul2(mul2(vd[i], up1), up2);
+          __half* to = vscale + (((lane >> 1) & 3) * 4 + (lane >> 3)) * 2 + (lane & 1);
+          to[(2 * i) * 32] = __ushort_as_half(static_cast<unsigned short>(d));
+          if (2 * i + 1 < NB) to[(2 * i + 1) * 32] = __ushort_as_half(static_cast<unsigned short>(d >> 16));
+        }
       }
       __syncwarp();
 
@@ -397,8 +470,8 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
           const uint32_t x = kw[i >> 2][i & 3], y = kw[(NB + i) >> 2][(NB + i) & 3], xs = x >> 8, ys = y >> 8;
-          const uint32_t a0 = codes0(x), a1 = codes0(y), a2 = codes1(x), a3 = codes1(y);
-          const uint32_t e0 = codes0(xs), e1 = codes0(ys), e2 = codes1(xs), e3 = codes1(ys);
+          const uint32_t a0 = unpack.low(x), a1 = unpack.low(y), a2 = unpack.next(x), a3 = unpack.next(y);
+          const uint32_t e0 = unpack.low(xs), e1 = unpack.low(ys), e2 = unpack.next(xs), e3 = unpack.next(ys);
           float c[4];
           mma16816(c, a0, a1, a2, a3, qf[i][0][0], qf[i][0][1], zero);
           mma16816(c, a0, a1, a2, a3, qf[i][0][2], qf[i][0][3], c);
@@ -410,7 +483,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
       }
 
       // ---- the running softmax of queries 2t and 2t + 1
-      const bool edge = key + WK > key1 || key + WK - 1 > w.len - w.n + tok0;
+      const bool edge = key + WK > key1 || key + WK - 1 > edge_key;
       if (edge) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -428,7 +501,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
         top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 8));
         top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 16)) * rs[i];
       }
-      if (__any_sync(~0u, top[0] > m[0] || top[1] > m[1])) {
+      if (__any_sync(~0u, top[0] > m[0] + SLACK || top[1] > m[1] + SLACK)) {
         float by[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -446,7 +519,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
       }
       const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0] - PEXP, m[1] == -INFINITY ? 0.f : m[1] - PEXP};
       // probabilities as halves, turned so that lane (g, t) has query g and keys 2t, 2t + 1 of each 8
-      __half2 hi[4], lo[4];
+      uint32_t hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -455,18 +528,12 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
           const float p1 = exp2_fast(fmaf(s[j][2 * i + 1], rs[1], -ms[1]));
           l[0] += p0;
           l[1] += p1;
-          __half2 ph, pl;
+          uint32_t ph, pl;
           split2(p0, p1, &ph, &pl);
-          hi[2 * j + i] = halves(transposed(bits(ph)));
-          lo[2 * j + i] = halves(transposed(bits(pl)));
+          hi[2 * j + i] = transposed(ph);
+          lo[2 * j + i] = transposed(pl);
         }
-      uint32_t seen = 0xffu;  // bit 2i + x: key 8i + 2t + x counts for query g
-      if (odd_scale && edge) {
-        const int last = w.len - w.n + row_token(g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (key + 8 * (i >> 1) + 2 * t + (i & 1) > last) seen &= ~(1u << i);
-      }
+      const bool fix = odd_scale && edge;
 
       // ---- o
 #pragma unroll
@@ -478,16 +545,15 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const __half2 d = halves(dw[x]);
-          const __half2 big = __hmul2(hi[x], d);
-          const __half2 rest = __hfma2(lo[x], d, __hfma2(hi[x], d, __hneg2(big)));
-          ph[x] = bits(big);
-          pl[x] = bits(rest);
+          ph[x] = mul2(hi[x], dw[x]);
+          pl[x] = fma2(lo[x], dw[x], fma2(hi[x], dw[x], neg2(ph[x])));
         }
-        if (seen != 0xffu) {  // a key that a row does not see counts nothing, whatever its scale is
+        if (fix) {  // a key that row g does not see counts nothing, whatever its scale is
+          const int last = row_last(g);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const uint32_t keep = ((seen >> (2 * x)) & 1u ? 0x0000ffffu : 0u) | ((seen >> (2 * x + 1)) & 1u ? 0xffff0000u : 0u);
+            const int k = key + 8 * x + 2 * t;
+            const uint32_t keep = (k <= last ? 0x0000ffffu : 0u) | (k + 1 <= last ? 0xffff0000u : 0u);
             ph[x] &= keep;
             pl[x] &= keep;
           }
@@ -495,11 +561,11 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t u = vw[2 * j], v = vw[2 * j + 1], us = u >> 8, vs = v >> 8;
-          const uint32_t a0 = codes0(u), a1 = codes1(u), a2 = codes0(v), a3 = codes1(v);
+          const uint32_t a0 = unpack.low(u), a1 = unpack.next(u), a2 = unpack.low(v), a3 = unpack.next(v);
+          const uint32_t c0 = unpack.low(us), c1 = unpack.next(us), c2 = unpack.low(vs), c3 = unpack.next(vs);
           mma16816(acc[i][0], a0, a1, a2, a3, ph[2 * j], ph[2 * j + 1], acc[i][0]);
-          mma16816(acc[i][0], a0, a1, a2, a3, pl[2 * j], pl[2 * j + 1], acc[i][0]);
-          const uint32_t c0 = codes0(us), c1 = codes1(us), c2 = codes0(vs), c3 = codes1(vs);
           mma16816(acc[i][1], c0, c1, c2, c3, ph[2 * j], ph[2 * j + 1], acc[i][1]);
+          mma16816(acc[i][0], a0, a1, a2, a3, pl[2 * j], pl[2 * j + 1], acc[i][0]);
           mma16816(acc[i][1], c0, c1, c2, c3, pl[2 * j], pl[2 * j + 1], acc[i][1]);
         }
       }
@@ -533,15 +599,17 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
       }
     }
     __syncthreads();
-    const bool whole = at == item_at && seg_end == item_end;
-    float* part = a.part + static_cast<size_t>(2 * blockIdx.x + (at == item_at ? 1 : 0)) * RT * (HD + 2);
+    const Place p = place;
+    const long long item_end = p.item_at + p.units;
+    const bool whole = p.at == p.item_at && item_end <= p.end;
+    float* part = a.part + static_cast<size_t>(2 * blockIdx.x + (p.at == p.item_at ? 1 : 0)) * RT * (HD + 2);
     auto write = [&](int r, int c4, float M, float L, float4 o) {
-      const int tk = tok0 + r / width, hh = h * a.group + head0 + r % width;
+      const int tk = p.w.first + tok0 + r / width, hh = p.h * a.group + head0 + r % width;
       const float inv = M == -INFINITY ? 0.f : 1.f / L;
-      reinterpret_cast<float4*>(a.o + static_cast<size_t>(w.first + tk) * a.o_ld + static_cast<size_t>(hh) * HD)[c4] =
+      reinterpret_cast<float4*>(a.o + static_cast<size_t>(tk) * a.o_ld + static_cast<size_t>(hh) * HD)[c4] =
           make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
       if (a.lse && c4 == 0)
-        a.lse[static_cast<size_t>(w.first + tk) * a.c.kv_heads * a.group + hh] =
+        a.lse[static_cast<size_t>(tk) * a.c.kv_heads * a.group + hh] =
             M == -INFINITY ? -INFINITY : M * 0.69314718055994531f + logf(L);
     };
     for (int i = tid; i < RT * HD / 4; i += W * 32) {
@@ -573,7 +641,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
     }
     if (!whole) {
       // ---- the last of the item's CTAs to arrive joins the parts
-      const int first_cta = kv_cta_of(item_at, total, ctas), last_cta = kv_cta_of(item_end - 1, total, ctas);
+      const int first_cta = kv_cta_of(p.item_at, p.total, p.ctas), last_cta = kv_cta_of(item_end - 1, p.total, p.ctas);
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -589,9 +657,9 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
           for (int x = first_cta; x <= last_cta; ++x) {
-            const float* p = a.part + static_cast<size_t>(2 * x + (x == first_cta ? 1 : 0)) * RT * (HD + 2);
-            const float pm = __ldcg(p + RT * HD + r), pl = __ldcg(p + RT * HD + RT + r);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(p) + i);
+            const float* y0 = a.part + static_cast<size_t>(2 * x + (x == first_cta ? 1 : 0)) * RT * (HD + 2);
+            const float pm = __ldcg(y0 + RT * HD + r), pl = __ldcg(y0 + RT * HD + RT + r);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(y0) + i);
             const float now = fmaxf(M, pm), ns = now == -INFINITY ? 0.f : now;
             const float old = exp2_fast(M - ns), by = exp2_fast(pm - ns);
             M = now;
@@ -605,24 +673,29 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
         }
       }
     }
-    __syncthreads();  // the shared memory is the rings again
-
     // ---- the next item: the next tile of rows, head, sequence that has any
-    at = seg_end;
-    if (at < end) {
-      item_at = item_end;
-      if (++tile == w.tiles) {
-        tile = 0;
-        if (++h == a.c.kv_heads) {
-          h = 0;
+    if (item_end >= p.end) return;
+    __syncthreads();  // all have read the place, and the shared memory is the rings again
+    if (tid == 0) {
+      Place& n = place;
+      n.at = n.item_at = item_end;
+      if (++n.tile == n.w.tiles) {
+        n.tile = 0;
+        if (++n.h == a.c.kv_heads) {
+          n.h = 0;
           do {  // units remain, so a sequence with rows does (were the lengths left alone meanwhile)
-            if (++b >= a.s.seqs) return;
-            w = kv_rows(a.s, a.c.page, a.group, RT, b, a.err);
-          } while (w.tiles == 0);
+            if (++n.b >= a.s.seqs) {
+              n.b = -1;
+              break;
+            }
+            n.w = kv_rows(a.s, a.c.page, a.group, RT, n.b, a.err);
+          } while (n.w.tiles == 0);
         }
       }
-      units = kv_run_units(w, tile / w.parts, UNIT);
+      if (n.b >= 0) n.units = kv_run_units(n.w, n.tile / n.w.parts, UNIT);
     }
+    __syncthreads();
+    if (place.b < 0) return;
   }
 }
 
@@ -678,6 +751,7 @@ extern "C" int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const g
   if (reinterpret_cast<uintptr_t>(lse) & 3) return no("lse must be 4-byte aligned");
   const int group = num_heads / cache->num_kv_heads;
   if (static_cast<long long>(batch->num_rows) * group > 0x40000000) return no("too many query rows");
+  if (glc::kv_pools(*cache).chunk * cache->num_kv_heads > 0xffffffffu) return no("a page must stay below 4 GB");
   if (batch->num_rows == 0 || batch->num_seqs == 0) return GLC_OK;
   glc::DeviceScope on(c);
   glc::AttnKv a;
@@ -693,6 +767,8 @@ extern "C" int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const g
   a.part = nullptr;
   a.count = c->kv_count;
   a.err = c->d_err;
+  a.k1024 = 0x64006400u;
+  a.less72 = 0xd480d480u;
   // the cache's share of the traffic depends on lengths that the host does not have
   glc::ProfScope prof(c, glc::PROF_OTHER, 8.0 * batch->num_rows * width, c->stream);
   switch (cache->head_dim) {

@@ -209,31 +209,23 @@ struct KvTile {
   static constexpr int CODES = KV_WK * ROW;
   static constexpr int SCALES = KV_WK * NB * 2;
   static constexpr int BYTES = 2 * (CODES + SCALES);
-  static constexpr int CODE_PIECES = KV_WK * NB;  // of one side
-  static constexpr int SCALE_PIECES = 8 * NB;     // of both sides
+  // 8 lanes copy one side of one group of 16 tokens, in 16-byte pieces: lane i
+  // the pieces i + 8 j of the codes, and piece i of the scales if there is one.
+  static constexpr int LANE_PIECES = 2 * NB;
+  static constexpr int GROUP_SCALES = 2 * NB;
+  static_assert(16 * ROW == 8 * LANE_PIECES * 16, "a group's codes");
 
-  // Byte of piece `ch` of a token.  The 16-byte pieces are swizzled so that a
-  // piece of 8 tokens falls in 8 different quads of banks.
+  // Byte of piece `ch` of a token.  The pieces are swizzled so that a piece of 8
+  // tokens falls in 8 different quads of banks.
   static KV_HD int code_at(int token, int ch) {
     return token * ROW + 16 * (HD == 128 ? ch ^ ((token >> 1) & 3) : HD == 64 ? ch ^ ((token >> 2) & 1) : ch);
   }
-  // Piece id of the codes of a side: its token and where it comes from (relative
-  // to its token's codes) and goes to.
-  static KV_HD void code_piece(int id, int* token, int* from, int* to) {
-    const int tk = id / NB, ch = id - tk * NB;
-    *token = tk;
-    *from = 16 * ch;
-    *to = code_at(tk, ch);
-  }
-  // Piece id of the scales: its side, its group of 16 tokens, where it comes
-  // from (relative to the group's scales) and goes to (in the tile).
-  static KV_HD void scale_piece(int id, int* side, int* grp, int* from, int* to) {
-    *side = id / (4 * NB);
-    const int i = id - *side * 4 * NB;
-    *grp = i / (2 * NB);
-    *from = 16 * (i - *grp * 2 * NB);
-    *to = 2 * CODES + *side * SCALES + 16 * i;
-  }
+  // Where piece i + 8 j of the codes goes, relative to piece i's unswizzled
+  // place: the tokens of 8 pieces in a row share their swizzle.
+  static KV_HD int swizzle(int j) { return HD == 128 ? (j & 3) << 4 : HD == 64 ? (j & 1) << 4 : 0; }
+  // The first byte of a side of a group in the tile: of its codes and scales.
+  static KV_HD int codes_of(int side, int grp) { return side * CODES + grp * 16 * ROW; }
+  static KV_HD int scales_of(int side, int grp) { return 2 * CODES + side * SCALES + grp * 32 * NB; }
 };
 
 // The page (index in the sequence) and the slot in it, both in groups of 16

@@ -91,25 +91,29 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int rt, int warps, int gr
               base[i] = (ok[i] ? static_cast<size_t>(p) * c.kv_heads * c.chunk : 0) + h * c.chunk;
             }
           }
-          for (int id = 0; id < Tile::CODE_PIECES; ++id) {
-            int tk, from, to;
-            Tile::code_piece(id, &tk, &from, &to);
-            const int i = tk >> 4;
-            if (to < 0 || to + 16 > Tile::CODES || to % 16 || !to_all.insert(to).second) return 8;
-            if (!ok[i] || key + tk >= key1) continue;
-            const size_t src = base[i] + static_cast<size_t>(g[i].slot * 16 + (tk & 15)) * Tile::ROW + from;
-            if (src + 16 > pool || src % 16) return 10;
-            if ((src - base[i]) + 16 > static_cast<size_t>(c.scales_at)) return 11;
-            if (from == 0) ++count[key + tk];
+          for (int lane = 0; lane < 32; ++lane) {
+            const int lane8 = lane & 7, side = lane >> 4, i = (lane >> 3) & 1;
+            for (int j = 0; j < Tile::LANE_PIECES; ++j) {
+              const int to = Tile::codes_of(side, i) + ((lane8 * 16) ^ Tile::swizzle(j & 3)) + 128 * j;
+              const int token = (lane8 + 8 * j) * 16 / Tile::ROW, ch = (lane8 + 8 * j) % Tile::NB;
+              if (to % 16 || !to_all.insert(to).second) return 8;
+              if (to != side * Tile::CODES + Tile::code_at(16 * i + token, ch)) return 9;
+              if (!ok[i]) continue;
+              const size_t src = base[i] + static_cast<size_t>(g[i].slot) * 16 * Tile::ROW + lane8 * 16 + 128 * j;
+              if (src + 16 > pool || src % 16) return 10;
+              if (src - base[i] != static_cast<size_t>((key + 16 * i) % c.page + token) * Tile::ROW + 16 * ch) return 11;
+              if (src - base[i] + 16 > static_cast<size_t>(c.scales_at)) return 11;
+              if (side == 0 && ch == 0 && key + 16 * i + token < key1) ++count[key + 16 * i + token];
+            }
+            if (lane8 < Tile::GROUP_SCALES) {
+              const int to = Tile::scales_of(side, i) + lane8 * 16;
+              if (to < 2 * Tile::CODES || to + 16 > Tile::BYTES || !to_all.insert(to).second) return 12;
+              if (!ok[i]) continue;
+              const size_t src = base[i] + c.scales_at + static_cast<size_t>(g[i].slot) * 32 * Tile::NB + lane8 * 16;
+              if (src + 16 > base[i] + c.chunk || src + 16 > pool || src % 16) return 13;
+            }
           }
-          for (int id = 0; id < Tile::SCALE_PIECES; ++id) {
-            int side, grp, from, to;
-            Tile::scale_piece(id, &side, &grp, &from, &to);
-            if (to < 2 * Tile::CODES || to + 16 > Tile::BYTES || !to_all.insert(to).second) return 12;
-            if (!ok[grp]) continue;
-            const size_t src = base[grp] + c.scales_at + static_cast<size_t>(g[grp].slot) * 32 * Tile::NB + from;
-            if (src + 16 > base[grp] + c.chunk || src + 16 > pool || src % 16) return 13;
-          }
+          if (to_all.size() * 16 != Tile::BYTES) return 23;
           for (int i = 0; i < 2; ++i) g[i].advance(step_pages, step_slot, page16);
         }
       }
