@@ -18,7 +18,7 @@
 // the product over its 32 elements, a value's before it, on the probabilities'
 // halves (hi' = hi d, lo' = lo d + the exact rest fma(hi, d, -hi')).
 //
-// A work item is a sequence, a KV head and 8 query rows ((new token, head of
+// A work item is a sequence, a KV head and 8 to 32 query rows ((new token, head of
 // the KV head's group) pairs); its keys are cut into units, the units of all
 // items laid end to end and dealt out evenly over the CTAs, so that lengths
 // may differ and a single long sequence fills the device.  Each warp walks its
@@ -50,18 +50,20 @@ struct AttnKv {
   uint32_t k1024, less72;  // pairs of halves: 1024, -72
 };
 
-template <int HD, int W>
+// NQ: query tiles of 8 rows of an item; W: warps.
+template <int HD, int NQ, int W>
 struct Shape {
   using Tile = KvTile<HD>;
   static constexpr int NB = Tile::NB;
-  static constexpr int RT = 8;  // query rows of an item
+  static constexpr int RT = 8 * NQ;  // query rows of an item
   static constexpr int STAGES = HD >= 96 ? 2 : 3;
-  static constexpr int PER_SM = 16 / W;  // CTAs: 16 warps of 128 registers
-  static constexpr int KS = NB == 3 ? 4 : NB;  // floats of a key's scales
-  static constexpr int SCALES = WK * KS * 4 + NB * WK * 2;  // a tile's scales as the products take them
+  // CTAs of an SM: 20 warps of 96 registers, or 12 of 168 with more rows
+  static constexpr int PER_SM = W == 16 ? 1 : (NQ == 1 ? 20 : 12) / W;
+  static constexpr int SCALES = WK * NB * 6;  // a tile's scales as the products take them
   static constexpr int WARP = STAGES * Tile::BYTES + SCALES;
-  static constexpr int JOIN = W * RT * (HD + 2) * 4;  // the warps' (o, m, l), in the rings' place
-  static constexpr int SMEM = W * WARP > JOIN ? W * WARP : JOIN;
+  static constexpr int QUERIES = NQ * NB * 1024;  // the queries as operands
+  static constexpr int JOIN = W * RT * (HD + 2) * 4;  // the warps' (o, m, l), in the place of all this
+  static constexpr int SMEM = QUERIES + W * WARP > JOIN ? QUERIES + W * WARP : JOIN;
   static_assert(WARP % 16 == 0, "rings start on 16 bytes");
 };
 
@@ -173,10 +175,22 @@ struct Unpack {
   }
 };
 
-template <int HD, int W>
-__global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_kernel(const AttnKv a) {
+// (M, L, o) += the part (m, l, y)
+__device__ __forceinline__ void add_part(float m, float l, float4 y, float* M, float* L, float4* o) {
+  const float now = fmaxf(*M, m), ns = now == -INFINITY ? 0.f : now;
+  const float old = exp2_fast(*M - ns), by = exp2_fast(m - ns);
+  *M = now;
+  *L = fmaf(l, by, *L * old);
+  o->x = fmaf(y.x, by, o->x * old);
+  o->y = fmaf(y.y, by, o->y * old);
+  o->z = fmaf(y.z, by, o->z * old);
+  o->w = fmaf(y.w, by, o->w * old);
+}
+
+template <int HD, int NQ, int W>
+__global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv_kernel(const AttnKv a) {
   GLC_PDL_ENTRY();
-  using S = Shape<HD, W>;
+  using S = Shape<HD, NQ, W>;
   using Tile = KvTile<HD>;
   constexpr int NB = S::NB, RT = S::RT, STAGES = S::STAGES, UNIT = W * WK;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -189,6 +203,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
   __shared__ Place place;
   __shared__ long long sum_s[W];
   __shared__ int last_s;
+  __shared__ __align__(16) float rs_s[RT];  // what a row's products are short of its scores
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
 
@@ -245,9 +260,10 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
     if (place.b < 0) return;  // not reached, were the lengths left alone meanwhile
   }
 
-  uint8_t* ring = smem + warp * S::WARP;
-  float* kscale = reinterpret_cast<float*>(ring + STAGES * Tile::BYTES);            // [key][KS]
-  __half* vscale = reinterpret_cast<__half*>(ring + STAGES * Tile::BYTES + WK * S::KS * 4);  // [block][t][8 keys][pair]
+  uint4* queries = reinterpret_cast<uint4*>(smem);  // [query tile][block][half of it][lane]: hi, hi, lo, lo
+  uint8_t* ring = smem + S::QUERIES + warp * S::WARP;
+  float* kscale = reinterpret_cast<float*>(ring + STAGES * Tile::BYTES);                   // [block][key % 8][key / 8]
+  __half* vscale = reinterpret_cast<__half*>(ring + STAGES * Tile::BYTES + WK * NB * 4);  // [block][pair % 4][key / 8][2]
   const uint32_t ring_u = smem_u32(ring);
   const int page16 = a.c.page >> 4;
   const uint32_t page_bytes = static_cast<uint32_t>(a.c.chunk * a.c.kv_heads);
@@ -321,15 +337,13 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
-    // ---- the queries as operands: lane (g, t) holds elements 8t .. 8t + 7 of
-    // each block of row g, and of columns 2t and 2t + 1 what goes by query
-    uint32_t qf[NB][2][4];  // per block and half of it: hi, hi, lo, lo
-    float rs[2];            // what a product is short of s: the row's power of two and scale2
-    int last_key[2];        // the last key the row sees
-    {
-      const int my_row = g < rows ? g : 0, my_tok = tok0 + my_row / width, my_head = head0 + my_row % width;
+    // ---- the queries as operands, a tile of 8 rows per warp in turn: lane (g, t)
+    // has elements 8t .. 8t + 7 of each block of row g, in the order in which the
+    // codes of 8 elements come apart: (0,4), (1,5); (2,6), (3,7)
+    for (int n = warp; n < NQ; n += W) {
+      const int r = 8 * n + g < rows ? 8 * n + g : 0, token = tok0 + r / width, hh = head0 + r % width;
       const float* qp =
-          a.q + static_cast<size_t>(place.w.first + my_tok) * a.q_ld + static_cast<size_t>(place.h * a.group + my_head) * HD;
+          a.q + static_cast<size_t>(place.w.first + token) * a.q_ld + static_cast<size_t>(place.h * a.group + hh) * HD;
       float x[NB][8], top = 0.f;
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
@@ -346,35 +360,37 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
       int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
       e = e < -100 ? -100 : e > 126 ? 126 : e;
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
-      const float my_rs = a.scale2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * 0.0001220703125f;  // 2^(e - 13)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        rs[i] = __shfl_sync(~0u, my_rs, 4 * (2 * t + i));
-        last_key[i] = row_last(2 * t + i);
-      }
+      if (t == 0) rs_s[8 * n + g] = a.scale2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * 0.0001220703125f;  // 2^(e - 13)
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[i][j] *= up;
-        // in the order in which the codes of 8 elements come apart: (0,4), (1,5); (2,6), (3,7)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          split2(x[i][2 * j], x[i][2 * j + 4], &qf[i][j][0], &qf[i][j][2]);
-          split2(x[i][2 * j + 1], x[i][2 * j + 5], &qf[i][j][1], &qf[i][j][3]);
+          uint4 q;
+          split2(x[i][2 * j], x[i][2 * j + 4], &q.x, &q.z);
+          split2(x[i][2 * j + 1], x[i][2 * j + 5], &q.y, &q.w);
+          queries[((n * NB + i) * 2 + j) * 32 + lane] = q;
         }
       }
     }
+    __syncthreads();
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 
     // rows: elements 4g + e of a block, columns: queries; [..][j][0..1] is e = 2j, [2..3] e = 2j + 1
-    float acc[NB][2][4];
+    float acc[NQ][NB][2][4];
+    float m[NQ][2], l[NQ][2];  // of queries 8n + 2t and 8n + 2t + 1
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int n = 0; n < NQ; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) acc[i][j][x] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[n][i][j][x] = 0.f;
+    }
     // m is raised only when a score passes it by more than 2^SLACK, so that the
     // sums are seldom rescaled; probabilities are held at 2^PEXP and value scales
     // at 2^vexp times their size: their products stay below 2^15, and lo and lo'
@@ -402,17 +418,13 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
 #pragma unroll
           for (int i = 0; i < (NB + 1) / 2; ++i) kd[i] = vd[i] = 0;
         }
-        float kf[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t big = 0;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          kf[i] = half_float(i & 1 ? kd[i / 2] >> 16 : kd[i / 2]);
+          kscale[(i * 8 + lane8) * 4 + (lane >> 3)] = half_float(i & 1 ? kd[i / 2] >> 16 : kd[i / 2]);
           const uint32_t mag = (i & 1 ? vd[i / 2] >> 16 : vd[i / 2]) & 0x7fffu;
           big = big > mag ? big : mag;
         }
-        if constexpr (S::KS == 4) *reinterpret_cast<float4*>(kscale + lane * 4) = make_float4(kf[0], kf[1], kf[2], kf[3]);
-        else if constexpr (S::KS == 2) *reinterpret_cast<float2*>(kscale + lane * 2) = make_float2(kf[0], kf[1]);
-        else kscale[lane] = kf[0];
         big = __reduce_max_sync(~0u, big);
         odd_scale = big > 0x7bffu;
         if (big > vtop) {  // the same for the whole warp
@@ -422,11 +434,13 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
           const int now = 4 - e;
           const float by = vtop ? __uint_as_float(static_cast<uint32_t>(127 + now - vexp) << 23) : 0.f;
 #pragma unroll
-          for (int i = 0; i < NB; ++i)
+          for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int i = 0; i < NB; ++i)
 #pragma unroll
-              for (int x = 0; x < 4; ++x) acc[i][j][x] *= by;
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[n][i][j][x] *= by;
           vexp = now;
           vtop = e + 3 > 15 ? 0x7fffu : (static_cast<uint32_t>(e + 3 + 15) << 10) - 1;
           // 2^vexp as two halves, since 2^19 is none
@@ -445,128 +459,142 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
       __syncwarp();
 
       // ---- s of keys 16 j + g (x = 0, 1: queries 2t, 2t + 1) and 16 j + 8 + g (x = 2, 3)
-      float s[2][4];
+      float s[NQ][2][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        constexpr int PAIRS = (NB * 2 + 3) / 4;  // ldmatrix x4 per 16 keys: (8 keys, block) matrices
-        uint32_t kw[PAIRS][4];
+      for (int i = 0; i < NB; ++i) {
+        uint32_t kw[4];  // codes of elements 8t .. 8t + 7 of the block, keys 8x + g
+        ldsm4(kw, from + Tile::code_at(lane, i));
+        const float4 d = *reinterpret_cast<const float4*>(kscale + (i * 8 + g) * 4);
+        uint32_t ka[2][8];
 #pragma unroll
-        for (int p = 0; p < PAIRS; ++p) {
-          const int mi = p * 4 + (lane >> 3);
-          const int tl = mi / NB < 2 ? mi / NB : 0, bl = mi / NB < 2 ? mi % NB : 0;
-          ldsm4(kw[p], from + Tile::code_at(16 * j + 8 * tl + (lane & 7), bl));
-        }
-        float d0[4], d1[4];
-        if constexpr (NB >= 3) {
-          *reinterpret_cast<float4*>(d0) = *reinterpret_cast<const float4*>(kscale + (16 * j + g) * 4);
-          *reinterpret_cast<float4*>(d1) = *reinterpret_cast<const float4*>(kscale + (16 * j + 8 + g) * 4);
-        } else if constexpr (NB == 2) {
-          *reinterpret_cast<float2*>(d0) = *reinterpret_cast<const float2*>(kscale + (16 * j + g) * 2);
-          *reinterpret_cast<float2*>(d1) = *reinterpret_cast<const float2*>(kscale + (16 * j + 8 + g) * 2);
-        } else {
-          d0[0] = kscale[16 * j + g];
-          d1[0] = kscale[16 * j + 8 + g];
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t x = kw[2 * j], y = kw[2 * j + 1], xs = x >> 8, ys = y >> 8;
+          ka[j][0] = unpack.low(x), ka[j][1] = unpack.low(y), ka[j][2] = unpack.next(x), ka[j][3] = unpack.next(y);
+          ka[j][4] = unpack.low(xs), ka[j][5] = unpack.low(ys), ka[j][6] = unpack.next(xs), ka[j][7] = unpack.next(ys);
         }
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const uint32_t x = kw[i >> 2][i & 3], y = kw[(NB + i) >> 2][(NB + i) & 3], xs = x >> 8, ys = y >> 8;
-          const uint32_t a0 = unpack.low(x), a1 = unpack.low(y), a2 = unpack.next(x), a3 = unpack.next(y);
-          const uint32_t e0 = unpack.low(xs), e1 = unpack.low(ys), e2 = unpack.next(xs), e3 = unpack.next(ys);
-          float c[4];
-          mma16816(c, a0, a1, a2, a3, qf[i][0][0], qf[i][0][1], zero);
-          mma16816(c, a0, a1, a2, a3, qf[i][0][2], qf[i][0][3], c);
-          mma16816(c, e0, e1, e2, e3, qf[i][1][0], qf[i][1][1], c);
-          mma16816(c, e0, e1, e2, e3, qf[i][1][2], qf[i][1][3], c);
+        for (int n = 0; n < NQ; ++n) {
+          const uint4 q0 = queries[((n * NB + i) * 2) * 32 + lane], q1 = queries[((n * NB + i) * 2 + 1) * 32 + lane];
+          float c[2][4];
 #pragma unroll
-          for (int z = 0; z < 4; ++z) s[j][z] = i ? fmaf(z < 2 ? d0[i] : d1[i], c[z], s[j][z]) : (z < 2 ? d0[0] : d1[0]) * c[z];
-        }
-      }
-
-      // ---- the running softmax of queries 2t and 2t + 1
-      const bool edge = key + WK > key1 || key + WK - 1 > edge_key;
-      if (edge) {
+          for (int j = 0; j < 2; ++j) mma16816(c[j], ka[j][0], ka[j][1], ka[j][2], ka[j][3], q0.x, q0.y, zero);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < 2; ++j) mma16816(c[j], ka[j][4], ka[j][5], ka[j][6], ka[j][7], q1.x, q1.y, c[j]);
 #pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const int k = key + 16 * j + (z >> 1) * 8 + g;
-            if (k > last_key[z & 1] || k >= key1) s[j][z] = -INFINITY;
-          }
-      }
-      float top[2];
+          for (int j = 0; j < 2; ++j) mma16816(c[j], ka[j][0], ka[j][1], ka[j][2], ka[j][3], q0.z, q0.w, c[j]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[i] = fmaxf(fmaxf(s[0][i], s[0][i + 2]), fmaxf(s[1][i], s[1][i + 2]));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 4));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 8));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 16)) * rs[i];
-      }
-      if (__any_sync(~0u, top[0] > m[0] + SLACK || top[1] > m[1] + SLACK)) {
-        float by[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float now = fmaxf(m[i], top[i]);
-          by[i] = now == -INFINITY ? 0.f : exp2_fast(m[i] - now);
-          m[i] = now;
-          l[i] *= by[i];
-        }
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
+          for (int j = 0; j < 2; ++j) mma16816(c[j], ka[j][4], ka[j][5], ka[j][6], ka[j][7], q1.z, q1.w, c[j]);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) acc[i][j][x] *= by[x & 1];
+            for (int z = 0; z < 4; ++z) {
+              const float dd = j ? (z < 2 ? d.z : d.w) : (z < 2 ? d.x : d.y);
+              s[n][j][z] = i ? fmaf(dd, c[j][z], s[n][j][z]) : dd * c[j][z];
+            }
+        }
       }
-      const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0] - PEXP, m[1] == -INFINITY ? 0.f : m[1] - PEXP};
-      // probabilities as halves, turned so that lane (g, t) has query g and keys 2t, 2t + 1 of each 8
-      uint32_t hi[4], lo[4];
+
+      // ---- the running softmax of queries 8n + 2t and 8n + 2t + 1
+      const bool edge = key + WK > key1 || key + WK - 1 > edge_key;
+      // probabilities as halves, turned so that lane (g, t) has query 8n + g and keys 2t, 2t + 1 of each 8
+      uint32_t hi[NQ][4], lo[NQ][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int n = 0; n < NQ; ++n) {
+        const float2 rs = *reinterpret_cast<const float2*>(rs_s + 8 * n + 2 * t);
+        if (edge) {
+          const int last0 = row_last(8 * n + 2 * t), last1 = row_last(8 * n + 2 * t + 1);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const int k = key + 16 * j + (z >> 1) * 8 + g;
+              if (k > (z & 1 ? last1 : last0) || k >= key1) s[n][j][z] = -INFINITY;
+            }
+        }
+        float top[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float p0 = exp2_fast(fmaf(s[j][2 * i], rs[0], -ms[0]));
-          const float p1 = exp2_fast(fmaf(s[j][2 * i + 1], rs[1], -ms[1]));
-          l[0] += p0;
-          l[1] += p1;
-          uint32_t ph, pl;
-          split2(p0, p1, &ph, &pl);
-          hi[2 * j + i] = transposed(ph);
-          lo[2 * j + i] = transposed(pl);
+          top[i] = fmaxf(fmaxf(s[n][0][i], s[n][0][i + 2]), fmaxf(s[n][1][i], s[n][1][i + 2]));
+          top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 4));
+          top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 8));
+          top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 16)) * (i ? rs.y : rs.x);
         }
+        if (__any_sync(~0u, top[0] > m[n][0] + SLACK || top[1] > m[n][1] + SLACK)) {
+          float by[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float now = fmaxf(m[n][i], top[i]);
+            by[i] = now == -INFINITY ? 0.f : exp2_fast(m[n][i] - now);
+            m[n][i] = now;
+            l[n][i] *= by[i];
+          }
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) acc[n][i][j][x] *= by[x & 1];
+        }
+        const float ms[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0] - PEXP, m[n][1] == -INFINITY ? 0.f : m[n][1] - PEXP};
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float p0 = exp2_fast(fmaf(s[n][j][2 * i], rs.x, -ms[0]));
+            const float p1 = exp2_fast(fmaf(s[n][j][2 * i + 1], rs.y, -ms[1]));
+            l[n][0] += p0;
+            l[n][1] += p1;
+            uint32_t ph, pl;
+            split2(p0, p1, &ph, &pl);
+            hi[n][2 * j + i] = transposed(ph);
+            lo[n][2 * j + i] = transposed(pl);
+          }
+      }
       const bool fix = odd_scale && edge;
 
       // ---- o
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        uint32_t vw[4];  // codes of element pairs, 8 keys each
+        uint32_t vw[4];  // codes of elements 4g .. 4g + 3, keys 8x + 2t and 8x + 2t + 1
         ldsm4t(vw, from + Tile::CODES + Tile::code_at(lane, i));
         const uint4 d4 = *reinterpret_cast<const uint4*>(vscale + (i * 4 + t) * 8);
         const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w};
-        uint32_t ph[4], pl[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          ph[x] = mul2(hi[x], dw[x]);
-          pl[x] = fma2(lo[x], dw[x], fma2(hi[x], dw[x], neg2(ph[x])));
-        }
-        if (fix) {  // a key that row g does not see counts nothing, whatever its scale is
-          const int last = row_last(g);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int k = key + 8 * x + 2 * t;
-            const uint32_t keep = (k <= last ? 0x0000ffffu : 0u) | (k + 1 <= last ? 0xffff0000u : 0u);
-            ph[x] &= keep;
-            pl[x] &= keep;
-          }
-        }
+        uint32_t va[2][8];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t u = vw[2 * j], v = vw[2 * j + 1], us = u >> 8, vs = v >> 8;
-          const uint32_t a0 = unpack.low(u), a1 = unpack.next(u), a2 = unpack.low(v), a3 = unpack.next(v);
-          const uint32_t c0 = unpack.low(us), c1 = unpack.next(us), c2 = unpack.low(vs), c3 = unpack.next(vs);
-          mma16816(acc[i][0], a0, a1, a2, a3, ph[2 * j], ph[2 * j + 1], acc[i][0]);
-          mma16816(acc[i][1], c0, c1, c2, c3, ph[2 * j], ph[2 * j + 1], acc[i][1]);
-          mma16816(acc[i][0], a0, a1, a2, a3, pl[2 * j], pl[2 * j + 1], acc[i][0]);
-          mma16816(acc[i][1], c0, c1, c2, c3, pl[2 * j], pl[2 * j + 1], acc[i][1]);
+          va[j][0] = unpack.low(u), va[j][1] = unpack.next(u), va[j][2] = unpack.low(v), va[j][3] = unpack.next(v);
+          va[j][4] = unpack.low(us), va[j][5] = unpack.next(us), va[j][6] = unpack.low(vs), va[j][7] = unpack.next(vs);
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            ph[x] = mul2(hi[n][x], dw[x]);
+            pl[x] = fma2(lo[n][x], dw[x], fma2(hi[n][x], dw[x], neg2(ph[x])));
+          }
+          if (fix) {  // a key that a row does not see counts nothing, whatever its scale is
+            const int last = row_last(8 * n + g);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int k = key + 8 * x + 2 * t;
+              const uint32_t keep = (k <= last ? 0x0000ffffu : 0u) | (k + 1 <= last ? 0xffff0000u : 0u);
+              ph[x] &= keep;
+              pl[x] &= keep;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              mma16816(acc[n][i][e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], ph[2 * j],
+                       ph[2 * j + 1], acc[n][i][e]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              mma16816(acc[n][i][e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], pl[2 * j],
+                       pl[2 * j + 1], acc[n][i][e]);
+          }
         }
       }
       stage = stage == STAGES - 1 ? 0 : stage + 1;
@@ -574,28 +602,27 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
     copies_wait<0>();
 
     // ---- the warps' parts of the segment joined through shared memory
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) l[i] += __shfl_xor_sync(~0u, l[i], o);
-      l[i] *= 1.f / (1 << PEXP);
-    }
     const float down = __uint_as_float(static_cast<uint32_t>(127 - PEXP - vexp) << 23);
     __syncthreads();  // the rings are free
     float* jo = reinterpret_cast<float*>(smem) + warp * RT * HD;
     float* jm = reinterpret_cast<float*>(smem) + W * RT * HD;  // [W][RT] m, then l
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        *reinterpret_cast<float4*>(jo + (2 * t + x) * HD + 32 * i + 4 * g) =
-            make_float4(acc[i][0][x] * down, acc[i][0][2 + x] * down, acc[i][1][x] * down,
-                        acc[i][1][2 + x] * down);
-    if (g == 0) {
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          *reinterpret_cast<float4*>(jo + (8 * n + 2 * t + x) * HD + 32 * i + 4 * g) =
+              make_float4(acc[n][i][0][x] * down, acc[n][i][0][2 + x] * down, acc[n][i][1][x] * down,
+                          acc[n][i][1][2 + x] * down);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        jm[warp * RT + 2 * t + x] = m[x];
-        jm[W * RT + warp * RT + 2 * t + x] = l[x];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[n][x] += __shfl_xor_sync(~0u, l[n][x], o);
+        if (g == 0) {
+          jm[warp * RT + 8 * n + 2 * t + x] = m[n][x];
+          jm[W * RT + warp * RT + 8 * n + 2 * t + x] = l[n][x] * (1.f / (1 << PEXP));
+        }
       }
     }
     __syncthreads();
@@ -651,25 +678,38 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
       __syncthreads();
       if (last_s) {
         __threadfence();
-        for (int i = tid; i < rows * HD / 4; i += W * 32) {
+        // groups of threads take every GROUPSth part, and join through shared memory
+        constexpr int ELEMS = RT * HD / 4, GROUPS = ELEMS < W * 32 ? W * 32 / ELEMS : 1;
+        float4* so = reinterpret_cast<float4*>(smem);
+        float2* sm = reinterpret_cast<float2*>(smem + GROUPS * ELEMS * 16);
+        for (int i0 = 0; i0 < ELEMS; i0 += W * 32) {
+          const int group = GROUPS > 1 ? tid / ELEMS : 0, i = GROUPS > 1 ? tid - group * ELEMS : i0 + tid;
           const int r = i / (HD / 4), c4 = i - r * (HD / 4);
           float M = -INFINITY, L = 0.f;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int x = first_cta; x <= last_cta; ++x) {
-            const float* y0 = a.part + static_cast<size_t>(2 * x + (x == first_cta ? 1 : 0)) * RT * (HD + 2);
-            const float pm = __ldcg(y0 + RT * HD + r), pl = __ldcg(y0 + RT * HD + RT + r);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(y0) + i);
-            const float now = fmaxf(M, pm), ns = now == -INFINITY ? 0.f : now;
-            const float old = exp2_fast(M - ns), by = exp2_fast(pm - ns);
-            M = now;
-            L = fmaf(pl, by, L * old);
-            o.x = fmaf(y.x, by, o.x * old);
-            o.y = fmaf(y.y, by, o.y * old);
-            o.z = fmaf(y.z, by, o.z * old);
-            o.w = fmaf(y.w, by, o.w * old);
+          if (group < GROUPS && i < ELEMS) {
+#pragma unroll 8
+            for (int x = first_cta + group; x <= last_cta; x += GROUPS) {
+              const float* y0 = a.part + static_cast<size_t>(2 * x + (x == first_cta ? 1 : 0)) * RT * (HD + 2);
+              add_part(__ldcg(y0 + RT * HD + r), __ldcg(y0 + RT * HD + RT + r),
+                       __ldcg(reinterpret_cast<const float4*>(y0) + i), &M, &L, &o);
+            }
           }
-          write(r, c4, M, L, o);
+          if constexpr (GROUPS > 1) {
+            if (group < GROUPS) {
+              so[group * ELEMS + i] = o;
+              if (c4 == 0) sm[group * RT + r] = make_float2(M, L);
+            }
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+              for (int x = 1; x < GROUPS; ++x) {
+                const float2 ml = sm[x * RT + r];
+                add_part(ml.x, ml.y, so[x * ELEMS + i], &M, &L, &o);
+              }
+            }
+          }
+          if (group == 0 && i < ELEMS && r < rows) write(r, c4, M, L, o);
         }
       }
     }
@@ -699,13 +739,13 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, W>::PER_SM) attention_kv_ker
   }
 }
 
-template <int HD, int W>
+template <int HD, int NQ, int W>
 int launch(Context* ctx, const AttnKv& a, cudaStream_t s) {
-  using S = Shape<HD, W>;
+  using S = Shape<HD, NQ, W>;
   static thread_local int ready = -1;  // device on which the attribute is set
   if (ready != ctx->device) {
     const cudaError_t e =
-        cudaFuncSetAttribute(attention_kv_kernel<HD, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        cudaFuncSetAttribute(attention_kv_kernel<HD, NQ, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return ctx->fail_cuda(e, "attention_kv: shared memory");
     ready = ctx->device;
   }
@@ -716,18 +756,23 @@ int launch(Context* ctx, const AttnKv& a, cudaStream_t s) {
   if (rc) return rc;
   AttnKv b = a;
   b.part = static_cast<float*>(ws);
-  glc::launch_pdl(ctx, attention_kv_kernel<HD, W>, dim3(ctas), dim3(W * 32), S::SMEM, s, b);
+  glc::launch_pdl(ctx, attention_kv_kernel<HD, NQ, W>, dim3(ctas), dim3(W * 32), S::SMEM, s, b);
   GLC_LAUNCH_CHECK(ctx, "attention_kv");
   return GLC_OK;
 }
 
 template <int HD>
 int launch_for(Context* ctx, const AttnKv& a, cudaStream_t s) {
+  // Rows that share a KV head of a sequence, on average: as many query tiles in
+  // an item as they fill, since an item unpacks its keys and values once.
+  const long long rows = static_cast<long long>(a.s.rows) * a.group / a.s.seqs;
+  if (HD <= 64 && rows > 24) return launch<HD, HD <= 64 ? 4 : 2, 4>(ctx, a, s);
+  if (rows > 8) return launch<HD, 2, 4>(ctx, a, s);
   // Few items are cut between many CTAs, and few large CTAs leave fewer parts to
   // join; of many items a CTA has several, and small CTAs overlap one's joins
   // with another's copies.
   const long long items = static_cast<long long>(a.s.rows) * ((a.group + 7) / 8) * a.c.kv_heads;
-  return items >= ctx->num_sms / 2 ? launch<HD, 4>(ctx, a, s) : launch<HD, 16>(ctx, a, s);
+  return items >= ctx->num_sms / 2 ? launch<HD, 1, 4>(ctx, a, s) : launch<HD, 1, 16>(ctx, a, s);
 }
 
 }  // namespace
