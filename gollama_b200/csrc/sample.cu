@@ -1,9 +1,11 @@
 // Drawing the next token: temperature, top-k, top-p, min-p, and the inverse of
 // the kept tokens' running sum at a given random number.
 //
-// A token's weight is 2^((l - max) log2(e) / temperature) as a whole number of
-// 2^-42, so sums of weights are exact and every kernel order gives the same
-// one.  Tokens are ordered by (logit falling, index rising), a total order; the
+// A token's weight is exp((l - max) / temperature) as a whole number of 2^-42,
+// so sums of weights are exact and every order of summation gives the same one.
+// The weights themselves are good to 2^-39: with tens of thousands of tokens
+// kept, a sum that is off by 2^-25 of itself (float32 exponentials) moves past a
+// token's edge about once in a thousand rows, and that token is then another.  Tokens are ordered by (logit falling, index rising), a total order; the
 // kept ones of top-k and of top-p are each a prefix of it, so each filter is a
 // cut: its last kept token.  Nothing is sorted but the few tokens around a
 // cut: a histogram over 1024 bins of max - l finds the bin the cut falls in,
@@ -17,6 +19,7 @@
 // once; the histograms, the gathered tokens and the partial sums meet in the
 // first CTA through distributed shared memory.
 #include <cfloat>
+#include <climits>
 #include <cooperative_groups.h>
 
 #include "kv_cache.cuh"
@@ -49,7 +52,7 @@ using u64 = unsigned long long;
 
 // Position in the order: larger is earlier.
 __device__ __forceinline__ u64 order_of(float l, int index) {
-  const uint32_t b = __float_as_uint(l);
+  const uint32_t b = __float_as_uint(l + 0.f);  // -0 and 0 are equals
   const uint32_t key = b & 0x80000000u ? ~b : b | 0x80000000u;
   return (static_cast<u64>(key) << 32) | static_cast<uint32_t>(~index);
 }
@@ -59,29 +62,29 @@ __device__ __forceinline__ float logit_of(u64 order) {
 }
 __device__ __forceinline__ int index_of(u64 order) { return static_cast<int>(~static_cast<uint32_t>(order)); }
 
+constexpr int POWERS = 32;
+
 struct Weights {
-  float top, c_hi, c_lo;  // log2(e) / temperature in two floats
-  // round(2^(42 - t)), t = (top - l) * c: the fraction of t through the Taylor
-  // series of 2^f about 0 on [-1/2, 1/2] (error 2^-27), rounded to a float once,
-  // then its mantissa moved into place.  top - l rounds at random from token to
-  // token; c is held to 48 bits so that nothing is off the same way for all.
+  float top, c;         // c: 1 / temperature, for what needs no more than 24 bits
+  double dtop, inv;     // 1 / temperature
+  const double* powers; // 2^(42 - j / 32)
+  // round(2^42 exp(-y)), y = (top - l) / temperature = (32 q + j) ln2 / 32 + r with
+  // |r| <= ln2 / 64: 2^-q by a shift, 2^(-j/32) from the table, exp(-r) by four
+  // terms of its series (r^5 / 120 < 2^-39).
   __device__ __forceinline__ u64 operator()(float l) const {
     const float d = l == top ? 0.f : top - l;
-    if (!(d <= FLT_MAX)) return 0;
-    const float t = fmaf(d, c_hi, d * c_lo);
-    if (!(t < 43.f)) return 0;
-    const float n = rintf(t), f = n - t;
-    float p = 1.5252734e-5f;            // ln2^7 / 7!
-    p = fmaf(p, f, 1.5403530e-4f);      // ln2^6 / 6!
-    p = fmaf(p, f, 1.3333558e-3f);      // ln2^5 / 5!
-    p = fmaf(p, f, 9.6181291e-3f);      // ln2^4 / 4!
-    p = fmaf(p, f, 5.5504109e-2f);      // ln2^3 / 3!
-    p = fmaf(p, f, 2.4022651e-1f);      // ln2^2 / 2!
-    p = fmaf(p, f, 6.9314718e-1f);      // ln2
-    p = fmaf(p, f, 1.f);
-    const uint32_t b = __float_as_uint(p), mant = (b & 0x7fffffu) | 0x800000u;
-    const int shift = static_cast<int>(b >> 23) - 127 + 19 - static_cast<int>(n);
-    return shift >= 0 ? static_cast<u64>(mant) << shift : (mant + (1u << (-shift - 1))) >> -shift;
+    if (!(d * c < 29.8f)) return 0;  // below 2^-43; and where l is -infinity or not a number
+    const double y = (l == top ? 0.0 : dtop - static_cast<double>(l)) * inv;
+    const double k = fma(y, 32 * 1.4426950408889634, 6755399441055744.0);  // 1.5 2^52: the whole number in the low bits
+    const int n = __double2loint(k);
+    const double r = fma(k - 6755399441055744.0, -0.6931471805599453 / 32, y);
+    double e = fma(r, 1.0 / 24, -1.0 / 6);
+    e = fma(r, e, 0.5);
+    e = fma(r, e, -1.0);
+    e = fma(r, e, 1.0);
+    const double v = fma(powers[n & (POWERS - 1)], e, 4503599627370496.0);  // 2^52: the rounded value in the low bits
+    const u64 whole = static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
+    return whole >> (n >> 5);
   }
 };
 
@@ -103,12 +106,13 @@ struct Shared {
   uint32_t low[BINS], high[BINS];  // a histogram of 64-bit sums, halves apart
   u64 list[CAP], ranked[CAP];
   u64 warp_a[NW], warp_b[NW];
-  float warp_f[NW];
+  float warp_f[NW], warp_top[NW];
   int warp_n[NW];
+  double powers[POWERS];
   // what the other CTAs read
-  u64 best, total;
-  float sum;
-  int finite;
+  float top, sum;
+  int first, finite;
+  u64 total;
   int gathered[2];  // by the level's parity: a CTA may still read the last level's
   int bin;         // of the last histogram: where the cut falls,
   u64 base, all;   // what lies before that bin, and the whole sum
@@ -156,82 +160,91 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   const bool by_p = p_set < 1.f;
   const bool greedy = !(temp > 0.f) || k == 1 || p_set <= 0.f;
 
-  // ---- the logits into shared memory, with their largest and their mean
+  // ---- the logits into shared memory, with their largest, and the mean of some
   const float* src = a.logits + row * a.ld + first;
-  u64 best = 0;
-  float sum = 0.f;
+  float top = -INFINITY, sum = 0.f;
   int finite = 0;
-  auto take = [&](float l, int i) {
-    l = l != l ? -INFINITY : l + 0.f;  // -0 and 0 are equals
-    const u64 o = order_of(l, first + i);
-    best = o > best ? o : best;
+  auto some_of_mean = [&](float l) {
     if (fabsf(l) <= FLT_MAX) sum += l, ++finite;
-    return l;
   };
   if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
     const int n4 = n >> 2;
 #pragma unroll 8
     for (int i = tid; i < n4; i += NT) {
-      float4 v = __ldcs(reinterpret_cast<const float4*>(src) + i);
-      v.x = take(v.x, 4 * i);
-      v.y = take(v.y, 4 * i + 1);
-      v.z = take(v.z, 4 * i + 2);
-      v.w = take(v.w, 4 * i + 3);
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(src) + i);
+      top = fmaxf(fmaxf(top, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));  // (a NaN is passed over)
+      some_of_mean(v.x);
       reinterpret_cast<float4*>(x)[i] = v;
     }
-    for (int i = 4 * n4 + tid; i < n; i += NT) x[i] = take(src[i], i);
+    for (int i = 4 * n4 + tid; i < n; i += NT) {
+      const float l = src[i];
+      top = fmaxf(top, l);
+      some_of_mean(l);
+      x[i] = l;
+    }
   } else {
 #pragma unroll 8
-    for (int i = tid; i < n; i += NT) x[i] = take(__ldcs(src + i), i);
+    for (int i = tid; i < n; i += NT) {
+      const float l = __ldcs(src + i);
+      top = fmaxf(top, l);
+      some_of_mean(l);
+      x[i] = l;
+    }
   }
+  if (tid < POWERS) s.powers[tid] = exp2(42.0 - tid * (1.0 / POWERS));
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    const u64 y = __shfl_xor_sync(~0u, best, o);
-    best = y > best ? y : best;
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
     sum += __shfl_xor_sync(~0u, sum, o);
     finite += __shfl_xor_sync(~0u, finite, o);
   }
-  if (lane == 0) s.warp_a[warp] = best, s.warp_f[warp] = sum, s.warp_n[warp] = finite;
+  if (lane == 0) s.warp_top[warp] = top, s.warp_f[warp] = sum, s.warp_n[warp] = finite;
   __syncthreads();
   if (tid == 0) {
     for (int i = 1; i < NW; ++i) {
-      best = s.warp_a[i] > best ? s.warp_a[i] : best;
+      top = fmaxf(top, s.warp_top[i]);
       sum += s.warp_f[i];
       finite += s.warp_n[i];
     }
-    s.best = best;
+    s.top = top;
     s.sum = sum;
     s.finite = finite;
+    s.first = INT_MAX;
   }
   cluster.sync();
-  best = 0;
+  top = -INFINITY;
   sum = 0.f;
   finite = 0;
   for (int i = 0; i < ctas; ++i) {
     const Shared& o = *cluster.map_shared_rank(&s, i);
-    best = o.best > best ? o.best : best;
+    top = fmaxf(top, o.top);
     sum += o.sum;
     finite += o.finite;
   }
-  const float top = logit_of(best);
 
   auto finish = [&](int64_t token, float logp) {
     a.tokens[row] = token;
     if (a.logp) a.logp[row] = logp;
   };
   if (greedy || top == -INFINITY) {
-    if (rank == 0 && tid == 0) finish(top == -INFINITY ? -1 : index_of(best), top == -INFINITY ? -INFINITY : 0.f);
-    cluster.sync();  // the others may still read this CTA's memory
+    // the first of the largest; each CTA's own, then the first CTA that has one
+    int at = INT_MAX;
+    if (top > -INFINITY)
+      for (int i = tid; i < n; i += NT)
+        if (x[i] == top && first + i < at) at = first + i;
+    at = __reduce_min_sync(~0u, at);
+    if (lane == 0 && at != INT_MAX) atomicMin(&lead.first, at);
+    cluster.sync();
+    if (rank == 0 && tid == 0) finish(s.first == INT_MAX ? -1 : s.first, s.first == INT_MAX ? -INFINITY : 0.f);
     return;
   }
 
   Weights weight;
   weight.top = top;
-  {
-    const double c = fmin(1.4426950408889634 / static_cast<double>(temp), static_cast<double>(FLT_MAX));
-    weight.c_hi = static_cast<float>(c);
-    weight.c_lo = static_cast<float>(c - static_cast<double>(weight.c_hi));
-  }
+  weight.dtop = top;
+  weight.inv = 1.0 / static_cast<double>(temp);
+  weight.c = static_cast<float>(fmin(weight.inv, static_cast<double>(FLT_MAX)));
+  weight.powers = s.powers;
   // a token counts from this weight on; min_p >= 1 keeps the largest logit's equals
   const u64 least = min_set > 0.f && min_set < 1.f
                         ? static_cast<u64>(ceil(static_cast<double>(min_set) * 4398046511104.0))
@@ -241,23 +254,28 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   // the random number and p as 64-bit fractions; a goal is the high word of a product
   const u64 u64th = !(u > 0.f) ? 0 : u >= 1.f ? ~0ull : static_cast<u64>(static_cast<double>(u) * 18446744073709551616.0);
 
-  // ---- a filter's cut.  mass: tokens of the order before `from` (inclusive)
-  // are weighed until goal64/2^64 of them all; else they are counted to `count`.
-  // The bins cover [0, range] of top - l, the last one all that is beyond.
+  // ---- a filter's cut.  mass: the tokens of the order up to `from` are weighed
+  // until p64/2^64 of them all; else they are counted to `target`.  The bins
+  // divide [0, range] of top - l evenly, the last one has all that is beyond.
+  auto before_cut = [&](float l, int i, u64 from) {  // l is not NaN or -infinity
+    if (!from) return l > -INFINITY;
+    const float c = logit_of(from);
+    return l > c || (l == c && first + i <= index_of(from));
+  };
   auto bin_of = [&](float l, float scale) {
     const float d = l == top ? 0.f : top - l;
-    const int b = static_cast<int>(d * scale);  // not a number (0 * inf) is 0, too large the largest
-    return b < BINS - 1 ? (b < 0 ? 0 : b) : BINS - 1;
+    // a whole number in the low bits of the sum; beyond 2^23 of them it stays the largest
+    const int b = static_cast<int>(__float_as_uint(fmaf(d, scale, 8388608.f)) - 0x4b000000u);
+    return b < 0 || b >= BINS ? BINS - 1 : b;
   };
   // tokens the level looks at: of bin `bin0` alone once level > 0, and of them
   // those whose order has the prefix for its bits from `known` on
   auto digit_of = [&](float l, int i, u64 from, float scale, int level, int bin0, int shift, int known, u64 prefix) {
-    if (l == -INFINITY) return -1;
-    const u64 o = order_of(l, first + i);
-    if (o < from) return -1;
+    if (!before_cut(l, i, from)) return -1;
     const int b = bin_of(l, scale);
     if (level == 0) return b;
     if (b != bin0) return -1;
+    const u64 o = order_of(l, first + i);
     if (known < 64 && (o >> known) != prefix) return -1;
     return (BINS - 1) - static_cast<int>((o >> shift) & (BINS - 1));
   };
@@ -415,8 +433,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   }
   if (by_p) {
     bool listed;
-    // beyond 43 / c every weight is 0; half as far behind the mean as before it, few tokens are left
-    float r = 43.f / weight.c_hi;
+    // beyond 29.8 / c every weight is 0; half as far behind the mean as before it, few tokens are left
+    float r = 29.8f / weight.c;
     if (range > 0.f && 1.5f * range < r) r = 1.5f * range;
     const float scale = r > 0.f && r <= FLT_MAX ? static_cast<float>(BINS) / r : 0.f;
     const u64 p64 = static_cast<u64>(static_cast<double>(p_set) * 18446744073709551616.0);

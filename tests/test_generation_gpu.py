@@ -487,12 +487,12 @@ def sample(ctx, x, t, k=None, p=None, m=None, u=None, ld=None, shift=0):
 
 
 def check_sample(x, t, k, p, m, u, tok, logp):
-    """A weight is off by at most 43 (2^-23 + 2^-24) ln2 + 2^-23 of itself (the
-    distance to the largest logit and its product with 1/temperature round once
-    each; then the power) and half of 2^-42 of the largest: 6e-6.  So a running sum
-    is, and a token whose interval has u within that of it is right; a token whose
-    weight or sum is that near to a cut may be in or out."""
-    tol = 6e-6
+    """A weight is off by at most 2^-39 of itself and 2^-42 of the largest, so a
+    running sum of V <= 393216 of them by 2^-39 + V 2^-42 < 1e-7 of the kept sum (the
+    largest is among them).  A token whose interval has u within that of it is right;
+    a token whose weight or sum is that near to a cut may be in or out.  logp is that
+    rounded to fp32 (a weight below 1e-5 of the largest has fewer than 25 of the 42 bits)."""
+    tol = 1e-7
     R, V = x.shape
     b = lambda a, none: np.broadcast_to(np.asarray(none if a is None else a, np.float64), (R,))  # noqa: E731
     f = lambda a, none: b(a, none).astype(np.float32).astype(np.float64)  # noqa: E731  (the settings are fp32)
