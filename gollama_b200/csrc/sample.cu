@@ -1,23 +1,27 @@
 // Drawing the next token: temperature, top-k, top-p, min-p, and the inverse of
 // the kept tokens' running sum at a given random number.
 //
-// A token's weight is exp((l - max) / temperature) as a whole number of 2^-42,
+// A token's weight is exp((l - max) / temperature) as a whole number of 2^-31,
 // so sums of weights are exact and every order of summation gives the same one.
-// The weights themselves are good to 2^-39: with tens of thousands of tokens
-// kept, a sum that is off by 2^-25 of itself (float32 exponentials) moves past a
-// token's edge about once in a thousand rows, and that token is then another.  Tokens are ordered by (logit falling, index rising), a total order; the
-// kept ones of top-k and of top-p are each a prefix of it, so each filter is a
-// cut: its last kept token.  Nothing is sorted but the few tokens around a
-// cut: a histogram over 1024 bins of max - l finds the bin the cut falls in,
-// that bin's tokens (or, for a small k, all down to it) are gathered and
-// ranked against each other.  A bin of more than 512 tokens is first narrowed
-// by the bits of the order itself, 10 at a time, which ends for any input,
-// equal logits too.  The draw itself is a sum over the kept tokens in index
-// order, taken apart in CTAs, warps and lanes.
+// It is computed in 64 bits and rounded once: with tens of thousands of tokens
+// kept, sums of float32 exponentials are off by about 2^-25 of themselves, which
+// moves past a token's edge about once in a thousand rows, and that token is
+// then another; rounding errors of 2^-32 of the largest do so once in 10^5.
 //
-// A cluster of 1 to 8 CTAs holds a row in shared memory, so the logits are read
-// once; the histograms, the gathered tokens and the partial sums meet in the
-// first CTA through distributed shared memory.
+// Tokens are ordered by (logit falling, index rising), a total order; the kept
+// ones of top-k and of top-p are each a prefix of it, so each filter is a cut:
+// its last kept token.  Nothing is sorted but the few tokens around a cut: a
+// histogram finds the bin the cut falls in (of top-k: bins of max - l; of top-p:
+// 64 bins per factor of two of the weight), that bin's tokens (or, for a small
+// k, all down to it) are gathered and ranked against each other.  A bin of more
+// than 512 tokens is first narrowed by the bits of the order itself, 10 at a
+// time, which ends for any input, equal logits too.  The draw itself is a sum
+// over the kept tokens in index order, taken apart in CTAs, warps and lanes.
+//
+// A cluster of CTAs holds a row in shared memory, first its logits and then, in
+// their place, the weights, so each is read and computed once; the histograms,
+// the gathered tokens and the partial sums meet through distributed shared
+// memory.  Only what is near a cut reads a logit again.
 #include <cfloat>
 #include <climits>
 #include <cooperative_groups.h>
@@ -30,10 +34,14 @@ namespace glc {
 namespace {
 
 constexpr int NT = 512, NW = NT / 32;
-constexpr int BINS = 1024;
-constexpr int CAP = NT;  // tokens that are ranked at once, one per thread
+constexpr int BINS = 2048, PER_BIN = BINS / NT;
+constexpr int CAP = NT;          // tokens that are ranked at once, one per thread
+constexpr int POWERS = 64;       // bins per factor of two of the weight
+constexpr int DIGIT = 10;        // bits of the order per step of narrowing
 constexpr int MAX_CLUSTER = 8;
-constexpr int SLICE_MAX = 49152;  // tokens of a CTA: 192 KB of its shared memory
+constexpr int SLICE_MAX = 49152; // tokens of a CTA: 192 KB of its shared memory
+constexpr uint32_t ONE = 1u << 31;  // the largest weight
+static_assert((1 << DIGIT) <= BINS && 32 * POWERS <= BINS, "digits and weights have a bin");
 
 struct Sample {
   const float* logits;
@@ -62,29 +70,29 @@ __device__ __forceinline__ float logit_of(u64 order) {
 }
 __device__ __forceinline__ int index_of(u64 order) { return static_cast<int>(~static_cast<uint32_t>(order)); }
 
-constexpr int POWERS = 32;
-
 struct Weights {
-  float top, c;         // c: 1 / temperature, for what needs no more than 24 bits
-  double dtop, inv;     // 1 / temperature
-  const double* powers; // 2^(42 - j / 32)
-  // round(2^42 exp(-y)), y = (top - l) / temperature = (32 q + j) ln2 / 32 + r with
-  // |r| <= ln2 / 64: 2^-q by a shift, 2^(-j/32) from the table, exp(-r) by four
-  // terms of its series (r^5 / 120 < 2^-39).
-  __device__ __forceinline__ u64 operator()(float l) const {
-    const float d = l == top ? 0.f : top - l;
-    if (!(d * c < 29.8f)) return 0;  // below 2^-43; and where l is -infinity or not a number
-    const double y = (l == top ? 0.0 : dtop - static_cast<double>(l)) * inv;
-    const double k = fma(y, 32 * 1.4426950408889634, 6755399441055744.0);  // 1.5 2^52: the whole number in the low bits
-    const int n = __double2loint(k);
-    const double r = fma(k - 6755399441055744.0, -0.6931471805599453 / 32, y);
+  float top, c;          // c: 1 / temperature, for what needs no more than 24 bits
+  double dtop, inv;      // 1 / temperature
+  const double* powers;  // 2^(42 - j / 64)
+  // round(2^31 exp(-y)), y = (top - l) / temperature = (64 q + j) ln2 / 64 + r with
+  // |r| <= ln2 / 128: 2^-q by a shift, 2^(-j/64) from the table, exp(-r) by four
+  // terms of its series (r^5 / 120 < 2^-44).  *bin: 64 q + j.  A logit that is
+  // -infinity or not a number has weight 0.
+  __device__ __forceinline__ uint32_t operator()(float l, int* bin) const {
+    const bool some = (top - l) * c < 22.17f;  // else it rounds to 0, and n stays below 32 * 64
+    const double y = (dtop - static_cast<double>(l)) * inv;
+    const double k = fma(y, POWERS * 1.4426950408889634, 6755399441055744.0);  // 1.5 2^52: the whole number in the low bits
+    const int n = some ? __double2loint(k) : 32 * POWERS - 1;
+    const double r = fma(k - 6755399441055744.0, -0.6931471805599453 / POWERS, y);
     double e = fma(r, 1.0 / 24, -1.0 / 6);
     e = fma(r, e, 0.5);
     e = fma(r, e, -1.0);
     e = fma(r, e, 1.0);
     const double v = fma(powers[n & (POWERS - 1)], e, 4503599627370496.0);  // 2^52: the rounded value in the low bits
     const u64 whole = static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
-    return whole >> (n >> 5);
+    const int shift = 11 + n / POWERS;
+    *bin = n;
+    return some ? static_cast<uint32_t>((whole + (1ull << (shift - 1))) >> shift) : 0;
   }
 };
 
@@ -103,22 +111,31 @@ __device__ __forceinline__ u64 warp_scan(u64 x, int lane) {
 }
 
 struct Shared {
-  uint32_t low[BINS], high[BINS];  // a histogram of 64-bit sums, halves apart
-  u64 list[CAP], ranked[CAP];
+  union {
+    uint32_t hist[2][BINS];  // sums of the low and high halves of weights
+    struct {                 // (the first CTA) gathered when the histograms have been read
+      u64 list[CAP], ranked[CAP];
+      uint32_t weights[CAP];
+    };
+  };
+  u64 sums_of[BINS];  // (the first CTA) the row's histogram
+  double powers[POWERS];
   u64 warp_a[NW], warp_b[NW];
   float warp_f[NW], warp_top[NW];
   int warp_n[NW];
-  double powers[POWERS];
-  // what the other CTAs read
-  float top, sum;
-  int first, finite;
-  u64 total;
+  // what the CTAs of the row tell each other, by their rank
+  float tops[MAX_CLUSTER], sums[MAX_CLUSTER];
+  int finites[MAX_CLUSTER];
+  u64 totals[MAX_CLUSTER];
+  // what the other CTAs read from the first
+  int first;
   int gathered[2];  // by the level's parity: a CTA may still read the last level's
-  int bin;         // of the last histogram: where the cut falls,
-  u64 base, all;   // what lies before that bin, and the whole sum
-  uint32_t in_bin; // (of a count) and what is in it
-  u64 cut;         // the last kept token of a filter
+  int bin;          // of the last histogram: where the cut falls,
+  u64 base, all;    // what lies before that bin, and the goal
+  uint32_t in_bin;  // (of a count) and what is in it
+  u64 cut;          // the last kept token of a filter
 };
+static_assert(MAX_CLUSTER <= 32, "a lane per CTA of a row");
 
 // The sum over the block's threads of x before this thread's, and of all.
 __device__ __forceinline__ u64 block_before(u64 x, u64* warps, u64* all, int lane, int warp) {
@@ -143,11 +160,13 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared& s = *reinterpret_cast<Shared*>(raw);
   float* x = reinterpret_cast<float*>(raw + (sizeof(Shared) + 15) / 16 * 16);
+  uint32_t* wt = reinterpret_cast<uint32_t*>(x);  // in the logits' place
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
   const int row = blockIdx.x / ctas;
   const int first = rank * a.slice;
   const int n = a.vocab - first < a.slice ? (a.vocab - first > 0 ? a.vocab - first : 0) : a.slice;
+  const int n4 = (n + 3) >> 2;
   Shared& lead = *cluster.map_shared_rank(&s, 0);
 
   // ---- the row's settings
@@ -165,21 +184,22 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   float top = -INFINITY, sum = 0.f;
   int finite = 0;
   auto some_of_mean = [&](float l) {
-    if (fabsf(l) <= FLT_MAX) sum += l, ++finite;
+    const bool is = fabsf(l) <= FLT_MAX;
+    sum += is ? l : 0.f;
+    finite += is;
   };
   if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-    const int n4 = n >> 2;
+    const int whole4 = n >> 2;
 #pragma unroll 8
-    for (int i = tid; i < n4; i += NT) {
+    for (int i = tid; i < whole4; i += NT) {
       const float4 v = __ldcs(reinterpret_cast<const float4*>(src) + i);
       top = fmaxf(fmaxf(top, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));  // (a NaN is passed over)
       some_of_mean(v.x);
       reinterpret_cast<float4*>(x)[i] = v;
     }
-    for (int i = 4 * n4 + tid; i < n; i += NT) {
+    for (int i = 4 * whole4 + tid; i < n; i += NT) {
       const float l = src[i];
       top = fmaxf(top, l);
-      some_of_mean(l);
       x[i] = l;
     }
   } else {
@@ -191,6 +211,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
       x[i] = l;
     }
   }
+  if (n + tid < 4 * n4) x[n + tid] = __uint_as_float(0x7fc00000u);  // the last 4 tokens are whole
   if (tid < POWERS) s.powers[tid] = exp2(42.0 - tid * (1.0 / POWERS));
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -200,26 +221,24 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   }
   if (lane == 0) s.warp_top[warp] = top, s.warp_f[warp] = sum, s.warp_n[warp] = finite;
   __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < NW; ++i) {
-      top = fmaxf(top, s.warp_top[i]);
-      sum += s.warp_f[i];
-      finite += s.warp_n[i];
-    }
-    s.top = top;
-    s.sum = sum;
-    s.finite = finite;
-    s.first = INT_MAX;
+  if (tid < ctas) {  // to each CTA of the row
+    top = s.warp_top[0], sum = s.warp_f[0], finite = s.warp_n[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) top = fmaxf(top, s.warp_top[i]), sum += s.warp_f[i], finite += s.warp_n[i];
+    Shared& o = *cluster.map_shared_rank(&s, tid);
+    o.tops[rank] = top;
+    o.sums[rank] = sum;
+    o.finites[rank] = finite;
+    if (tid == 0) s.first = INT_MAX;
   }
   cluster.sync();
   top = -INFINITY;
   sum = 0.f;
   finite = 0;
   for (int i = 0; i < ctas; ++i) {
-    const Shared& o = *cluster.map_shared_rank(&s, i);
-    top = fmaxf(top, o.top);
-    sum += o.sum;
-    finite += o.finite;
+    top = fmaxf(top, s.tops[i]);
+    sum += s.sums[i];
+    finite += s.finites[i];
   }
 
   auto finish = [&](int64_t token, float logp) {
@@ -227,16 +246,27 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     if (a.logp) a.logp[row] = logp;
   };
   if (greedy || top == -INFINITY) {
-    // the first of the largest; each CTA's own, then the first CTA that has one
+    // the first of the largest
     int at = INT_MAX;
     if (top > -INFINITY)
-      for (int i = tid; i < n; i += NT)
-        if (x[i] == top && first + i < at) at = first + i;
+      for (int i = tid; i < n4; i += NT) {
+        const float4 v = reinterpret_cast<const float4*>(x)[i];
+        const int j = v.x == top ? 0 : v.y == top ? 1 : v.z == top ? 2 : v.w == top ? 3 : 4;
+        if (j < 4 && first + 4 * i + j < at) at = first + 4 * i + j;
+      }
     at = __reduce_min_sync(~0u, at);
     if (lane == 0 && at != INT_MAX) atomicMin(&lead.first, at);
     cluster.sync();
     if (rank == 0 && tid == 0) finish(s.first == INT_MAX ? -1 : s.first, s.first == INT_MAX ? -INFINITY : 0.f);
     return;
+  }
+  const bool no_end = top > FLT_MAX;  // the infinite ones share all
+  auto plain = [&](float l) { return !no_end ? l : l > FLT_MAX ? 0.f : -INFINITY; };
+  if (no_end) {
+    for (int i = tid; i < n; i += NT) x[i] = plain(x[i]);
+    top = 0.f;
+    __syncthreads();
+    // (src is read again through plain)
   }
 
   Weights weight;
@@ -246,234 +276,330 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   weight.c = static_cast<float>(fmin(weight.inv, static_cast<double>(FLT_MAX)));
   weight.powers = s.powers;
   // a token counts from this weight on; min_p >= 1 keeps the largest logit's equals
-  const u64 least = min_set > 0.f && min_set < 1.f
-                        ? static_cast<u64>(ceil(static_cast<double>(min_set) * 4398046511104.0))
-                        : 0;
   const bool only_top = min_set >= 1.f;
-  auto enough = [&](float l, u64 w) { return w >= least && (!only_top || l == top); };
+  const uint32_t least = min_set > 0.f ? static_cast<uint32_t>(ceil(fmin(static_cast<double>(min_set), 1.0) * ONE)) : 1u;
+  auto enough = [&](uint32_t w, auto logit) { return w >= least && (!only_top || logit() == top); };
   // the random number and p as 64-bit fractions; a goal is the high word of a product
   const u64 u64th = !(u > 0.f) ? 0 : u >= 1.f ? ~0ull : static_cast<u64>(static_cast<double>(u) * 18446744073709551616.0);
+  const u64 p64 = by_p ? static_cast<u64>(static_cast<double>(fmaxf(p_set, 0.f)) * 18446744073709551616.0) : 0;
+  auto p_goal = [&](u64 all) { return __umul64hi(all, p64) + (all * p64 != 0); };  // the least whole number not below p * all
 
-  // ---- a filter's cut.  mass: the tokens of the order up to `from` are weighed
-  // until p64/2^64 of them all; else they are counted to `target`.  The bins
-  // divide [0, range] of top - l evenly, the last one has all that is beyond.
-  auto before_cut = [&](float l, int i, u64 from) {  // l is not NaN or -infinity
-    if (!from) return l > -INFINITY;
-    const float c = logit_of(from);
-    return l > c || (l == c && first + i <= index_of(from));
+  // a token of the order up to `cut` (all but NaN and -infinity where it is 0)
+  auto before_cut = [&](float l, int i, u64 cut) {
+    if (!cut) return l > -INFINITY;
+    const float c = logit_of(cut);
+    return l > c || (l == c && first + i <= index_of(cut));
   };
-  auto bin_of = [&](float l, float scale) {
-    const float d = l == top ? 0.f : top - l;
+  // bins of top - l for the count, the last one all that is beyond
+  const float range = finite > 0 ? top - sum / static_cast<float>(finite) : 0.f;
+  const float scale = range > 0.f ? static_cast<float>(BINS) / range : 0.f;
+  auto count_bin = [&](float l) {
     // a whole number in the low bits of the sum; beyond 2^23 of them it stays the largest
-    const int b = static_cast<int>(__float_as_uint(fmaf(d, scale, 8388608.f)) - 0x4b000000u);
+    const int b = static_cast<int>(__float_as_uint(fmaf(top - l, scale, 8388608.f)) - 0x4b000000u);
     return b < 0 || b >= BINS ? BINS - 1 : b;
   };
-  // tokens the level looks at: of bin `bin0` alone once level > 0, and of them
-  // those whose order has the prefix for its bits from `known` on
-  auto digit_of = [&](float l, int i, u64 from, float scale, int level, int bin0, int shift, int known, u64 prefix) {
-    if (!before_cut(l, i, from)) return -1;
-    const int b = bin_of(l, scale);
-    if (level == 0) return b;
-    if (b != bin0) return -1;
-    const u64 o = order_of(l, first + i);
-    if (known < 64 && (o >> known) != prefix) return -1;
-    return (BINS - 1) - static_cast<int>((o >> shift) & (BINS - 1));
-  };
-  // one histogram over the cluster; afterwards s.bin, s.base, s.all and
-  // s.in_bin of the first CTA hold where `target` (mass: set from its sum at
-  // level 0) falls
-  auto histogram = [&](bool mass, u64* target, u64 base, u64 p64, u64 from, float scale, int level, int bin0, int shift,
-                       int known, u64 prefix) {
-    for (int i = tid; i < BINS; i += NT) s.low[i] = s.high[i] = 0;
-    if (tid == 0) s.gathered[level & 1] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += NT) {
-      const float l = x[i];
-      const int d = digit_of(l, i, from, scale, level, bin0, shift, known, prefix);
-      if (d < 0) continue;
-      if (!mass) {
-        atomicAdd(&s.low[d], 1u);
-      } else {
-        const u64 w = weight(l);
-        if (w == 0) continue;
-        const uint32_t lo = static_cast<uint32_t>(w), hi = static_cast<uint32_t>(w >> 32);
-        const uint32_t carry = atomicAdd(&s.low[d], lo) > ~lo ? 1u : 0u;
-        if (hi + carry) atomicAdd(&s.high[d], hi + carry);
+
+  // ---- adds the CTAs' histograms up: where in the row's the sum reaches *target
+  // (with `mass` at level 0 the goal of top-p, of a count at most all there is)
+  auto locate = [&](bool mass, int level, u64 base, u64* target) {
+    cluster.sync();
+    const int share = BINS / ctas;  // of the bins, per CTA
+    for (int i = tid; i < share; i += NT) {
+      u64 lo = 0, hi = 0;
+#pragma unroll 4
+      for (int j = 0; j < ctas; ++j) {
+        const Shared& o = *cluster.map_shared_rank(&s, j);
+        lo += o.hist[0][rank * share + i];
+        hi += o.hist[1][rank * share + i];
       }
+      lead.sums_of[rank * share + i] = lo + (hi << 16);
     }
     cluster.sync();
     if (rank == 0) {
-      u64 v[2] = {0, 0};
-      for (int i = 0; i < ctas; ++i) {
-        const Shared& o = *cluster.map_shared_rank(&s, i);
+      u64 v[PER_BIN], sum_v = 0, all;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) v[j] += (static_cast<u64>(o.high[2 * tid + j]) << 32) + o.low[2 * tid + j];
-      }
-      u64 all;
-      const u64 before = block_before(v[0] + v[1], s.warp_a, &all, lane, warp) + base;
+      for (int j = 0; j < PER_BIN; ++j) sum_v += v[j] = s.sums_of[PER_BIN * tid + j];
+      u64 before = block_before(sum_v, s.warp_a, &all, lane, warp) + base;
       u64 goal = *target;
-      if (level == 0) {  // the least whole number not below p * all; no more tokens than there are
-        if (mass) goal = __umul64hi(all, p64) + (all * p64 != 0);
-        else if (goal > all) goal = all;
-      }
-      // the first bin whose sum with all before it reaches the goal
-      if (before < goal && goal <= before + v[0] + v[1]) {
-        const int j = goal <= before + v[0] ? 0 : 1;
-        s.bin = 2 * tid + j;
-        s.base = before + (j ? v[0] : 0);
-        s.in_bin = static_cast<uint32_t>(v[j]);
+      if (level == 0) goal = mass ? p_goal(all) : goal < all ? goal : all;
+#pragma unroll
+      for (int j = 0; j < PER_BIN; ++j) {
+        if (before < goal && goal <= before + v[j]) {
+          s.bin = PER_BIN * tid + j;
+          s.base = before;
+          s.in_bin = static_cast<uint32_t>(v[j]);
+        }
+        before += v[j];
       }
       if (tid == 0) s.all = goal;
     }
     cluster.sync();
     *target = lead.all;
   };
-  // tokens of the level's bin `want` (level 0 with `upto`: of all bins to it)
-  // gathered in the first CTA; how many there are
-  auto gather = [&](u64 from, float scale, int level, int bin0, int shift, int known, u64 prefix, int want, bool upto) {
-    for (int i = tid; i < n; i += NT) {
-      const float l = x[i];
-      const int d = digit_of(l, i, from, scale, level, bin0, shift, known, prefix);
-      if (d < 0 || (upto ? d > want : d != want)) continue;
-      const int at = atomicAdd(&lead.gathered[level & 1], 1);
-      if (at < CAP) lead.list[at] = order_of(l, first + i);
-    }
-    cluster.sync();
-    return lead.gathered[level & 1];
+  auto clear = [&](int level) {
+    for (int i = tid; i < 2 * BINS; i += NT) (&s.hist[0][0])[i] = 0;
+    if (tid == 0) s.gathered[level & 1] = 0;
+    __syncthreads();
   };
-  // (first CTA) the list in order
+  auto add = [&](int bin, uint32_t w) {  // at most 2^16 tokens in a CTA: the halves' sums fit
+    if (w & 0xffffu) atomicAdd(&s.hist[0][bin], w & 0xffffu);
+    if (w >> 16) atomicAdd(&s.hist[1][bin], w >> 16);
+  };
+  auto list = [&](int level, float l, int i) {
+    const int at = atomicAdd(&lead.gathered[level & 1], 1);
+    if (at < CAP) lead.list[at] = order_of(l, first + i);
+  };
+  // (first CTA) the list in order, with weights
   auto rank_list = [&](int m) {
     if (tid < m) {
       const u64 mine = s.list[tid];
-      int r = 0;
+      int r = 0, bin;
+#pragma unroll 8
       for (int i = 0; i < m; ++i) r += s.list[i] > mine;
       s.ranked[r] = mine;
+      s.weights[r] = weight(logit_of(mine), &bin);
     }
     __syncthreads();
   };
-  auto narrow = [&](bool mass, u64 target, u64 p64, u64 from, float scale, bool all_listed, bool* listed) -> u64 {
-    u64 base = 0, prefix = 0;
-    int level = 0, bin0 = 0, shift = 54, known = 64;
-    *listed = false;
-    // 7 steps of 10 bits know all 64, and then a bin holds one token at most
-    for (; level < 9; ++level) {
-      histogram(mass, &target, base, p64, from, scale, level, bin0, shift, known, prefix);
-      const int bin = lead.bin;
+  // (first CTA) of the m ranked tokens, the last with less than the goal before it
+  auto cut_of = [&](bool mass, int m, u64 base, u64 goal) {
+    if (mass) {
+      u64 all;
+      const u64 w = tid < m ? s.weights[tid] : 0;
+      const u64 before = base + block_before(w, s.warp_a, &all, lane, warp);
+      if (tid < m && before < goal && (tid == m - 1 || before + w >= goal)) s.cut = s.ranked[tid];
+    } else if (tid == 0) {
+      s.cut = s.ranked[goal - base - 1];
+    }
+    __syncthreads();
+  };
+  // A bin of level 0 with more tokens than are ranked at once, narrowed by the
+  // order's bits: the logits are read again.  in_bin(l, i) says what the bin has.
+  auto narrow = [&](bool mass, u64 base, u64 target, auto in_bin) -> u64 {
+    u64 prefix = 0;
+    int known = 64, shift = 64 - DIGIT;
+    for (int level = 1; level < 9; ++level) {  // 7 steps know all 64 bits, and then a bin has one token at most
+      auto digit_of = [&](float l, int i) {
+        if (!in_bin(l, i)) return -1;
+        const u64 o = order_of(l, first + i);
+        if (known < 64 && (o >> known) != prefix) return -1;
+        return ((1 << DIGIT) - 1) - static_cast<int>((o >> shift) & ((1 << DIGIT) - 1));
+      };
+      clear(level);
+      for (int i = tid; i < n; i += NT) {
+        const float l = plain(src[i]);
+        const int d = digit_of(l, i);
+        int bin;
+        if (d >= 0) add(d, mass ? weight(l, &bin) : 1);
+      }
+      locate(mass, level, base, &target);
+      const int want = lead.bin;
       base = lead.base;
-      // with a few tokens to keep in all, everything down to the cut is listed
-      const bool upto = all_listed && level == 0 && base + lead.in_bin <= CAP;
-      const int m = gather(from, scale, level, bin0, shift, known, prefix, bin, upto);
+      for (int i = tid; i < n; i += NT) {
+        const float l = plain(src[i]);
+        if (digit_of(l, i) == want) list(level, l, i);
+      }
+      cluster.sync();
+      const int m = lead.gathered[level & 1];
       if (m <= CAP) {
         if (rank == 0) {
           rank_list(m);
-          if (upto) base = 0;
-          if (mass) {
-            const u64 w = tid < m ? weight(logit_of(s.ranked[tid])) : 0;
-            u64 all;
-            const u64 before = block_before(w, s.warp_a, &all, lane, warp) + base;
-            // the last token with less than the goal before it
-            if (tid < m && before < target && (tid == m - 1 || before + w >= target)) s.cut = s.ranked[tid];
-          } else if (tid == 0) {
-            s.cut = s.ranked[target - base - 1];
-          }
-          __syncthreads();
+          cut_of(mass, m, base, target);
         }
-        *listed = upto;
-        if (!upto) cluster.sync();  // the cut is there for the others
+        cluster.sync();
         return lead.cut;
       }
-      if (level == 0) {
-        bin0 = bin;
-      } else {  // the digit is known now; the last step's digit repeats bits that are
-        prefix = known < 64 ? (prefix << (known - shift)) | (((BINS - 1) - bin) & ((1 << (known - shift)) - 1))
-                            : static_cast<u64>((BINS - 1) - bin);
-        known = shift;
-        shift = shift >= 10 ? shift - 10 : 0;
-      }
+      // the digit is known now; the last step's digit repeats bits that are
+      const u64 digit = ((1 << DIGIT) - 1) - want;
+      prefix = known < 64 ? (prefix << (known - shift)) | (digit & ((1 << (known - shift)) - 1)) : digit;
+      known = shift;
+      shift = shift >= DIGIT ? shift - DIGIT : 0;
     }
     return 0;
   };
 
+  // ---- top-k
   u64 cut = 0;  // the last token kept, all if 0
-  const float range = top <= FLT_MAX && finite > 0 ? top - sum / static_cast<float>(finite) : 0.f;
   if (k < a.vocab) {
-    bool listed;
-    const float scale = range > 0.f ? static_cast<float>(BINS) / range : 0.f;
-    cut = narrow(false, static_cast<u64>(k), 0, 0, scale, true, &listed);
-    if (listed) {
-      // ---- the first CTA has all of the first k: it ends the row by itself
+    clear(0);
+    uint32_t far = 0;  // the last bin, where most tokens are, is counted in registers
+#pragma unroll 2
+    for (int i = tid; i < n4; i += NT) {
+      const float4 v = reinterpret_cast<const float4*>(x)[i];
+      const float ls[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int b = count_bin(ls[j]);
+        const bool is = ls[j] > -INFINITY;
+        far += is && b == BINS - 1;
+        if (is && b < BINS - 1) atomicAdd(&s.hist[0][b], 1u);
+      }
+    }
+    far = __reduce_add_sync(~0u, far);
+    if (lane == 0 && far) atomicAdd(&s.hist[0][BINS - 1], far);
+    u64 target = k;
+    locate(false, 0, 0, &target);
+    const int want = lead.bin;
+    const u64 base = lead.base;
+    // with a few tokens to keep in all, everything down to the cut is listed
+    const bool upto = base + lead.in_bin <= CAP;
+#pragma unroll 2
+    for (int i = tid; i < n4; i += NT) {
+      const float4 v = reinterpret_cast<const float4*>(x)[i];
+      const float ls[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int b = count_bin(ls[j]);
+        if (ls[j] > -INFINITY && (upto ? b <= want : b == want)) list(0, ls[j], 4 * i + j);
+      }
+    }
+    cluster.sync();
+    const int m = lead.gathered[0];
+    if (upto) {
+      // the first CTA has all of the first k: it ends the row by itself
       if (rank == 0) {
-        const u64 mine = tid < k && tid < CAP ? s.ranked[tid] : 0;
-        const bool some = tid < k && tid < s.gathered[0];
-        const float l = logit_of(mine);
-        u64 w = some ? weight(l) : 0, all;
-        u64 before = block_before(w, s.warp_a, &all, lane, warp);
-        if (by_p) {
-          const u64 p64 = static_cast<u64>(static_cast<double>(p_set) * 18446744073709551616.0);
-          const u64 goal = __umul64hi(all, p64) + (all * p64 != 0);
-          if (before >= goal && tid > 0) w = 0;
-        }
-        if (!enough(l, w)) w = 0;
-        // in index order: the weight of the kept tokens up to each one
-        s.list[tid] = w ? static_cast<u64>(index_of(mine)) : ~0ull;
-        s.ranked[tid] = w;
-        block_before(w, s.warp_a, &all, lane, warp);  // (its barriers: list and ranked are there)
-        if (w) {
-          u64 upto = 0;
-          const int m = k < CAP ? k : CAP;
-          for (int i = 0; i < m; ++i) upto += s.list[i] <= s.list[tid] ? s.ranked[i] : 0;
-          const u64 goal = __umul64hi(all, u64th);
-          if (upto - w <= goal && goal < upto)
-            finish(index_of(mine), static_cast<float>(log(static_cast<double>(w) / static_cast<double>(all))));
+        rank_list(m);
+        const int kept = static_cast<int>(target);
+        u64 all;
+        uint32_t w = tid < kept ? s.weights[tid] : 0;
+        const u64 before = block_before(w, s.warp_a, &all, lane, warp);
+        if (by_p && before >= p_goal(all)) w = 0;
+        if (w && !enough(w, [&] { return logit_of(s.ranked[tid]); })) w = 0;
+        block_before(w, s.warp_a, &all, lane, warp);
+        const int index = tid < kept ? index_of(s.ranked[tid]) : INT_MAX;
+        if (tid < kept) s.weights[tid] = w;
+        __syncthreads();
+        const u64 goal = __umul64hi(all, u64th);
+        if (w) {  // in index order: the token whose interval has the goal
+          u64 lower = 0;
+          for (int i = 0; i < kept; ++i) lower += index_of(s.ranked[i]) < index ? s.weights[i] : 0;
+          if (lower <= goal && goal < lower + w)
+            finish(index, static_cast<float>((static_cast<double>(logit_of(s.ranked[tid])) - weight.dtop) * weight.inv -
+                                             log(static_cast<double>(all) * (1.0 / ONE))));
         }
       }
       cluster.sync();
       return;
     }
-  }
-  if (by_p) {
-    bool listed;
-    // beyond 29.8 / c every weight is 0; half as far behind the mean as before it, few tokens are left
-    float r = 29.8f / weight.c;
-    if (range > 0.f && 1.5f * range < r) r = 1.5f * range;
-    const float scale = r > 0.f && r <= FLT_MAX ? static_cast<float>(BINS) / r : 0.f;
-    const u64 p64 = static_cast<u64>(static_cast<double>(p_set) * 18446744073709551616.0);
-    const u64 c = narrow(true, 0, p64, cut, scale, false, &listed);
-    cut = c > cut ? c : cut;
+    if (m <= CAP) {
+      if (rank == 0) {
+        rank_list(m);
+        cut_of(false, m, base, target);
+      }
+      cluster.sync();
+      cut = lead.cut;
+    } else {
+      cut = narrow(false, base, target, [&](float l, int) { return l > -INFINITY && count_bin(l) == want; });
+    }
   }
 
-  // ---- the draw: warps hold runs of the slice, so sums go in index order
-  const float cut_l = cut ? logit_of(cut) : -INFINITY;
-  const int cut_i = cut ? index_of(cut) : -1;
-  auto kept = [&](int i) -> u64 {
-    const float l = x[i];
-    if (!(l > cut_l || (l == cut_l && first + i <= cut_i))) return 0;
-    const u64 w = weight(l);
-    return enough(l, w) ? w : 0;
+  // ---- the weights, in the logits' place; of top-p, their histogram
+  if (by_p) clear(0);
+#pragma unroll 1
+  for (int i = tid; i < n4; i += NT) {
+    const float4 v = reinterpret_cast<const float4*>(x)[i];
+    const float ls[4] = {v.x, v.y, v.z, v.w};
+    uint32_t w[4];
+    int bin[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = weight(ls[j], &bin[j]);
+    if (cut) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = before_cut(ls[j], 4 * i + j, cut) ? w[j] : 0;
+    }
+    if (by_p) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) add(bin[j], w[j]);
+    }
+    reinterpret_cast<uint4*>(wt)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __syncthreads();
+  // a token's weight and its logit, where that is needed
+  uint32_t cut_w = 1;
+  if (by_p) {
+    u64 target = 0;
+    const u64 k_cut = cut;
+    locate(true, 0, 0, &target);
+    const int want = lead.bin;
+    const u64 base = lead.base;
+    // the bin's weights, a little more on both ends, and then the bin itself
+    const double mid = exp2(31.0 - want * (1.0 / POWERS)), half = 0.0055;  // (2^(1/128) - 1 = 0.00543)
+    const uint32_t low = mid * (1 - half) > 2.0 ? static_cast<uint32_t>(mid * (1 - half)) - 1 : 1;
+    const uint32_t high = mid * (1 + half) + 2 >= 4294967295.0 ? ~0u : static_cast<uint32_t>(mid * (1 + half)) + 2;
+    auto in_bin = [&](float l, int i) {
+      int bin;
+      const uint32_t w = weight(l, &bin);
+      return w && bin == want && before_cut(l, i, k_cut);
+    };
+#pragma unroll 2
+    for (int i = tid; i < n4; i += NT) {
+      const uint4 v = reinterpret_cast<const uint4*>(wt)[i];
+      const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (ws[j] >= low && ws[j] <= high) {
+          const float l = plain(src[4 * i + j]);
+          if (in_bin(l, 4 * i + j)) list(0, l, 4 * i + j);
+        }
+    }
+    cluster.sync();
+    const int m = lead.gathered[0];
+    if (m <= CAP) {
+      if (rank == 0) {
+        rank_list(m);
+        cut_of(true, m, base, target);
+      }
+      cluster.sync();
+      cut = lead.cut;
+    } else {
+      cut = narrow(true, base, target, in_bin);
+    }
+    int bin;
+    cut_w = weight(logit_of(cut), &bin);
+  }
+
+  // ---- the draw: warps hold runs of the slice, so sums go in index order.  A
+  // weight above the cut's is before it, an equal one goes by its logit (the
+  // weights of top-k's dropped tokens are 0)
+  const uint32_t floor_w = cut_w > least ? cut_w : least;
+  const bool exact = (by_p && floor_w == cut_w) || only_top;  // equals of floor_w are looked at
+  auto kept = [&](uint32_t w, int i) -> uint32_t {
+    if (w < floor_w) return 0;
+    if (exact && (w == floor_w || only_top)) {
+      const float l = plain(src[i]);
+      if (only_top ? l != top : false) return 0;
+      if (by_p && !before_cut(l, i, cut)) return 0;
+    }
+    return w;
   };
-  const int chunk = ((n + NW - 1) / NW + 31) & ~31;
+  const int chunk = ((n + NW - 1) / NW + 127) & ~127;
   {
     u64 w = 0;
     const int end = (warp + 1) * chunk < n ? (warp + 1) * chunk : n;
-    for (int i = warp * chunk + lane; i < end; i += 32) w += kept(i);
+#pragma unroll 2
+    for (int i = warp * chunk + 4 * lane; i < end; i += 128) {
+      const uint4 v = *reinterpret_cast<const uint4*>(wt + i);
+      w += static_cast<u64>(kept(v.x, i)) + kept(v.y, i + 1);
+      w += static_cast<u64>(kept(v.z, i + 2)) + kept(v.w, i + 3);
+    }
     w = warp_sum(w);
     if (lane == 0) s.warp_a[warp] = w;
     __syncthreads();
-    if (tid == 0) {
+    if (tid < ctas) {
       u64 all = 0;
+#pragma unroll
       for (int i = 0; i < NW; ++i) all += s.warp_a[i];
-      s.total = all;
+      cluster.map_shared_rank(&s, tid)->totals[rank] = all;
     }
   }
   cluster.sync();
   u64 all = 0, before = 0;
   for (int i = 0; i < ctas; ++i) {
-    const u64 y = cluster.map_shared_rank(&s, i)->total;
-    if (i < rank) before += y;
-    all += y;
+    if (i < rank) before += s.totals[i];
+    all += s.totals[i];
   }
   u64 goal = __umul64hi(all, u64th);
-  if (goal >= before && goal - before < s.total) {
+  if (goal >= before && goal - before < s.totals[rank]) {
     // this CTA's: the warp's run it falls in, split over the warps once more
     goal -= before;
     int w0 = 0;
@@ -482,7 +608,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     const int run0 = w0 * chunk, run1 = run0 + chunk < n ? run0 + chunk : n;
     const int p0 = run0 + warp * part, p1 = p0 + part < run1 ? p0 + part : run1;
     u64 w = 0;
-    for (int i = p0 + lane; i < p1; i += 32) w += kept(i);
+    for (int i = p0 + lane; i < p1; i += 32) w += kept(wt[i], i);
     w = warp_sum(w);
     if (lane == 0) s.warp_b[warp] = w;
     __syncthreads();
@@ -490,16 +616,17 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     for (int i = 0; i < warp; ++i) at += s.warp_b[i];
     if (at <= goal && goal < at + w) {
       for (int i = p0; i < p1; i += 32) {
-        const u64 mine = i + lane < p1 ? kept(i + lane) : 0;
+        const u64 mine = i + lane < p1 ? kept(wt[i + lane], i + lane) : 0;
         const u64 upto = at + warp_scan(mine, lane);
         if (upto - mine <= goal && goal < upto)
-          finish(first + i + lane, static_cast<float>(log(static_cast<double>(mine) / static_cast<double>(all))));
+          finish(first + i + lane,
+                 static_cast<float>((static_cast<double>(plain(src[i + lane])) - weight.dtop) * weight.inv -
+                                    log(static_cast<double>(all) * (1.0 / ONE))));
         at = __shfl_sync(~0u, upto, 31);
         if (goal < at) break;
       }
     }
   }
-  cluster.sync();  // the others may still read this CTA's memory
 }
 
 }  // namespace
@@ -540,6 +667,8 @@ extern "C" int glc_sample(glc_ctx* ctx, const float* logits, int ld, int rows, i
         glc::sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
         static_cast<int>((sizeof(glc::Shared) + 15) / 16 * 16 + sizeof(float) * (glc::SLICE_MAX + 4)));
     if (e != cudaSuccess) return c->fail_cuda(e, "sample: shared memory");
+    const cudaError_t e2 = cudaFuncSetAttribute(glc::sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e2 != cudaSuccess) return c->fail_cuda(e2, "sample: clusters of 16");
     ready = c->device;
   }
   glc::ProfScope prof(c, glc::PROF_OTHER, 4.0 * rows * vocab, c->stream);
