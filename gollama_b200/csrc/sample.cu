@@ -34,14 +34,17 @@ namespace glc {
 namespace {
 
 constexpr int NT = 512, NW = NT / 32;
-constexpr int BINS = 2048, PER_BIN = BINS / NT;
+constexpr int BINS = 2048;
 constexpr int CAP = NT;          // tokens that are ranked at once, one per thread
 constexpr int POWERS = 64;       // bins per factor of two of the weight
 constexpr int DIGIT = 10;        // bits of the order per step of narrowing
 constexpr int MAX_CLUSTER = 8;
 constexpr int SLICE_MAX = 49152; // tokens of a CTA: 192 KB of its shared memory
 constexpr uint32_t ONE = 1u << 31;  // the largest weight
-static_assert((1 << DIGIT) <= BINS && 32 * POWERS <= BINS, "digits and weights have a bin");
+constexpr int GROUPS = BINS / 32;
+static_assert(2 << DIGIT == BINS && 32 * POWERS == BINS, "digits (two sums each) and weights have a bin");
+static_assert(NT == MAX_CLUSTER * GROUPS && CAP == NT, "a thread per CTA and group of bins, and per listed token");
+static_assert(SLICE_MAX < (1 << 16), "sums of 16-bit numbers over a slice have 32 bits");
 
 struct Sample {
   const float* logits;
@@ -77,8 +80,9 @@ struct Weights {
   // round(2^31 exp(-y)), y = (top - l) / temperature = (64 q + j) ln2 / 64 + r with
   // |r| <= ln2 / 128: 2^-q by a shift, 2^(-j/64) from the table, exp(-r) by four
   // terms of its series (r^5 / 120 < 2^-44).  *bin: 64 q + j.  A logit that is
-  // -infinity or not a number has weight 0.
-  __device__ __forceinline__ uint32_t operator()(float l, int* bin) const {
+  // -infinity or not a number has weight 0.  *lead: the first 16 bits of the weight
+  // before its shift.
+  __device__ __forceinline__ uint32_t operator()(float l, int* bin, uint32_t* lead) const {
     const bool some = (top - l) * c < 22.17f;  // else it rounds to 0, and n stays below 32 * 64
     const double y = (dtop - static_cast<double>(l)) * inv;
     const double k = fma(y, POWERS * 1.4426950408889634, 6755399441055744.0);  // 1.5 2^52: the whole number in the low bits
@@ -92,7 +96,13 @@ struct Weights {
     const u64 whole = static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
     const int shift = 11 + n / POWERS;
     *bin = n;
+    *lead = some ? static_cast<uint32_t>(whole >> 27) : 0;
     return some ? static_cast<uint32_t>((whole + (1ull << (shift - 1))) >> shift) : 0;
+  }
+  __device__ __forceinline__ uint32_t operator()(float l) const {
+    int bin;
+    uint32_t lead;
+    return (*this)(l, &bin, &lead);
   }
 };
 
@@ -111,29 +121,27 @@ __device__ __forceinline__ u64 warp_scan(u64 x, int lane) {
 }
 
 struct Shared {
-  union {
-    uint32_t hist[2][BINS];  // sums of the low and high halves of weights
-    struct {                 // (the first CTA) gathered when the histograms have been read
-      u64 list[CAP], ranked[CAP];
-      uint32_t weights[CAP];
-    };
-  };
-  u64 sums_of[BINS];  // (the first CTA) the row's histogram
+  // what the CTAs of the row read of each other
+  uint32_t hist[BINS];
+  u64 coarse[GROUPS];  // its sums over 32 bins
+  u64 list[CAP];       // tokens near a cut
+  int listed[2];       // how many, by the round's parity: a CTA may still read the last round's
+  int first;
+  // what they tell each other, by their rank
+  float tops[MAX_CLUSTER], sums[MAX_CLUSTER];
+  int finites[MAX_CLUSTER];
+  u64 totals[2][MAX_CLUSTER], bases[MAX_CLUSTER];
+  // a CTA's own
+  u64 parts[MAX_CLUSTER][GROUPS];
+  u64 pulled[CAP], ranked[CAP];
+  uint32_t weights[CAP];
   double powers[POWERS];
   u64 warp_a[NW], warp_b[NW];
   float warp_f[NW], warp_top[NW];
   int warp_n[NW];
-  // what the CTAs of the row tell each other, by their rank
-  float tops[MAX_CLUSTER], sums[MAX_CLUSTER];
-  int finites[MAX_CLUSTER];
-  u64 totals[MAX_CLUSTER];
-  // what the other CTAs read from the first
-  int first;
-  int gathered[2];  // by the level's parity: a CTA may still read the last level's
-  int bin;          // of the last histogram: where the cut falls,
-  u64 base, all;    // what lies before that bin, and the goal
-  uint32_t in_bin;  // (of a count) and what is in it
-  u64 cut;          // the last kept token of a filter
+  int bin;           // where a histogram's sum reaches its goal,
+  u64 base, in_bin;  // what lies before it and in it
+  u64 cut;           // the last kept token of a filter
 };
 static_assert(MAX_CLUSTER <= 32, "a lane per CTA of a row");
 
@@ -299,118 +307,154 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     return b < 0 || b >= BINS ? BINS - 1 : b;
   };
 
-  // ---- adds the CTAs' histograms up: where in the row's the sum reaches *target
-  // (with `mass` at level 0 the goal of top-p, of a count at most all there is)
-  auto locate = [&](bool mass, int level, u64 base, u64* target) {
-    cluster.sync();
-    const int share = BINS / ctas;  // of the bins, per CTA
-    for (int i = tid; i < share; i += NT) {
-      u64 lo = 0, hi = 0;
-#pragma unroll 4
-      for (int j = 0; j < ctas; ++j) {
-        const Shared& o = *cluster.map_shared_rank(&s, j);
-        lo += o.hist[0][rank * share + i];
-        hi += o.hist[1][rank * share + i];
-      }
-      lead.sums_of[rank * share + i] = lo + (hi << 16);
+  int round = 0;  // of histogram and list
+  auto clear = [&] {
+    for (int i = tid; i < BINS; i += NT) s.hist[i] = 0;
+    if (tid == 0) s.listed[round & 1] = 0;
+    __syncthreads();
+  };
+  // The row's histogram, found in each CTA by itself: the bin where its sum,
+  // `base` with it, reaches the goal.  value(CTA, bin) is a bin of a CTA's;
+  // goal_of(sum of all) the goal.  First in groups of 32 bins, then in one.
+  auto locate = [&](int bins, u64 base, auto value, auto goal_of) {
+    __syncthreads();
+    for (int i = warp; i < bins / 32; i += NW) {
+      const u64 y = warp_sum(value(s, 32 * i + lane));
+      if (lane == 0) s.coarse[i] = y;
     }
     cluster.sync();
-    if (rank == 0) {
-      u64 v[PER_BIN], sum_v = 0, all;
+    {
+      const int group = tid % GROUPS, peer = tid / GROUPS;
+      s.parts[peer][group] = peer < ctas && group < bins / 32 ? cluster.map_shared_rank(&s, peer)->coarse[group] : 0;
+    }
+    __syncthreads();
+    u64 goal = 0;
+    if (warp == 0) {
+      u64 y[GROUPS / 32], sum_y = 0;
 #pragma unroll
-      for (int j = 0; j < PER_BIN; ++j) sum_v += v[j] = s.sums_of[PER_BIN * tid + j];
-      u64 before = block_before(sum_v, s.warp_a, &all, lane, warp) + base;
-      u64 goal = *target;
-      if (level == 0) goal = mass ? p_goal(all) : goal < all ? goal : all;
+      for (int j = 0; j < GROUPS / 32; ++j) {
+        y[j] = 0;
 #pragma unroll
-      for (int j = 0; j < PER_BIN; ++j) {
-        if (before < goal && goal <= before + v[j]) {
-          s.bin = PER_BIN * tid + j;
+        for (int i = 0; i < MAX_CLUSTER; ++i) y[j] += s.parts[i][GROUPS / 32 * lane + j];
+        sum_y += y[j];
+      }
+      const u64 upto = warp_scan(sum_y, lane);
+      goal = goal_of(__shfl_sync(~0u, upto, 31));
+      u64 before = base + upto - sum_y;
+#pragma unroll
+      for (int j = 0; j < GROUPS / 32; ++j) {
+        if (before < goal && goal <= before + y[j]) {
+          s.bin = GROUPS / 32 * lane + j;
           s.base = before;
-          s.in_bin = static_cast<uint32_t>(v[j]);
         }
-        before += v[j];
+        before += y[j];
       }
-      if (tid == 0) s.all = goal;
     }
-    cluster.sync();
-    *target = lead.all;
-  };
-  auto clear = [&](int level) {
-    for (int i = tid; i < 2 * BINS; i += NT) (&s.hist[0][0])[i] = 0;
-    if (tid == 0) s.gathered[level & 1] = 0;
+    __syncthreads();
+    const int group = s.bin;
+    if (tid < 32 * MAX_CLUSTER) {
+      const int peer = tid / 32;
+      s.parts[peer][lane] = peer < ctas ? value(*cluster.map_shared_rank(&s, peer), 32 * group + lane) : 0;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      u64 y = 0;
+#pragma unroll
+      for (int i = 0; i < MAX_CLUSTER; ++i) y += s.parts[i][lane];
+      const u64 before = s.base + warp_scan(y, lane) - y;
+      __syncwarp();
+      if (before < goal && goal <= before + y) {
+        s.bin = 32 * group + lane;
+        s.base = before;
+        s.in_bin = y;
+      }
+    }
     __syncthreads();
   };
-  auto add = [&](int bin, uint32_t w) {  // at most 2^16 tokens in a CTA: the halves' sums fit
-    if (w & 0xffffu) atomicAdd(&s.hist[0][bin], w & 0xffffu);
-    if (w >> 16) atomicAdd(&s.hist[1][bin], w >> 16);
+  auto list = [&](float l, int i) {
+    const int at = atomicAdd(&s.listed[round & 1], 1);
+    if (at < CAP) s.list[at] = order_of(l, first + i);
   };
-  auto list = [&](int level, float l, int i) {
-    const int at = atomicAdd(&lead.gathered[level & 1], 1);
-    if (at < CAP) lead.list[at] = order_of(l, first + i);
-  };
-  // (first CTA) the list in order, with weights
-  auto rank_list = [&](int m) {
-    if (tid < m) {
-      const u64 mine = s.list[tid];
-      int r = 0, bin;
+  // after the lists' barrier: how many tokens they have; where that can be ranked
+  // and `mine`, all of them in order, with weights
+  auto rank_lists = [&](bool mine) {
+    int m = lane < ctas ? cluster.map_shared_rank(&s, lane)->listed[round & 1] : 0;
+    int upto = m;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += y;
+    }
+    m = __shfl_sync(~0u, upto, 31);
+    if (m <= CAP && mine) {
+      int peer = 0, at = tid;
+#pragma unroll
+      for (int i = 0; i < MAX_CLUSTER; ++i) {
+        const int end = __shfl_sync(~0u, upto, i);
+        if (i < ctas && tid >= end) peer = i + 1, at = tid - end;
+      }
+      const u64 order = tid < m ? cluster.map_shared_rank(&s, peer)->list[at] : 0;
+      s.pulled[tid] = order;
+      __syncthreads();
+      if (tid < m) {
+        int r = 0;
 #pragma unroll 8
-      for (int i = 0; i < m; ++i) r += s.list[i] > mine;
-      s.ranked[r] = mine;
-      s.weights[r] = weight(logit_of(mine), &bin);
+        for (int i = 0; i < m; ++i) r += s.pulled[i] > order;
+        s.ranked[r] = order;
+        s.weights[r] = weight(logit_of(order));
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    return m;
   };
-  // (first CTA) of the m ranked tokens, the last with less than the goal before it
+  // of the m ranked tokens, the last with less than the goal before it
   auto cut_of = [&](bool mass, int m, u64 base, u64 goal) {
     if (mass) {
       u64 all;
       const u64 w = tid < m ? s.weights[tid] : 0;
       const u64 before = base + block_before(w, s.warp_a, &all, lane, warp);
       if (tid < m && before < goal && (tid == m - 1 || before + w >= goal)) s.cut = s.ranked[tid];
-    } else if (tid == 0) {
-      s.cut = s.ranked[goal - base - 1];
+      __syncthreads();
+      return s.cut;
     }
-    __syncthreads();
+    return s.ranked[goal - base - 1];
   };
-  // A bin of level 0 with more tokens than are ranked at once, narrowed by the
-  // order's bits: the logits are read again.  in_bin(l, i) says what the bin has.
-  auto narrow = [&](bool mass, u64 base, u64 target, auto in_bin) -> u64 {
+  // A region of the order with more tokens than are ranked at once, narrowed by
+  // the order's bits: the logits are read again.  in_region(l, i) says what it has.
+  auto narrow = [&](bool mass, u64 base, u64 goal, auto in_region) -> u64 {
     u64 prefix = 0;
     int known = 64, shift = 64 - DIGIT;
-    for (int level = 1; level < 9; ++level) {  // 7 steps know all 64 bits, and then a bin has one token at most
+    constexpr int DIGITS = 1 << DIGIT;
+    for (int step = 0; step < 8; ++step) {  // 7 know all 64 bits, and then a bin has one token at most
       auto digit_of = [&](float l, int i) {
-        if (!in_bin(l, i)) return -1;
+        if (!in_region(l, i)) return -1;
         const u64 o = order_of(l, first + i);
         if (known < 64 && (o >> known) != prefix) return -1;
-        return ((1 << DIGIT) - 1) - static_cast<int>((o >> shift) & ((1 << DIGIT) - 1));
+        return (DIGITS - 1) - static_cast<int>((o >> shift) & (DIGITS - 1));
       };
-      clear(level);
+      ++round;
+      clear();
       for (int i = tid; i < n; i += NT) {
         const float l = plain(src[i]);
         const int d = digit_of(l, i);
-        int bin;
-        if (d >= 0) add(d, mass ? weight(l, &bin) : 1);
+        if (d < 0) continue;
+        const uint32_t w = mass ? wt[i] : 1;
+        atomicAdd(&s.hist[d], w & 0xffffu);
+        if (w >> 16) atomicAdd(&s.hist[DIGITS + d], w >> 16);
       }
-      locate(mass, level, base, &target);
-      const int want = lead.bin;
-      base = lead.base;
+      locate(DIGITS, base, [](const Shared& o, int i) { return o.hist[i] + (static_cast<u64>(o.hist[DIGITS + i]) << 16); },
+             [&](u64) { return goal; });
+      const int want = s.bin;
+      base = s.base;
       for (int i = tid; i < n; i += NT) {
         const float l = plain(src[i]);
-        if (digit_of(l, i) == want) list(level, l, i);
+        if (digit_of(l, i) == want) list(l, i);
       }
       cluster.sync();
-      const int m = lead.gathered[level & 1];
-      if (m <= CAP) {
-        if (rank == 0) {
-          rank_list(m);
-          cut_of(mass, m, base, target);
-        }
-        cluster.sync();
-        return lead.cut;
-      }
+      const int m = rank_lists(true);
+      if (m <= CAP) return cut_of(mass, m, base, goal);
       // the digit is known now; the last step's digit repeats bits that are
-      const u64 digit = ((1 << DIGIT) - 1) - want;
+      const u64 digit = (DIGITS - 1) - want;
       prefix = known < 64 ? (prefix << (known - shift)) | (digit & ((1 << (known - shift)) - 1)) : digit;
       known = shift;
       shift = shift >= DIGIT ? shift - DIGIT : 0;
@@ -421,7 +465,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   // ---- top-k
   u64 cut = 0;  // the last token kept, all if 0
   if (k < a.vocab) {
-    clear(0);
+    clear();
     uint32_t far = 0;  // the last bin, where most tokens are, is counted in registers
 #pragma unroll 2
     for (int i = tid; i < n4; i += NT) {
@@ -432,17 +476,22 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
         const int b = count_bin(ls[j]);
         const bool is = ls[j] > -INFINITY;
         far += is && b == BINS - 1;
-        if (is && b < BINS - 1) atomicAdd(&s.hist[0][b], 1u);
+        if (is && b < BINS - 1) atomicAdd(&s.hist[b], 1u);
       }
     }
     far = __reduce_add_sync(~0u, far);
-    if (lane == 0 && far) atomicAdd(&s.hist[0][BINS - 1], far);
-    u64 target = k;
-    locate(false, 0, 0, &target);
-    const int want = lead.bin;
-    const u64 base = lead.base;
+    if (lane == 0 && far) atomicAdd(&s.hist[BINS - 1], far);
+    u64 goal = k;
+    locate(BINS, 0, [](const Shared& o, int i) { return static_cast<u64>(o.hist[i]); }, [&](u64 all) {
+      goal = goal < all ? goal : all;  // (the first warp's; below it is the others' too)
+      if (lane == 0) s.warp_b[0] = goal;
+      return goal;
+    });
+    goal = s.warp_b[0];
+    const int want = s.bin;
+    const u64 base = s.base;
     // with a few tokens to keep in all, everything down to the cut is listed
-    const bool upto = base + lead.in_bin <= CAP;
+    const bool upto = base + s.in_bin <= CAP;
 #pragma unroll 2
     for (int i = tid; i < n4; i += NT) {
       const float4 v = reinterpret_cast<const float4*>(x)[i];
@@ -450,112 +499,137 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int b = count_bin(ls[j]);
-        if (ls[j] > -INFINITY && (upto ? b <= want : b == want)) list(0, ls[j], 4 * i + j);
+        if (ls[j] > -INFINITY && (upto ? b <= want : b == want)) list(ls[j], 4 * i + j);
       }
     }
     cluster.sync();
-    const int m = lead.gathered[0];
     if (upto) {
-      // the first CTA has all of the first k: it ends the row by itself
-      if (rank == 0) {
-        rank_list(m);
-        const int kept = static_cast<int>(target);
-        u64 all;
-        uint32_t w = tid < kept ? s.weights[tid] : 0;
-        const u64 before = block_before(w, s.warp_a, &all, lane, warp);
-        if (by_p && before >= p_goal(all)) w = 0;
-        if (w && !enough(w, [&] { return logit_of(s.ranked[tid]); })) w = 0;
-        block_before(w, s.warp_a, &all, lane, warp);
-        const int index = tid < kept ? index_of(s.ranked[tid]) : INT_MAX;
-        if (tid < kept) s.weights[tid] = w;
-        __syncthreads();
-        const u64 goal = __umul64hi(all, u64th);
-        if (w) {  // in index order: the token whose interval has the goal
-          u64 lower = 0;
-          for (int i = 0; i < kept; ++i) lower += index_of(s.ranked[i]) < index ? s.weights[i] : 0;
-          if (lower <= goal && goal < lower + w)
-            finish(index, static_cast<float>((static_cast<double>(logit_of(s.ranked[tid])) - weight.dtop) * weight.inv -
-                                             log(static_cast<double>(all) * (1.0 / ONE))));
-        }
+      // the first CTA takes all of the first k and ends the row by itself
+      if (rank == 0) rank_lists(true);
+      cluster.sync();  // (the others' lists are read)
+      if (rank) return;
+      const int kept = static_cast<int>(goal);
+      u64 all;
+      uint32_t w = tid < kept ? s.weights[tid] : 0;
+      const u64 before = block_before(w, s.warp_a, &all, lane, warp);
+      if (by_p && before >= p_goal(all)) w = 0;
+      if (w && !enough(w, [&] { return logit_of(s.ranked[tid]); })) w = 0;
+      block_before(w, s.warp_a, &all, lane, warp);
+      const int index = tid < kept ? index_of(s.ranked[tid]) : INT_MAX;
+      if (tid < kept) s.weights[tid] = w;
+      __syncthreads();
+      const u64 at = __umul64hi(all, u64th);
+      if (w) {  // in index order: the token whose interval has the goal
+        u64 lower = 0;
+        for (int i = 0; i < kept; ++i) lower += index_of(s.ranked[i]) < index ? s.weights[i] : 0;
+        if (lower <= at && at < lower + w)
+          finish(index, static_cast<float>((static_cast<double>(logit_of(s.ranked[tid])) - weight.dtop) * weight.inv -
+                                           log(static_cast<double>(all) * (1.0 / ONE))));
       }
-      cluster.sync();
       return;
     }
-    if (m <= CAP) {
-      if (rank == 0) {
-        rank_list(m);
-        cut_of(false, m, base, target);
-      }
-      cluster.sync();
-      cut = lead.cut;
-    } else {
-      cut = narrow(false, base, target, [&](float l, int) { return l > -INFINITY && count_bin(l) == want; });
-    }
+    const int m = rank_lists(true);
+    cut = m <= CAP ? cut_of(false, m, base, goal)
+                   : narrow(false, base, goal, [&](float l, int) { return l > -INFINITY && count_bin(l) == want; });
+    ++round;
   }
 
-  // ---- the weights, in the logits' place; of top-p, their histogram
-  if (by_p) clear(0);
+  // ---- the weights, in the logits' place; of top-p, their histogram: sums of
+  // their first 16 bits by bin, which is to say nearly where the cut is
+  if (by_p) clear();
+  u64 mine = 0;
 #pragma unroll 1
   for (int i = tid; i < n4; i += NT) {
     const float4 v = reinterpret_cast<const float4*>(x)[i];
     const float ls[4] = {v.x, v.y, v.z, v.w};
-    uint32_t w[4];
+    uint32_t w[4], lead16[4];
     int bin[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = weight(ls[j], &bin[j]);
+    for (int j = 0; j < 4; ++j) w[j] = weight(ls[j], &bin[j], &lead16[j]);
     if (cut) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = before_cut(ls[j], 4 * i + j, cut) ? w[j] : 0;
+      for (int j = 0; j < 4; ++j)
+        if (!before_cut(ls[j], 4 * i + j, cut)) w[j] = lead16[j] = 0;
     }
     if (by_p) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) add(bin[j], w[j]);
+      for (int j = 0; j < 4; ++j)
+        if (lead16[j]) atomicAdd(&s.hist[bin[j]], lead16[j]);
+      mine += static_cast<u64>(w[0]) + w[1];
+      mine += static_cast<u64>(w[2]) + w[3];
     }
     reinterpret_cast<uint4*>(wt)[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  __syncthreads();
-  // a token's weight and its logit, where that is needed
+  // the sum of x over this CTA to all of the row, in totals[which]
+  auto tell = [&](u64 sum_x, u64* (*place)(Shared&)) {
+    sum_x = warp_sum(sum_x);
+    if (lane == 0) s.warp_b[warp] = sum_x;
+    __syncthreads();
+    if (tid < ctas) {
+      u64 all = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) all += s.warp_b[i];
+      place(*cluster.map_shared_rank(&s, tid))[rank] = all;
+    }
+  };
+  auto told = [&](const u64* from) {
+    u64 all = 0;
+    for (int i = 0; i < ctas; ++i) all += from[i];
+    return all;
+  };
   uint32_t cut_w = 1;
   if (by_p) {
-    u64 target = 0;
-    const u64 k_cut = cut;
-    locate(true, 0, 0, &target);
-    const int want = lead.bin;
-    const u64 base = lead.base;
-    // the bin's weights, a little more on both ends, and then the bin itself
-    const double mid = exp2(31.0 - want * (1.0 / POWERS)), half = 0.0055;  // (2^(1/128) - 1 = 0.00543)
-    const uint32_t low = mid * (1 - half) > 2.0 ? static_cast<uint32_t>(mid * (1 - half)) - 1 : 1;
-    const uint32_t high = mid * (1 + half) + 2 >= 4294967295.0 ? ~0u : static_cast<uint32_t>(mid * (1 + half)) + 2;
-    auto in_bin = [&](float l, int i) {
-      int bin;
-      const uint32_t w = weight(l, &bin);
-      return w && bin == want && before_cut(l, i, k_cut);
-    };
+    tell(mine, [](Shared& o) -> u64* { return o.totals[0]; });
+    locate(BINS, 0, [](const Shared& o, int i) { return (static_cast<u64>(o.hist[i]) << 16) >> (i / POWERS); },
+           [&](u64 all) { return p_goal(all); });
+    int bin = s.bin;
+    const u64 goal = p_goal(told(s.totals[0]));
+    for (;;) {
+      // the region of that bin in whole weights: exactly what is before it and in it
+      const uint32_t high = bin == 0 ? ONE : static_cast<uint32_t>(exp2(31.0 - (bin - 0.5) * (1.0 / POWERS)));
+      const uint32_t low = bin == BINS - 1 ? 0 : static_cast<uint32_t>(exp2(31.0 - (bin + 0.5) * (1.0 / POWERS)));
+      u64 more = 0;
 #pragma unroll 2
-    for (int i = tid; i < n4; i += NT) {
-      const uint4 v = reinterpret_cast<const uint4*>(wt)[i];
-      const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
+      for (int i = tid; i < n4; i += NT) {
+        const uint4 v = reinterpret_cast<const uint4*>(wt)[i];
+        const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (ws[j] >= low && ws[j] <= high) {
-          const float l = plain(src[4 * i + j]);
-          if (in_bin(l, 4 * i + j)) list(0, l, 4 * i + j);
+        for (int j = 0; j < 4; ++j) {
+          if (ws[j] > high) more += ws[j];
+          else if (ws[j] > low) list(plain(src[4 * i + j]), 4 * i + j);
         }
-    }
-    cluster.sync();
-    const int m = lead.gathered[0];
-    if (m <= CAP) {
-      if (rank == 0) {
-        rank_list(m);
-        cut_of(true, m, base, target);
       }
+      tell(more, [](Shared& o) -> u64* { return o.bases; });
       cluster.sync();
-      cut = lead.cut;
-    } else {
-      cut = narrow(true, base, target, in_bin);
+      const u64 base = told(s.bases);
+      const int m = rank_lists(true);
+      // what the region has; of more tokens than can be ranked, summed in each CTA
+      u64 inside = 0;
+      if (m <= CAP) {
+        block_before(tid < m ? s.weights[tid] : 0, s.warp_a, &inside, lane, warp);
+      } else {
+        u64 y = 0;
+        for (int i = tid; i < n; i += NT) y += wt[i] > low && wt[i] <= high ? wt[i] : 0;
+        tell(y, [](Shared& o) -> u64* { return o.totals[1]; });
+        cluster.sync();
+        inside = told(s.totals[1]);
+      }
+      const int step = goal <= base ? -1 : goal > base + inside ? 1 : 0;
+      if (step == 0 || bin + step < 0 || bin + step >= BINS) {
+        cut = m <= CAP ? cut_of(true, m, base, goal)
+                       : narrow(true, base, goal, [&](float, int i) { return wt[i] > low && wt[i] <= high; });
+        break;
+      }
+      // the first 16 bits said a neighbour: once more
+      bin += step;
+      ++round;
+      cluster.sync();
+      if (tid == 0) s.listed[round & 1] = 0;
+      __syncthreads();
     }
-    int bin;
-    cut_w = weight(logit_of(cut), &bin);
+    cut_w = weight(logit_of(cut));
+  } else {
+    __syncthreads();
   }
 
   // ---- the draw: warps hold runs of the slice, so sums go in index order.  A
@@ -567,8 +641,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     if (w < floor_w) return 0;
     if (exact && (w == floor_w || only_top)) {
       const float l = plain(src[i]);
-      if (only_top ? l != top : false) return 0;
-      if (by_p && !before_cut(l, i, cut)) return 0;
+      if ((only_top && l != top) || (by_p && !before_cut(l, i, cut))) return 0;
     }
     return w;
   };
@@ -584,22 +657,16 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     }
     w = warp_sum(w);
     if (lane == 0) s.warp_a[warp] = w;
-    __syncthreads();
-    if (tid < ctas) {
-      u64 all = 0;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) all += s.warp_a[i];
-      cluster.map_shared_rank(&s, tid)->totals[rank] = all;
-    }
+    tell(lane == 0 ? w : 0, [](Shared& o) -> u64* { return o.totals[1]; });
   }
   cluster.sync();
   u64 all = 0, before = 0;
   for (int i = 0; i < ctas; ++i) {
-    if (i < rank) before += s.totals[i];
-    all += s.totals[i];
+    if (i < rank) before += s.totals[1][i];
+    all += s.totals[1][i];
   }
   u64 goal = __umul64hi(all, u64th);
-  if (goal >= before && goal - before < s.totals[rank]) {
+  if (goal >= before && goal - before < s.totals[1][rank]) {
     // this CTA's: the warp's run it falls in, split over the warps once more
     goal -= before;
     int w0 = 0;
