@@ -3,16 +3,17 @@
 //
 // A token's weight is exp((l - max) / temperature) as a whole number of 2^-31,
 // so sums of weights are exact and every order of summation gives the same one.
-// It is computed in 64 bits and rounded once: with tens of thousands of tokens
-// kept, sums of float32 exponentials are off by about 2^-25 of themselves, which
-// moves past a token's edge about once in a thousand rows, and that token is
-// then another; rounding errors of 2^-32 of the largest do so once in 10^5.
+// The exponent is reduced in 64 bits and the weight is right to about one unit:
+// with tens of thousands of tokens kept, sums of float32 exponentials are off by
+// about 2^-25 of themselves, which moves past a token's edge about once in a
+// thousand rows, and that token is then another; units of 2^-31 of the largest
+// weight do so about once in 10^5.
 //
 // Tokens are ordered by (logit falling, index rising), a total order; the kept
 // ones of top-k and of top-p are each a prefix of it, so each filter is a cut:
 // its last kept token.  Nothing is sorted but the few tokens around a cut: a
 // histogram finds the bin the cut falls in (of top-k: bins of max - l; of top-p:
-// 64 bins per factor of two of the weight), that bin's tokens (or, for a small
+// 256 bins per factor of two of the weight), that bin's tokens (or, for a small
 // k, all down to it) are gathered and ranked against each other.  A bin of more
 // than 512 tokens is first narrowed by the bits of the order itself, 10 at a
 // time, which ends for any input, equal logits too.  The draw itself is a sum
@@ -34,16 +35,17 @@ namespace glc {
 namespace {
 
 constexpr int NT = 512, NW = NT / 32;
-constexpr int BINS = 2048;
+constexpr int BINS = 8192;
 constexpr int CAP = NT;          // tokens that are ranked at once, one per thread
-constexpr int POWERS = 64;       // bins per factor of two of the weight
+constexpr int POWERS = 256;      // bins, and table entries, per factor of two of the weight
 constexpr int DIGIT = 10;        // bits of the order per step of narrowing
 constexpr int MAX_CLUSTER = 8;
-constexpr int SLICE_MAX = 49152; // tokens of a CTA: 192 KB of its shared memory
+constexpr int SLICE_MAX = 43008; // tokens of a CTA: 168 KB of its shared memory
 constexpr uint32_t ONE = 1u << 31;  // the largest weight
 constexpr int GROUPS = BINS / 32;
-static_assert(2 << DIGIT == BINS && 32 * POWERS == BINS, "digits (two sums each) and weights have a bin");
-static_assert(NT == MAX_CLUSTER * GROUPS && CAP == NT, "a thread per CTA and group of bins, and per listed token");
+static_assert(2 << DIGIT <= BINS && 32 * POWERS == BINS, "digits (two sums each) and weights have a bin");
+static_assert(CAP == NT && GROUPS % 32 == 0, "a thread per listed token, a lane per group of bins");
+static_assert(BINS == 16 * NT && GROUPS <= NT && 32 * MAX_CLUSTER <= NT, "a thread per group, and per bin of a group and CTA");
 static_assert(SLICE_MAX < (1 << 16), "sums of 16-bit numbers over a slice have 32 bits");
 
 struct Sample {
@@ -73,31 +75,36 @@ __device__ __forceinline__ float logit_of(u64 order) {
 }
 __device__ __forceinline__ int index_of(u64 order) { return static_cast<int>(~static_cast<uint32_t>(order)); }
 
+// 2^(31 - j / 256), as the whole number less the bits of ROUND, and as a float.
+struct Power {
+  uint32_t whole;
+  float power;
+};
+constexpr float ROUND = 12582912.f;  // 1.5 2^23: added to a number below 2^22, the nearest whole one in the low bits
+
 struct Weights {
-  float top, c;          // c: 1 / temperature, for what needs no more than 24 bits
-  double dtop, inv;      // 1 / temperature
-  const double* powers;  // 2^(42 - j / 64)
-  // round(2^31 exp(-y)), y = (top - l) / temperature = (64 q + j) ln2 / 64 + r with
-  // |r| <= ln2 / 128: 2^-q by a shift, 2^(-j/64) from the table, exp(-r) by four
-  // terms of its series (r^5 / 120 < 2^-44).  *bin: 64 q + j.  A logit that is
-  // -infinity or not a number has weight 0.  *lead: the first 16 bits of the weight
-  // before its shift.
+  float top, c;         // c: 1 / temperature, for what needs no more than 24 bits
+  double dtop, scale;   // 256 log2(e) / temperature
+  const Power* powers;
+  // (top - l) / temperature = (256 q + j + f) ln2 / 256, |f| <= 1/2, f exact to 2^-40:
+  // 2^-q by a shift, 2^(-j/256) from the table, 1 - exp(-f ln2 / 256) by three terms
+  // of its series (the fourth is below 2^-41), rounded to units before it is taken
+  // off.  *bin: 256 q + j; *lead: the weight's first 16 bits, before the shift.
+  // A logit that is -infinity or not a number has weight 0.
   __device__ __forceinline__ uint32_t operator()(float l, int* bin, uint32_t* lead) const {
-    const bool some = (top - l) * c < 22.17f;  // else it rounds to 0, and n stays below 32 * 64
-    const double y = (dtop - static_cast<double>(l)) * inv;
-    const double k = fma(y, POWERS * 1.4426950408889634, 6755399441055744.0);  // 1.5 2^52: the whole number in the low bits
+    const bool some = (top - l) * c < 22.17f;  // else it rounds to 0 or 1, and bins stay below 8192
+    const double d = dtop - static_cast<double>(l);
+    const double k = fma(d, scale, 6755399441055744.0);  // 1.5 2^52: the whole number in the low bits
+    const float f = static_cast<float>(fma(d, scale, 6755399441055744.0 - k));
     const int n = some ? __double2loint(k) : 32 * POWERS - 1;
-    const double r = fma(k - 6755399441055744.0, -0.6931471805599453 / POWERS, y);
-    double e = fma(r, 1.0 / 24, -1.0 / 6);
-    e = fma(r, e, 0.5);
-    e = fma(r, e, -1.0);
-    e = fma(r, e, 1.0);
-    const double v = fma(powers[n & (POWERS - 1)], e, 4503599627370496.0);  // 2^52: the rounded value in the low bits
-    const u64 whole = static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
-    const int shift = 11 + n / POWERS;
+    constexpr float L = static_cast<float>(0.6931471805599453 / POWERS);
+    const float y = f * fmaf(f, fmaf(f, L * L * L / 6, -L * L / 2), L);
+    const Power p = powers[n & (POWERS - 1)];
+    const uint32_t w = p.whole - __float_as_uint(fmaf(p.power, y, ROUND));
+    const int q = n / POWERS;
     *bin = n;
-    *lead = some ? static_cast<uint32_t>(whole >> 27) : 0;
-    return some ? static_cast<uint32_t>((whole + (1ull << (shift - 1))) >> shift) : 0;
+    *lead = some ? w >> 15 : 0;
+    return some ? (w + ((1u << q) >> 1)) >> q : 0;
   }
   __device__ __forceinline__ uint32_t operator()(float l) const {
     int bin;
@@ -122,8 +129,14 @@ __device__ __forceinline__ u64 warp_scan(u64 x, int lane) {
 
 struct Shared {
   // what the CTAs of the row read of each other
-  uint32_t hist[BINS];
-  u64 coarse[GROUPS];  // its sums over 32 bins
+  union {
+    uint32_t hist[BINS];
+    struct {  // a CTA's own, after the barrier behind which no histogram is read
+      u64 pulled[CAP], ranked[CAP];
+      uint32_t weights[CAP];
+    };
+  };
+  u64 coarse[GROUPS];  // sums of the histogram over 32 bins
   u64 list[CAP];       // tokens near a cut
   int listed[2];       // how many, by the round's parity: a CTA may still read the last round's
   int first;
@@ -132,10 +145,8 @@ struct Shared {
   int finites[MAX_CLUSTER];
   u64 totals[2][MAX_CLUSTER], bases[MAX_CLUSTER];
   // a CTA's own
-  u64 parts[MAX_CLUSTER][GROUPS];
-  u64 pulled[CAP], ranked[CAP];
-  uint32_t weights[CAP];
-  double powers[POWERS];
+  u64 groups[GROUPS], parts[MAX_CLUSTER][32];
+  Power powers[POWERS];
   u64 warp_a[NW], warp_b[NW];
   float warp_f[NW], warp_top[NW];
   int warp_n[NW];
@@ -220,7 +231,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     }
   }
   if (n + tid < 4 * n4) x[n + tid] = __uint_as_float(0x7fc00000u);  // the last 4 tokens are whole
-  if (tid < POWERS) s.powers[tid] = exp2(42.0 - tid * (1.0 / POWERS));
+  if (tid < POWERS) {
+    const double y = exp2(31.0 - tid * (1.0 / POWERS));
+    s.powers[tid] = {static_cast<uint32_t>(y + 0.5) + __float_as_uint(ROUND), static_cast<float>(y)};
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
@@ -280,12 +294,13 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   Weights weight;
   weight.top = top;
   weight.dtop = top;
-  weight.inv = 1.0 / static_cast<double>(temp);
-  weight.c = static_cast<float>(fmin(weight.inv, static_cast<double>(FLT_MAX)));
+  const double inv = 1.0 / static_cast<double>(temp);
+  weight.scale = inv * (POWERS * 1.4426950408889634);
+  weight.c = static_cast<float>(fmin(inv, static_cast<double>(FLT_MAX)));
   weight.powers = s.powers;
   // a token counts from this weight on; min_p >= 1 keeps the largest logit's equals
   const bool only_top = min_set >= 1.f;
-  const uint32_t least = min_set > 0.f ? static_cast<uint32_t>(ceil(fmin(static_cast<double>(min_set), 1.0) * ONE)) : 1u;
+  const uint32_t least = only_top ? ONE : min_set > 0.f ? static_cast<uint32_t>(ceil(static_cast<double>(min_set) * ONE)) : 1u;
   auto enough = [&](uint32_t w, auto logit) { return w >= least && (!only_top || logit() == top); };
   // the random number and p as 64-bit fractions; a goal is the high word of a product
   const u64 u64th = !(u > 0.f) ? 0 : u >= 1.f ? ~0ull : static_cast<u64>(static_cast<double>(u) * 18446744073709551616.0);
@@ -309,7 +324,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
 
   int round = 0;  // of histogram and list
   auto clear = [&] {
-    for (int i = tid; i < BINS; i += NT) s.hist[i] = 0;
+    for (int i = tid; i < BINS / 4; i += NT) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) s.listed[round & 1] = 0;
     __syncthreads();
   };
@@ -318,26 +333,28 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   // goal_of(sum of all) the goal.  First in groups of 32 bins, then in one.
   auto locate = [&](int bins, u64 base, auto value, auto goal_of) {
     __syncthreads();
-    for (int i = warp; i < bins / 32; i += NW) {
-      const u64 y = warp_sum(value(s, 32 * i + lane));
-      if (lane == 0) s.coarse[i] = y;
+    {  // two threads have the bins of a group
+      u64 y = 0;
+      if (tid < bins / 16)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y += value(s, 16 * tid + ((i + tid) & 15));  // (each lane another bank)
+      y += __shfl_xor_sync(~0u, y, 1);
+      if (tid < bins / 16 && !(tid & 1)) s.coarse[tid / 2] = y;
     }
     cluster.sync();
-    {
-      const int group = tid % GROUPS, peer = tid / GROUPS;
-      s.parts[peer][group] = peer < ctas && group < bins / 32 ? cluster.map_shared_rank(&s, peer)->coarse[group] : 0;
+    if (tid < GROUPS) {
+      u64 y = 0;
+      if (tid < bins / 32)
+#pragma unroll
+        for (int i = 0; i < MAX_CLUSTER; ++i) y += i < ctas ? cluster.map_shared_rank(&s, i)->coarse[tid] : 0;
+      s.groups[tid] = y;
     }
     __syncthreads();
     u64 goal = 0;
     if (warp == 0) {
       u64 y[GROUPS / 32], sum_y = 0;
 #pragma unroll
-      for (int j = 0; j < GROUPS / 32; ++j) {
-        y[j] = 0;
-#pragma unroll
-        for (int i = 0; i < MAX_CLUSTER; ++i) y[j] += s.parts[i][GROUPS / 32 * lane + j];
-        sum_y += y[j];
-      }
+      for (int j = 0; j < GROUPS / 32; ++j) sum_y += y[j] = s.groups[GROUPS / 32 * lane + j];
       const u64 upto = warp_scan(sum_y, lane);
       goal = goal_of(__shfl_sync(~0u, upto, 31));
       u64 before = base + upto - sum_y;
@@ -374,6 +391,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   auto list = [&](float l, int i) {
     const int at = atomicAdd(&s.listed[round & 1], 1);
     if (at < CAP) s.list[at] = order_of(l, first + i);
+  };
+  auto list_place = [&](int i) {  // its logit is read later, with the others'
+    const int at = atomicAdd(&s.listed[round & 1], 1);
+    if (at < CAP) s.list[at] = i;
   };
   // after the lists' barrier: how many tokens they have; where that can be ranked
   // and `mine`, all of them in order, with weights
@@ -417,7 +438,9 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
       __syncthreads();
       return s.cut;
     }
-    return s.ranked[goal - base - 1];
+    const u64 last = s.ranked[goal - base - 1];
+    __syncthreads();  // (a histogram may take the list's place)
+    return last;
   };
   // A region of the order with more tokens than are ranked at once, narrowed by
   // the order's bits: the logits are read again.  in_region(l, i) says what it has.
@@ -523,7 +546,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
         u64 lower = 0;
         for (int i = 0; i < kept; ++i) lower += index_of(s.ranked[i]) < index ? s.weights[i] : 0;
         if (lower <= at && at < lower + w)
-          finish(index, static_cast<float>((static_cast<double>(logit_of(s.ranked[tid])) - weight.dtop) * weight.inv -
+          finish(index, static_cast<float>((static_cast<double>(logit_of(s.ranked[tid])) - weight.dtop) * inv -
                                            log(static_cast<double>(all) * (1.0 / ONE))));
       }
       return;
@@ -580,7 +603,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   uint32_t cut_w = 1;
   if (by_p) {
     tell(mine, [](Shared& o) -> u64* { return o.totals[0]; });
-    locate(BINS, 0, [](const Shared& o, int i) { return (static_cast<u64>(o.hist[i]) << 16) >> (i / POWERS); },
+    locate(BINS, 0, [](const Shared& o, int i) { return (static_cast<u64>(o.hist[i]) << 15) >> (i / POWERS); },
            [&](u64 all) { return p_goal(all); });
     int bin = s.bin;
     const u64 goal = p_goal(told(s.totals[0]));
@@ -596,10 +619,14 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (ws[j] > high) more += ws[j];
-          else if (ws[j] > low) list(plain(src[4 * i + j]), 4 * i + j);
+          else if (ws[j] > low) list_place(4 * i + j);
         }
       }
       tell(more, [](Shared& o) -> u64* { return o.bases; });
+      if (tid < s.listed[round & 1]) {  // (tell's barrier: the places are there)
+        const int i = static_cast<int>(s.list[tid]);
+        s.list[tid] = order_of(plain(src[i]), first + i);
+      }
       cluster.sync();
       const u64 base = told(s.bases);
       const int m = rank_lists(true);
@@ -633,13 +660,16 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   }
 
   // ---- the draw: warps hold runs of the slice, so sums go in index order.  A
-  // weight above the cut's is before it, an equal one goes by its logit (the
-  // weights of top-k's dropped tokens are 0)
-  const uint32_t floor_w = cut_w > least ? cut_w : least;
-  const bool exact = (by_p && floor_w == cut_w) || only_top;  // equals of floor_w are looked at
+  // token with more than the cut's weight is before it, near that weight its logit
+  // says (weights are not monotone to the last unit; those of top-k's dropped
+  // tokens are 0)
+  constexpr uint32_t NEAR = 4;
+  const uint32_t near_cut = by_p ? cut_w + NEAR : 0;
+  const uint32_t from_cut = cut_w > NEAR ? cut_w - NEAR : 1;
+  const uint32_t floor_w = from_cut > least ? from_cut : least;
   auto kept = [&](uint32_t w, int i) -> uint32_t {
     if (w < floor_w) return 0;
-    if (exact && (w == floor_w || only_top)) {
+    if (w <= near_cut || only_top) {
       const float l = plain(src[i]);
       if ((only_top && l != top) || (by_p && !before_cut(l, i, cut))) return 0;
     }
@@ -687,7 +717,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
         const u64 upto = at + warp_scan(mine, lane);
         if (upto - mine <= goal && goal < upto)
           finish(first + i + lane,
-                 static_cast<float>((static_cast<double>(plain(src[i + lane])) - weight.dtop) * weight.inv -
+                 static_cast<float>((static_cast<double>(plain(src[i + lane])) - weight.dtop) * inv -
                                     log(static_cast<double>(all) * (1.0 / ONE))));
         at = __shfl_sync(~0u, upto, 31);
         if (goal < at) break;
@@ -709,7 +739,7 @@ extern "C" int glc_sample(glc_ctx* ctx, const float* logits, int ld, int rows, i
   auto no = [&](const char* why) { return c->fail(GLC_ERR_INVALID, std::string("sample: ") + why); };
   if (rows < 0 || vocab <= 0 || ld < vocab) return no("rows must not be negative, vocab positive, ld at least vocab");
   if (vocab > glc::MAX_CLUSTER * glc::SLICE_MAX)
-    return c->fail(GLC_ERR_UNSUPPORTED, "sample: vocab must be at most 393216");
+    return c->fail(GLC_ERR_UNSUPPORTED, "sample: vocab must be at most 344064");
   if (rows == 0) return GLC_OK;
   if (!logits || !temperature || !uniform || !tokens) return no("logits, temperature, uniform and tokens must be given");
   if (((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(temperature) |

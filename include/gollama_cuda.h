@@ -457,8 +457,8 @@ GLC_API int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const glc_
  * counts as -infinity; -infinity is never drawn; where a row has nothing else
  * its token is -1 and its logp -infinity.  logp (nullable): the natural
  * logarithm of the drawn token's share of the kept probability.  Weights are
- * whole numbers of 2^-42 of the largest, so that sums do not depend on their
- * order.  vocab at most 393216. */
+ * whole numbers of 2^-31 of the largest, so that sums do not depend on their
+ * order.  vocab at most 344064. */
 GLC_API int glc_sample(glc_ctx* ctx, const float* logits, int ld, int rows, int vocab, const float* temperature,
                        const int* top_k, const float* top_p, const float* min_p, const float* uniform,
                        int64_t* tokens, float* logp);

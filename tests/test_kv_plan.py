@@ -211,7 +211,7 @@ def test_sample_refuses(call, field, value, code):
 
 
 def test_sample_refuses_a_vocabulary_that_no_cluster_holds(call):
-    refused(call, "glc_sample", {**SAMPLE, "ld": 400000}, "vocab", 393217, UNSUPPORTED)
+    refused(call, "glc_sample", {**SAMPLE, "ld": 400000}, "vocab", 344065, UNSUPPORTED)
 
 
 def test_calls_without_work_return_at_once(call):
