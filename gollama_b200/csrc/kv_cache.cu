@@ -5,150 +5,217 @@
 // moves (num_heads + 2 num_kv_heads) * head_dim floats in, num_heads *
 // head_dim floats and 2 num_kv_heads * head_dim * 9/16 bytes out.
 #include <cfloat>
+#include <climits>
 
 #include "kv_cache.cuh"
 
 namespace glc {
 namespace {
 
+constexpr int ROWS = 256;  // rows that a block looks up at once, a thread each
+constexpr int AHEAD = 4;   // of them, read before the first is used
+constexpr int MOST = 8;    // rows of a block
+
+// Where a row lies.  The lookup is four or five reads deep: done for all of a
+// block's rows at once, the rows' own reads then wait for none of it.
+struct RowAt {
+  int pos;   // -1: no token
+  int page;  // -1: none
+  int slot;
+};
+__device__ __forceinline__ RowAt row_at(const KvPools& c, const KvSeqs& s, int t, int limit, int* err) {
+  RowAt r = {-1, -1, 0};
+  int seq, pos;
+  if (t < s.rows && kv_row(s, c.page, t, err, &seq, &pos)) {
+    if (pos >= limit) {
+      kv_bad(err);
+    } else {
+      const int index = pos / c.page;
+      r.pos = pos;
+      r.slot = pos - index * c.page;
+      r.page = kv_page(s, c.num_pages, seq, index, err);
+    }
+  }
+  return r;
+}
+
 // A thread holds 4 consecutive elements (two rotation pairs) of one head of
 // one row; 8 neighbouring lanes hold the 32 that share a scale, so the largest
-// magnitude is three shuffles and no shared memory is used.  blockIdx.x covers
-// the heads of a row (queries, keys, values, in that order), blockIdx.y
-// strides over the rows.
+// magnitude is three shuffles.  blockIdx.x covers the heads of a row (queries,
+// keys, values, in that order), blockIdx.y the rows, `step` in a row for a block.
 __global__ void __launch_bounds__(256)
     kv_append_kernel(KvPools c, KvSeqs s, const float* __restrict__ q, size_t q_ld, float* __restrict__ q_out,
                      size_t q_out_ld, int heads, const float* __restrict__ k, size_t k_ld,
                      const float* __restrict__ v, size_t v_ld, const float* __restrict__ cos_t,
-                     const float* __restrict__ sin_t, int table_rows, int* __restrict__ err) {
+                     const float* __restrict__ sin_t, int table_rows, int step, int* __restrict__ err) {
   GLC_PDL_ENTRY();
+  __shared__ RowAt at_s[ROWS];
   const int quads = c.head_dim >> 2;
   const int u = blockIdx.x * blockDim.x + threadIdx.x;
-  // a warp whose first unit is past the row has none inside (units come in
-  // whole groups of 8 lanes); the groups past the end stay for the shuffles
-  if ((u & ~31) >= (heads + 2 * c.kv_heads) * quads) return;
   const int head = u / quads, at = u - head * quads;
   const bool is_q = head < heads, is_k = !is_q && head < heads + c.kv_heads;
+  // units come in whole groups of 8 lanes; those past the row stay for the shuffles
   const bool some = head < heads + 2 * c.kv_heads;
   const int h = is_q ? head : is_k ? head - heads : head - heads - c.kv_heads;
   const int half = c.head_dim >> 1;
   const int lane = threadIdx.x & 31;
-  for (int t = blockIdx.y; t < s.rows; t += gridDim.y) {
-    int seq, pos;
-    if (!kv_row(s, c.page, t, err, &seq, &pos)) continue;  // the same for the whole block
-    if (cos_t && pos >= table_rows) {
-      if (threadIdx.x == 0) kv_bad(err);
-      continue;
-    }
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (some) {
-      const float* src = is_q ? q + t * q_ld : is_k ? k + t * k_ld : v + t * v_ld;
-      const float4 y = reinterpret_cast<const float4*>(src + static_cast<size_t>(h) * c.head_dim)[at];
-      x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-      if (cos_t && (is_q || is_k)) {
-        // glc_rope's arithmetic: every product and sum rounded on its own
-        const float2 co = reinterpret_cast<const float2*>(cos_t + static_cast<size_t>(pos) * half)[at];
-        const float2 si = reinterpret_cast<const float2*>(sin_t + static_cast<size_t>(pos) * half)[at];
-        const float a0 = __fsub_rn(__fmul_rn(x[0], co.x), __fmul_rn(x[1], si.x));
-        const float b0 = __fadd_rn(__fmul_rn(x[0], si.x), __fmul_rn(x[1], co.x));
-        const float a1 = __fsub_rn(__fmul_rn(x[2], co.y), __fmul_rn(x[3], si.y));
-        const float b1 = __fadd_rn(__fmul_rn(x[2], si.y), __fmul_rn(x[3], co.y));
-        x[0] = a0, x[1] = b0, x[2] = a1, x[3] = b1;
+  const float* src = (is_q ? q : is_k ? k : v) + static_cast<size_t>(h) * c.head_dim + 4 * at;
+  const size_t ld = is_q ? q_ld : is_k ? k_ld : v_ld;
+  const bool turn = cos_t && (is_q || is_k);
+  const int end = min(s.rows, (static_cast<int>(blockIdx.y) + 1) * step);
+  for (int t0 = blockIdx.y * step; t0 < end; t0 += ROWS) {
+    const int rows = min(ROWS, end - t0);
+    __syncthreads();
+    if (threadIdx.x < rows) at_s[threadIdx.x] = row_at(c, s, t0 + threadIdx.x, cos_t ? table_rows : INT_MAX, err);
+    __syncthreads();
+    for (int r0 = 0; r0 < rows; r0 += AHEAD) {
+      float4 x4[AHEAD];
+      float2 co[AHEAD], si[AHEAD];
+#pragma unroll
+      for (int r = 0; r < AHEAD; ++r) {
+        x4[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        co[r] = si[r] = make_float2(0.f, 0.f);
+        if (r0 + r < rows && some && at_s[r0 + r].pos >= 0) {
+          const int pos = at_s[r0 + r].pos;
+          x4[r] = *reinterpret_cast<const float4*>(src + (t0 + r0 + r) * ld);
+          if (turn) {
+            co[r] = reinterpret_cast<const float2*>(cos_t + static_cast<size_t>(pos) * half)[at];
+            si[r] = reinterpret_cast<const float2*>(sin_t + static_cast<size_t>(pos) * half)[at];
+          }
+        }
       }
-      if (is_q)
-        reinterpret_cast<float4*>(q_out + t * q_out_ld + static_cast<size_t>(h) * c.head_dim)[at] =
-            make_float4(x[0], x[1], x[2], x[3]);
-    }
-    // the element of largest magnitude among the 32, the first of equals, and
-    // whether all are finite; no early exit, so every lane takes the shuffles
-    float m = x[0];
-    bool fine = fabsf(x[0]) <= FLT_MAX;
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
-      if (fabsf(x[i]) > fabsf(m)) m = x[i];
-      fine = fine && fabsf(x[i]) <= FLT_MAX;
-    }
+      for (int r = 0; r < AHEAD; ++r) {
+        if (r0 + r >= rows || at_s[r0 + r].pos < 0) continue;  // the same for the whole block
+        const RowAt place = at_s[r0 + r];
+        float x[4] = {x4[r].x, x4[r].y, x4[r].z, x4[r].w};
+        if (turn) {
+          // glc_rope's arithmetic: every product and sum rounded on its own
+          const float a0 = __fsub_rn(__fmul_rn(x[0], co[r].x), __fmul_rn(x[1], si[r].x));
+          const float b0 = __fadd_rn(__fmul_rn(x[0], si[r].x), __fmul_rn(x[1], co[r].x));
+          const float a1 = __fsub_rn(__fmul_rn(x[2], co[r].y), __fmul_rn(x[3], si[r].y));
+          const float b1 = __fadd_rn(__fmul_rn(x[2], si[r].y), __fmul_rn(x[3], co[r].y));
+          x[0] = a0, x[1] = b0, x[2] = a1, x[3] = b1;
+        }
+        if (is_q)
+          *reinterpret_cast<float4*>(q_out + (t0 + r0 + r) * q_out_ld + static_cast<size_t>(h) * c.head_dim + 4 * at) =
+              make_float4(x[0], x[1], x[2], x[3]);
+        if (__all_sync(~0u, is_q)) continue;
+        // the element of largest magnitude among the 32, the first of equals, and
+        // whether all are finite; no early exit, so every lane takes the shuffles
+        float m = x[0];
+        bool fine = fabsf(x[0]) <= FLT_MAX;
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      const float pm = __shfl_xor_sync(~0u, m, o);
-      if (fabsf(pm) > fabsf(m) || (fabsf(pm) == fabsf(m) && (lane & o))) m = pm;
-    }
-    const unsigned all_fine = __ballot_sync(~0u, fine);
-    if (!some || is_q) continue;
-    const int index = pos / c.page, slot = pos - index * c.page;
-    const int page = kv_page(s, c.num_pages, seq, index, err);
-    if (page < 0) continue;
-    const bool nan = ((all_fine >> (lane & 24)) & 0xffu) != 0xffu;
-    const __half d16 = nan ? __ushort_as_half(0x7e00)
-                           : __float2half_rn(fminf(fmaxf(__fmul_rn(m, -0.125f), -65504.f), 65504.f));
-    const float d = __half2float(d16);
-    unsigned bits = 0x8888u;
-    if (!nan && d != 0.f) {
-      // the whole number nearest to the exact x / d: a first guess by the
-      // reciprocal, then its residual x - n d, which is exact (n d has 15 bits,
-      // and the difference lies on x's grid and below d), against d / 2
-      const float r = __frcp_rn(d), edge = 0.5f * fabsf(d);
-      bits = 0;
+        for (int i = 1; i < 4; ++i) {
+          if (fabsf(x[i]) > fabsf(m)) m = x[i];
+          fine = fine && fabsf(x[i]) <= FLT_MAX;
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float n = rintf(__fmul_rn(x[i], r));
-        n = fminf(fmaxf(n, -16.f), 16.f);
-        const float rest = fmaf(-n, d, x[i]);
-        const float step = (rest < 0.f) == (d < 0.f) ? 1.f : -1.f;
-        if (fabsf(rest) > edge || (fabsf(rest) == edge && (static_cast<int>(n) & 1))) n += step;
-        n = fminf(fmaxf(n, -8.f), 7.f);
-        bits |= static_cast<unsigned>(static_cast<int>(n) + 8) << (4 * i);
+        for (int o = 1; o < 8; o <<= 1) {
+          const float pm = __shfl_xor_sync(~0u, m, o);
+          if (fabsf(pm) > fabsf(m) || (fabsf(pm) == fabsf(m) && (lane & o))) m = pm;
+        }
+        const unsigned all_fine = __ballot_sync(~0u, fine);
+        if (!some || is_q || place.page < 0) continue;
+        const bool nan = ((all_fine >> (lane & 24)) & 0xffu) != 0xffu;
+        const __half d16 = nan ? __ushort_as_half(0x7e00)
+                               : __float2half_rn(fminf(fmaxf(__fmul_rn(m, -0.125f), -65504.f), 65504.f));
+        const float d = __half2float(d16);
+        unsigned bits = 0x8888u;
+        if (!nan && d != 0.f) {
+          // the whole number nearest to the exact x / d: a first guess by the
+          // reciprocal, then its residual x - n d, which is exact (n d has 15 bits,
+          // and the difference lies on x's grid and below d), against d / 2
+          const float rd = __frcp_rn(d), edge = 0.5f * fabsf(d);
+          bits = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float n = rintf(__fmul_rn(x[i], rd));
+            n = fminf(fmaxf(n, -16.f), 16.f);
+            const float rest = fmaf(-n, d, x[i]);
+            const float by = (rest < 0.f) == (d < 0.f) ? 1.f : -1.f;
+            if (fabsf(rest) > edge || (fabsf(rest) == edge && (static_cast<int>(n) & 1))) n += by;
+            n = fminf(fmaxf(n, -8.f), 7.f);
+            bits |= static_cast<unsigned>(static_cast<int>(n) + 8) << (4 * i);
+          }
+        }
+        uint8_t* to = (is_k ? c.k : c.v) + (static_cast<size_t>(place.page) * c.kv_heads + h) * c.chunk;
+        reinterpret_cast<uint16_t*>(to + static_cast<size_t>(place.slot) * half)[at] = static_cast<uint16_t>(bits);
+        if ((lane & 7) == 0)
+          reinterpret_cast<__half*>(to + c.scales_at)[place.slot * (c.head_dim / KV_GROUP) + (at >> 3)] = d16;
       }
     }
-    uint8_t* to = (is_k ? c.k : c.v) + (static_cast<size_t>(page) * c.kv_heads + h) * c.chunk;
-    reinterpret_cast<uint16_t*>(to + static_cast<size_t>(slot) * half)[at] = static_cast<uint16_t>(bits);
-    if ((lane & 7) == 0)
-      reinterpret_cast<__half*>(to + c.scales_at)[slot * (c.head_dim / KV_GROUP) + (at >> 3)] = d16;
   }
 }
 
-// A thread reads 8 codes (4 bytes) and their scale and writes 8 floats.
+// A thread reads 4 codes (2 bytes) and their scale and writes 4 floats; rows as above.
 __global__ void __launch_bounds__(256)
     kv_read_kernel(KvPools c, KvSeqs s, float* __restrict__ k, size_t k_ld, float* __restrict__ v, size_t v_ld,
-                   int* __restrict__ err) {
+                   int step, int* __restrict__ err) {
   GLC_PDL_ENTRY();
-  const int eighths = c.head_dim >> 3;
+  __shared__ RowAt at_s[ROWS];
+  const int quads = c.head_dim >> 2;
   int u = blockIdx.x * blockDim.x + threadIdx.x;
-  const int one = c.kv_heads * eighths;
+  const int one = c.kv_heads * quads;
   // with one of k and v missing, the units are the other's alone
-  if (u >= one * ((k ? 1 : 0) + (v ? 1 : 0))) return;
+  const bool some = u < one * ((k ? 1 : 0) + (v ? 1 : 0));
   const bool is_k = k && u < one;
   if (k && !is_k) u -= one;
-  const int h = u / eighths, at = u - h * eighths;
-  for (int t = blockIdx.y; t < s.rows; t += gridDim.y) {
-    int seq, pos;
-    if (!kv_row(s, c.page, t, err, &seq, &pos)) continue;
-    const int index = pos / c.page, slot = pos - index * c.page;
-    const int page = kv_page(s, c.num_pages, seq, index, err);
-    if (page < 0) continue;
-    const uint8_t* from = (is_k ? c.k : c.v) + (static_cast<size_t>(page) * c.kv_heads + h) * c.chunk;
-    const unsigned w = reinterpret_cast<const unsigned*>(from + static_cast<size_t>(slot) * (c.head_dim >> 1))[at];
-    const float d = __half2float(
-        reinterpret_cast<const __half*>(from + c.scales_at)[slot * (c.head_dim / KV_GROUP) + (at >> 2)]);
-    float x[8];
+  const int h = u / quads, at = u - h * quads;
+  const uint8_t* from = (is_k ? c.k : c.v) + static_cast<size_t>(h) * c.chunk;
+  const size_t page_bytes = c.chunk * c.kv_heads;
+  float* to = (is_k ? k : v) + static_cast<size_t>(h) * c.head_dim + 4 * at;
+  const size_t ld = is_k ? k_ld : v_ld;
+  const int end = min(s.rows, (static_cast<int>(blockIdx.y) + 1) * step);
+  for (int t0 = blockIdx.y * step; t0 < end; t0 += ROWS) {
+    const int rows = min(ROWS, end - t0);
+    __syncthreads();
+    if (threadIdx.x < rows) at_s[threadIdx.x] = row_at(c, s, t0 + threadIdx.x, INT_MAX, err);
+    __syncthreads();
+    if (!some) continue;
+    for (int r0 = 0; r0 < rows; r0 += AHEAD) {
+      uint32_t w[AHEAD];
+      __half d[AHEAD];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(d, static_cast<float>(static_cast<int>((w >> (4 * i)) & 15u) - 8));
-    float4* to = reinterpret_cast<float4*>((is_k ? k + t * k_ld : v + t * v_ld) + static_cast<size_t>(h) * c.head_dim) +
-                 2 * at;
-    to[0] = make_float4(x[0], x[1], x[2], x[3]);
-    to[1] = make_float4(x[4], x[5], x[6], x[7]);
+      for (int r = 0; r < AHEAD; ++r) {
+        w[r] = 0;
+        d[r] = __ushort_as_half(0);
+        if (r0 + r < rows && at_s[r0 + r].page >= 0) {
+          const uint8_t* p = from + static_cast<size_t>(at_s[r0 + r].page) * page_bytes;
+          const int slot = at_s[r0 + r].slot;
+          w[r] = reinterpret_cast<const uint16_t*>(p + static_cast<size_t>(slot) * (c.head_dim >> 1))[at];
+          d[r] = reinterpret_cast<const __half*>(p + c.scales_at)[slot * (c.head_dim / KV_GROUP) + (at >> 3)];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < AHEAD; ++r) {
+        if (r0 + r >= rows || at_s[r0 + r].page < 0) continue;
+        const float f = __half2float(d[r]);
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __fmul_rn(f, static_cast<float>(static_cast<int>((w[r] >> (4 * i)) & 15u) - 8));
+        *reinterpret_cast<float4*>(to + (t0 + r0 + r) * ld) = make_float4(x[0], x[1], x[2], x[3]);
+      }
+    }
   }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// A block per row stripe: as many as fill the device a few times over.
-dim3 row_grid(const Context* ctx, int units, int rows) {
+// Blocks of 256 units by runs of rows: of one row while there are few, of up to
+// `most` where the device is full anyway (a run looks its rows up once; longer
+// ones spread the blocks at work at a time over too much memory).
+struct RowGrid {
+  dim3 grid;
+  int step;
+};
+RowGrid row_grid(const Context* ctx, int units, int rows, int most) {
   const int bx = (units + 255) / 256;
-  int by = (ctx->num_sms * 16 + bx - 1) / bx;
-  if (by > rows) by = rows;
-  if (by > 65535) by = 65535;
-  return dim3(bx, by);
+  const long long blocks = static_cast<long long>(bx) * rows, full = 8LL * ctx->num_sms;
+  int step = 1;
+  while (step < most && blocks > full * step) step *= 2;
+  while ((rows + step - 1) / step > 65535) step *= 2;
+  return {dim3(bx, (rows + step - 1) / step), step};
 }
 
 int cache_check(const char* what, const glc_kv_cache* c, std::string* msg) {
@@ -233,10 +300,11 @@ int glc_kv_append(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* b
   const double moved = static_cast<double>(batch->num_rows) *
                        (8.0 * (q ? q_width : 0) + (8.0 + 9.0 / 8.0) * kv_width);
   glc::ProfScope prof(c, glc::PROF_OTHER, moved, c->stream);
-  glc::launch_pdl(c, glc::kv_append_kernel, glc::row_grid(c, units, batch->num_rows), 256, 0, c->stream,
+  const glc::RowGrid g = glc::row_grid(c, units, batch->num_rows, glc::MOST);
+  glc::launch_pdl(c, glc::kv_append_kernel, g.grid, 256, 0, c->stream,
                   glc::kv_pools(*cache), glc::kv_seqs(*batch), q, static_cast<size_t>(q_ld), q_out,
                   static_cast<size_t>(q_out_ld), heads, k, static_cast<size_t>(k_ld), v, static_cast<size_t>(v_ld),
-                  cos_t, sin_t, table_rows, c->d_err);
+                  cos_t, sin_t, table_rows, g.step, c->d_err);
   GLC_LAUNCH_CHECK(c, "kv_append");
   return GLC_OK;
 }
@@ -257,12 +325,13 @@ int glc_kv_read(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* bat
   if (batch->num_rows == 0 || batch->num_seqs == 0) return GLC_OK;
   glc::DeviceScope on(c);
   const int sides = (k ? 1 : 0) + (v ? 1 : 0);
-  const int units = sides * cache->num_kv_heads * (cache->head_dim / 8);
+  const int units = sides * cache->num_kv_heads * (cache->head_dim / 4);
   glc::ProfScope prof(c, glc::PROF_OTHER, static_cast<double>(batch->num_rows) * sides * width * (4.0 + 9.0 / 16.0),
                       c->stream);
-  glc::launch_pdl(c, glc::kv_read_kernel, glc::row_grid(c, units, batch->num_rows), 256, 0, c->stream,
+  const glc::RowGrid g = glc::row_grid(c, units, batch->num_rows, glc::MOST);
+  glc::launch_pdl(c, glc::kv_read_kernel, g.grid, 256, 0, c->stream,
                   glc::kv_pools(*cache), glc::kv_seqs(*batch), k, static_cast<size_t>(k_ld), v,
-                  static_cast<size_t>(v_ld), c->d_err);
+                  static_cast<size_t>(v_ld), g.step, c->d_err);
   GLC_LAUNCH_CHECK(c, "kv_read");
   return GLC_OK;
 }
