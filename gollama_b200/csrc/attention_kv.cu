@@ -43,6 +43,7 @@ struct AttnKv {
   size_t o_ld;
   float* lse;
   int group;     // query heads per KV head
+  int toks, parts;  // of a tile of query rows: tokens, or tiles of a token
   float scale2;  // log2(e) / sqrt(head_dim)
   float* part;   // [2 * CTAs][RT * (HD + 2)]
   int* count;    // arrivals, by the CTA in which the item starts; zero between calls
@@ -57,8 +58,8 @@ struct Shape {
   static constexpr int NB = Tile::NB;
   static constexpr int RT = 8 * NQ;  // query rows of an item
   static constexpr int STAGES = HD >= 96 ? 2 : 3;
-  // CTAs of an SM: 20 warps of 96 registers, or 12 of 168 with more rows
-  static constexpr int PER_SM = W == 16 ? 1 : (NQ == 1 ? 20 : 12) / W;
+  // CTAs of an SM: 16 warps of 128 registers or 20 of 96, or 12 of 168 with more rows
+  static constexpr int PER_SM = W == 16 ? 1 : (NQ > 1 ? 12 : HD >= 96 ? 16 : 20) / W;
   static constexpr int SCALES = WK * NB * 6;  // a tile's scales as the products take them
   static constexpr int WARP = STAGES * Tile::BYTES + SCALES;
   static constexpr int QUERIES = NQ * NB * 1024;  // the queries as operands
@@ -194,14 +195,8 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
   using Tile = KvTile<HD>;
   constexpr int NB = S::NB, RT = S::RT, STAGES = S::STAGES, UNIT = W * WK;
   extern __shared__ __align__(128) uint8_t smem[];
-  // the share and where in it the CTA is, by thread 0
-  struct Place {
-    long long at, end, item_at, total, ctas;
-    int b, h, tile, units;
-    KvRows w;
-  };
-  __shared__ Place place;
-  __shared__ long long sum_s[W];
+  __shared__ KvPlace place;
+  __shared__ int sum_s[2][W];
   __shared__ int last_s;
   __shared__ __align__(16) float rs_s[RT];  // what a row's products are short of its scores
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -211,49 +206,62 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
   // sequences, a scan over the threads finds the run that the share begins in
   {
     if (tid == 0) place.b = -1;
-    const int run = (a.s.seqs + W * 32 - 1) / (W * 32);
+    const int run = a.s.seqs <= W * 32 ? 1 : (a.s.seqs + W * 32 - 1) / (W * 32);
     const int b0 = tid * run < a.s.seqs ? tid * run : a.s.seqs;
     const int b1 = b0 + run < a.s.seqs ? b0 + run : a.s.seqs;
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b)
-      mine += kv_head_units(kv_rows(a.s, a.c.page, a.group, RT, b, a.err), UNIT) * a.c.kv_heads;
-    long long upto = mine;
+    KvRows w = {};
+    if (b0 < b1) w = kv_rows(a.s, a.c.page, a.toks, a.parts, b0, a.err);
+    // pieces of `per` units of the run, those of all before it, and of all
+    int calls = 0;
+    auto count = [&](int per, int* mine, int* before, int* total) {
+      int y = 0;
+      for (int b = b0; b < b1; ++b)
+        y += kv_head_pieces(run == 1 ? w : kv_rows(a.s, a.c.page, a.toks, a.parts, b, a.err), UNIT, per) * a.c.kv_heads;
+      int upto = y;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(~0u, upto, o);
-      if (lane >= o) upto += v;
-    }
-    if (lane == 31) sum_s[warp] = upto;
-    __syncthreads();
-    long long total = 0, before = 0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += v;
+      }
+      int* sums = sum_s[calls++ & 1];
+      if (lane == 31) sums[warp] = upto;
+      __syncthreads();
+      *mine = y;
+      *before = upto - y;
+      *total = 0;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      if (i < warp) before += sum_s[i];
-      total += sum_s[i];
+      for (int i = 0; i < W; ++i) {
+        if (i < warp) *before += sums[i];
+        *total += sums[i];
+      }
+    };
+    int mine, before, total;
+    count(1, &mine, &before, &total);
+    const int ctas = total < static_cast<int>(gridDim.x) ? total : static_cast<int>(gridDim.x);
+    if (static_cast<int>(blockIdx.x) >= ctas) return;
+    // one piece of one item for each CTA, where pieces come out even enough
+    const int least = (total + ctas - 1) / ctas;
+    int per = 1, alone = 0, begin = kv_cta_begin(blockIdx.x, total, ctas);
+    for (int i = least; i <= kv_most_per(least); i += least < 16 ? 1 : least / 16) {
+      int m, f, pieces;
+      count(i, &m, &f, &pieces);
+      if (pieces <= static_cast<int>(gridDim.x)) {
+        if (static_cast<int>(blockIdx.x) >= pieces) return;
+        per = i, alone = 1, begin = blockIdx.x, mine = m, before = f;
+        break;
+      }
     }
-    upto += before;
-    const long long ctas = total < gridDim.x ? total : gridDim.x;
-    if (blockIdx.x >= ctas) return;
-    const long long begin = total * blockIdx.x / ctas;
-    if (upto - mine <= begin && begin < upto) {
-      long long at = upto - mine;
+    if (before <= begin && begin < before + mine) {
+      place.total = total;
+      place.ctas = ctas;
       for (int b = b0; b < b1; ++b) {
-        const KvRows w = kv_rows(a.s, a.c.page, a.group, RT, b, a.err);
-        const long long per_head = kv_head_units(w, UNIT), u = per_head * a.c.kv_heads;
-        if (begin < at + u) {
-          const int h = static_cast<int>((begin - at) / per_head);
-          place.at = begin;
-          place.end = total * (blockIdx.x + 1) / ctas;
-          place.total = total;
-          place.ctas = ctas;
-          place.b = b;
-          place.h = h;
-          place.tile = kv_find_tile(w, UNIT, begin - at - h * per_head, &place.item_at, &place.units);
-          place.item_at += at + h * per_head;
-          place.w = w;
+        if (run > 1) w = kv_rows(a.s, a.c.page, a.toks, a.parts, b, a.err);
+        const int y = kv_head_pieces(w, UNIT, per) * a.c.kv_heads;
+        if (begin < before + y) {
+          kv_place(&place, w, b, UNIT, per, alone, blockIdx.x, begin - before, before);
           break;
         }
-        at += u;
+        before += y;
       }
     }
     __syncthreads();
@@ -284,11 +292,11 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     const int* table;
     const uint8_t* head;  // piece lane8 of the item's head in page 0 of the lane's side
     {
-      const Place& p = place;
-      const int run_at = p.tile / p.w.parts, part_at = p.tile - run_at * p.w.parts;
-      const long long seg_end = p.item_at + p.units < p.end ? p.item_at + p.units : p.end;
-      key0 = static_cast<int>(p.at - p.item_at) * UNIT;
-      key1 = static_cast<int>(seg_end - p.item_at) * UNIT;
+      const KvPlace& p = place;
+      const int run_at = p.w.parts == 1 ? p.tile : p.tile / p.w.parts, part_at = p.tile - run_at * p.w.parts;
+      const int seg_end = p.item_at + p.units < p.end ? p.item_at + p.units : p.end;
+      key0 = (p.at - p.item_at) * UNIT;
+      key1 = (seg_end - p.item_at) * UNIT;
       const int keys = kv_run_keys(p.w, run_at);
       if (key1 > keys) key1 = keys;
       table = a.s.table + static_cast<size_t>(p.b) * a.s.max_pages;
@@ -303,6 +311,21 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     // the last key that row r sees
     auto row_last = [&](int r) { return edge_key + (r < rows ? r : 0) / width; };
 
+    // the queries' values are on their way while the table's are looked up
+    static_assert(NQ <= W, "a warp per query tile");
+    float x[NB][8];
+    if (warp < NQ) {
+      const int r = 8 * warp + g < rows ? 8 * warp + g : 0, token = tok0 + r / width, hh = head0 + r % width;
+      const float* qp =
+          a.q + static_cast<size_t>(place.w.first + token) * a.q_ld + static_cast<size_t>(place.h * a.group + hh) * HD;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const float4 u = *reinterpret_cast<const float4*>(qp + 32 * i + 8 * t);
+        const float4 v = *reinterpret_cast<const float4*>(qp + 32 * i + 8 * t + 4);
+        x[i][0] = u.x, x[i][1] = u.y, x[i][2] = u.z, x[i][3] = u.w;
+        x[i][4] = v.x, x[i][5] = v.y, x[i][6] = v.z, x[i][7] = v.w;
+      }
+    }
     auto table_page = [&](int index) {
       const int p = table[index];
       if (static_cast<unsigned>(p) < static_cast<unsigned>(a.c.num_pages)) return p;
@@ -337,23 +360,16 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
-    // ---- the queries as operands, a tile of 8 rows per warp in turn: lane (g, t)
-    // has elements 8t .. 8t + 7 of each block of row g, in the order in which the
-    // codes of 8 elements come apart: (0,4), (1,5); (2,6), (3,7)
-    for (int n = warp; n < NQ; n += W) {
-      const int r = 8 * n + g < rows ? 8 * n + g : 0, token = tok0 + r / width, hh = head0 + r % width;
-      const float* qp =
-          a.q + static_cast<size_t>(place.w.first + token) * a.q_ld + static_cast<size_t>(place.h * a.group + hh) * HD;
-      float x[NB][8], top = 0.f;
+    // ---- the queries as operands, a tile of 8 rows per warp: lane (g, t) has
+    // elements 8t .. 8t + 7 of each block of row g, in the order in which the codes
+    // of 8 elements come apart: (0,4), (1,5); (2,6), (3,7)
+    if (warp < NQ) {
+      const int n = warp;
+      float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const float4 u = *reinterpret_cast<const float4*>(qp + 32 * i + 8 * t);
-        const float4 v = *reinterpret_cast<const float4*>(qp + 32 * i + 8 * t + 4);
-        x[i][0] = u.x, x[i][1] = u.y, x[i][2] = u.z, x[i][3] = u.w;
-        x[i][4] = v.x, x[i][5] = v.y, x[i][6] = v.z, x[i][7] = v.w;
+      for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i][j]));
-      }
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
       // the row's largest magnitude goes to [2^13, 2^14)
@@ -626,8 +642,8 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
       }
     }
     __syncthreads();
-    const Place p = place;
-    const long long item_end = p.item_at + p.units;
+    const KvPlace p = place;
+    const int item_end = p.item_at + p.units;
     const bool whole = p.at == p.item_at && item_end <= p.end;
     float* part = a.part + static_cast<size_t>(2 * blockIdx.x + (p.at == p.item_at ? 1 : 0)) * RT * (HD + 2);
     auto write = [&](int r, int c4, float M, float L, float4 o) {
@@ -668,7 +684,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     }
     if (!whole) {
       // ---- the last of the item's CTAs to arrive joins the parts
-      const int first_cta = kv_cta_of(p.item_at, p.total, p.ctas), last_cta = kv_cta_of(item_end - 1, p.total, p.ctas);
+      const int first_cta = kv_first_cta(p), last_cta = kv_last_cta(p);
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -714,10 +730,10 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
       }
     }
     // ---- the next item: the next tile of rows, head, sequence that has any
-    if (item_end >= p.end) return;
+    if (p.alone || item_end >= p.end) return;
     __syncthreads();  // all have read the place, and the shared memory is the rings again
     if (tid == 0) {
-      Place& n = place;
+      KvPlace& n = place;
       n.at = n.item_at = item_end;
       if (++n.tile == n.w.tiles) {
         n.tile = 0;
@@ -728,7 +744,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
               n.b = -1;
               break;
             }
-            n.w = kv_rows(a.s, a.c.page, a.group, RT, n.b, a.err);
+            n.w = kv_rows(a.s, a.c.page, a.toks, a.parts, n.b, a.err);
           } while (n.w.tiles == 0);
         }
       }
@@ -756,6 +772,8 @@ int launch(Context* ctx, const AttnKv& a, cudaStream_t s) {
   if (rc) return rc;
   AttnKv b = a;
   b.part = static_cast<float*>(ws);
+  b.toks = a.group < S::RT ? S::RT / a.group : 1;
+  b.parts = (a.group + S::RT - 1) / S::RT;
   glc::launch_pdl(ctx, attention_kv_kernel<HD, NQ, W>, dim3(ctas), dim3(W * 32), S::SMEM, s, b);
   GLC_LAUNCH_CHECK(ctx, "attention_kv");
   return GLC_OK;
@@ -797,6 +815,10 @@ extern "C" int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const g
   const int group = num_heads / cache->num_kv_heads;
   if (static_cast<long long>(batch->num_rows) * group > 0x40000000) return no("too many query rows");
   if (glc::kv_pools(*cache).chunk * cache->num_kv_heads > 0xffffffffu) return no("a page must stay below 4 GB");
+  // units of the smallest tiles and units, at most: they are counted in 32 bits
+  const double units = (static_cast<double>(batch->num_rows) * ((group + 7) / 8) + batch->num_seqs) * cache->num_kv_heads *
+                       (static_cast<double>(batch->max_pages) * cache->page_size / 128 + 1);
+  if (units > 2147483647.0) return no("num_rows, num_kv_heads and max_pages are too large together");
   if (batch->num_rows == 0 || batch->num_seqs == 0) return GLC_OK;
   glc::DeviceScope on(c);
   glc::AttnKv a;

@@ -127,22 +127,22 @@ KV_HD int kv_page(const KvSeqs& s, int num_pages, int b, int index, int* err) {
 constexpr int KV_WK = 32;  // keys of a warp's tile
 
 // The items of one KV head of a sequence.  A tile of `rt` query rows holds the
-// heads of `toks` whole tokens, or, where a group has more heads than that, up
-// to rt heads of one token (`parts` tiles per token).  Tile i sees the keys of
-// its last token, in units of `unit` keys, one at least (an item without keys
-// still writes its rows).
+// heads of `toks` whole tokens, or, where a group has more heads than that, up to
+// rt heads of one token (`parts` tiles per token).  Tile i sees the keys of its
+// last token, in units of `unit` keys, one at least (an item without keys still
+// writes its rows).
 struct KvRows {
   int first, n, len, toks, parts, tiles;
 };
-KV_HD KvRows kv_rows(const KvSeqs& s, int page, int group, int rt, int b, int* err) {
+KV_HD KvRows kv_rows(const KvSeqs& s, int page, int toks, int parts, int b, int* err) {
   const KvSpan r = kv_span(s, page, b, err);
   KvRows w;
   w.first = r.first;
   w.n = r.n;
   w.len = r.len;
-  w.toks = group < rt ? rt / group : 1;
-  w.parts = (group + rt - 1) / rt;
-  w.tiles = (r.n + w.toks - 1) / w.toks * w.parts;
+  w.toks = toks;
+  w.parts = parts;
+  w.tiles = r.n <= toks ? (r.n ? parts : 0) : (r.n + toks - 1) / toks * parts;
   return w;
 }
 // Keys seen by the last token of the run of tokens `run`.
@@ -160,29 +160,35 @@ KV_HD int kv_run_units(const KvRows& w, int run, int unit) {
 KV_HD int kv_run_equals(const KvRows& w, int run, int units, int unit) {
   const long long room = static_cast<long long>(units) * unit - (w.len - w.n);  // new tokens that fit
   if (room >= w.n) return w.tiles / w.parts;
-  const int end = static_cast<int>(room / w.toks);
+  const int end = static_cast<int>(room) / w.toks;
   return end > run ? end : run + 1;
 }
-KV_HD long long kv_head_units(const KvRows& w, int unit) {
+// The sum over the tiles of a head of their units, in pieces of `per` units
+// (per = 1: the units).
+KV_HD int kv_head_pieces(const KvRows& w, int unit, int per) {
+  if (w.tiles == w.parts) {  // one run of tokens
+    const int u = kv_run_units(w, 0, unit);
+    return (per == 1 ? u : (u + per - 1) / per) * w.parts;
+  }
   const int runs = w.tiles / w.parts;
-  long long sum = 0;
+  int sum = 0;
   for (int i = 0; i < runs;) {
     const int u = kv_run_units(w, i, unit), next = kv_run_equals(w, i, u, unit);
-    sum += static_cast<long long>(u) * (next - i) * w.parts;
+    sum += (per == 1 ? u : (u + per - 1) / per) * (next - i) * w.parts;
     i = next;
   }
   return sum;
 }
-// The tile in which unit `at` of a head lies: its first unit and its units.
-KV_HD int kv_find_tile(const KvRows& w, int unit, long long at, long long* first, int* units) {
+// The tile in which piece `at` of a head lies: its first piece and its units.
+KV_HD int kv_find_tile(const KvRows& w, int unit, int per, int at, int* first, int* units) {
   const int runs = w.tiles / w.parts;
-  long long sum = 0;
+  int sum = 0;
   for (int i = 0; i < runs;) {
     const int u = kv_run_units(w, i, unit), next = kv_run_equals(w, i, u, unit);
-    const long long all = static_cast<long long>(u) * (next - i) * w.parts;
+    const int pieces = (u + per - 1) / per, all = pieces * (next - i) * w.parts;
     if (at < sum + all) {
-      const int skip = static_cast<int>((at - sum) / u);
-      *first = sum + static_cast<long long>(skip) * u;
+      const int skip = (at - sum) / pieces;
+      *first = sum + skip * pieces;
       *units = u;
       return i * w.parts + skip;
     }
@@ -194,10 +200,55 @@ KV_HD int kv_find_tile(const KvRows& w, int unit, long long at, long long* first
   return 0;
 }
 
-// Of `total` units, CTA c of `ctas` (at most total) has [c total / ctas,
-// (c + 1) total / ctas): the CTA that has a unit.
-KV_HD int kv_cta_of(long long unit, long long total, long long ctas) {
-  return static_cast<int>(((unit + 1) * ctas - 1) / total);
+// Of `total` units, CTA c of `ctas` (at most total) has a run of total / ctas, the
+// first total % ctas of them one more: where its run begins, and the CTA of a unit.
+KV_HD int kv_cta_begin(int cta, int total, int ctas) {
+  const int base = total / ctas, more = total - base * ctas;
+  return base * cta + (cta < more ? cta : more);
+}
+KV_HD int kv_cta_of(int unit, int total, int ctas) {
+  const int base = total / ctas, more = total - base * ctas, head = (base + 1) * more;
+  return unit < head ? unit / (base + 1) : more + (unit - head) / base;
+}
+// Items cut into even pieces of at most `per` units, one for each CTA, beat runs
+// of units that pass from item to item, as long as `per` is near the average:
+// how far it may go from the least that could do.
+KV_HD int kv_most_per(int least) { return least + (least < 8 ? 1 : least / 8); }
+
+// Where a CTA is in its share of the work: units [at, end) of all, in the item
+// [item_at, item_at + units).  alone: the share is one piece of one item, which the
+// CTAs first to last share.
+struct KvPlace {
+  int at, end, item_at, units, total, ctas;
+  int alone, first, last;
+  int b, h, tile;
+  KvRows w;
+};
+// The CTAs that share the item.
+KV_HD int kv_first_cta(const KvPlace& p) { return p.alone ? p.first : kv_cta_of(p.item_at, p.total, p.ctas); }
+KV_HD int kv_last_cta(const KvPlace& p) { return p.alone ? p.last : kv_cta_of(p.item_at + p.units - 1, p.total, p.ctas); }
+// The place of the CTA whose share begins at piece `at` of sequence b's (in pieces
+// of `per` units where `alone`, else in units), all before b being `before`.
+KV_HD void kv_place(KvPlace* p, const KvRows& w, int b, int unit, int per, int alone, int cta, int at, int before) {
+  const int per_head = kv_head_pieces(w, unit, per);
+  p->h = at / per_head;
+  p->b = b;
+  p->w = w;
+  p->alone = alone;
+  int first;
+  p->tile = kv_find_tile(w, unit, per, at - p->h * per_head, &first, &p->units);
+  const int piece = at - p->h * per_head - first;  // of the tile
+  if (alone) {
+    p->item_at = 0;
+    p->at = piece * per;
+    p->end = p->at + per < p->units ? p->at + per : p->units;
+    p->first = cta - piece;
+    p->last = p->first + (p->units + per - 1) / per - 1;
+  } else {
+    p->item_at = before + at - piece;
+    p->at = before + at;
+    p->end = kv_cta_begin(cta + 1, p->total, p->ctas);
+  }
 }
 
 // A tile of KV_WK keys in shared memory: codes of the keys, codes of the

@@ -29,43 +29,61 @@ template <int HD>
 int walk(const KvPools& c, const KvSeqs& s, int group, int rt, int warps, int grid, int* err) {
   using Tile = KvTile<HD>;
   const int unit = warps * KV_WK;
-  long long total = 0;
-  for (int b = 0; b < s.seqs; ++b) total += kv_head_units(kv_rows(s, c.page, group, rt, b, err), unit) * c.kv_heads;
-  const long long ctas = std::min<long long>(total, grid);
+  const int toks = group < rt ? rt / group : 1, parts_of = (group + rt - 1) / rt;
+  auto rows_of = [&](int b) { return kv_rows(s, c.page, toks, parts_of, b, err); };
+  auto pieces_of = [&](int per) {
+    int sum = 0;
+    for (int b = 0; b < s.seqs; ++b) sum += kv_head_pieces(rows_of(b), unit, per) * c.kv_heads;
+    return sum;
+  };
+  const int total = pieces_of(1);
+  const int ctas = std::min(total, grid);
   const size_t pool = static_cast<size_t>(c.num_pages) * c.kv_heads * c.chunk;
+  // the shares as the kernel finds them
+  int per = 1, alone = 0, used = ctas;
+  if (ctas > 0) {
+    const int least = (total + ctas - 1) / ctas;
+    for (int i = least; i <= kv_most_per(least); i += least < 16 ? 1 : least / 16)
+      if (pieces_of(i) <= grid) {
+        per = i;
+        alone = 1;
+        used = pieces_of(i);
+        break;
+      }
+  }
   // (sequence, head, tile) -> per key how often it was read; and who wrote it
   std::map<std::vector<int>, std::vector<int>> seen;
   std::map<std::vector<int>, std::vector<std::pair<int, int>>> parts;  // (cta, slot) of an item's parts
   std::map<int, int> arrivals, needed;
   std::set<std::vector<int>> whole;
-  for (int cta = 0; cta < ctas; ++cta) {
-    const long long begin = total * cta / ctas, end = total * (cta + 1) / ctas;
-    if (begin >= end) return 1;
-    for (long long x = begin; x < end; ++x)
-      if (kv_cta_of(x, total, ctas) != cta) return 2;
-    long long at_b = 0, units_b = 0;
-    int b = 0;
+  for (int cta = 0; cta < used; ++cta) {
+    const int begin = alone ? cta : kv_cta_begin(cta, total, ctas);
+    if (!alone) {
+      if (begin >= kv_cta_begin(cta + 1, total, ctas)) return 1;
+      for (int x = begin; x < kv_cta_begin(cta + 1, total, ctas); ++x)
+        if (kv_cta_of(x, total, ctas) != cta) return 2;
+    }
+    KvPlace p = {};
+    p.total = total;
+    p.ctas = ctas;
+    int before = 0, b = 0;
     for (; b < s.seqs; ++b) {
-      units_b = kv_head_units(kv_rows(s, c.page, group, rt, b, err), unit) * c.kv_heads;
-      if (begin < at_b + units_b) break;
-      at_b += units_b;
+      const int y = kv_head_pieces(rows_of(b), unit, per) * c.kv_heads;
+      if (begin < before + y) break;
+      before += y;
     }
     if (b == s.seqs) return 3;
-    KvRows w = kv_rows(s, c.page, group, rt, b, err);
-    const long long per_head = units_b / c.kv_heads;
-    int h = static_cast<int>((begin - at_b) / per_head);
-    long long item_at;
-    int units;
-    int tile = kv_find_tile(w, unit, begin - at_b - h * per_head, &item_at, &units);
-    item_at += at_b + h * per_head;
+    kv_place(&p, rows_of(b), b, unit, per, alone, cta, begin - before, before);
     const int page16 = c.page >> 4, step_pages = (unit / 16) / page16, step_slot = (unit / 16) % page16;
-    for (long long at = begin; at < end;) {
-      const long long item_end = item_at + units, seg_end = std::min(item_end, end);
-      if (at < item_at || at >= item_end) return 4;
+    for (;;) {
+      const KvRows& w = p.w;
+      const int item_end = p.item_at + p.units, seg_end = std::min(item_end, p.end), at = p.at, tile = p.tile, h = p.h;
+      b = p.b;
+      if (at < p.item_at || at >= seg_end) return 4;
       const int run_at = tile / w.parts, part_at = tile - run_at * w.parts;
       const int keys = kv_run_keys(w, run_at);
-      const int key0 = static_cast<int>(at - item_at) * unit;
-      const int key1 = std::min(static_cast<int>(seg_end - item_at) * unit, keys);
+      const int key0 = (at - p.item_at) * unit;
+      const int key1 = std::min((seg_end - p.item_at) * unit, keys);
       const int tok0 = run_at * w.toks, head0 = part_at * rt;
       const int width = group < rt ? group : std::min(group - head0, rt);
       const int rows = std::min(w.n - tok0, w.toks) * width;
@@ -117,30 +135,28 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int rt, int warps, int gr
           for (int i = 0; i < 2; ++i) g[i].advance(step_pages, step_slot, page16);
         }
       }
-      if (at == item_at && seg_end == item_end) {
+      if (at == p.item_at && seg_end == item_end) {
         if (!whole.insert({b, h, tile}).second) return 14;
       } else {
-        const int first = kv_cta_of(item_at, total, ctas), last = kv_cta_of(item_end - 1, total, ctas);
-        parts[{b, h, tile}].push_back({cta, at == item_at ? 1 : 0});
-        if ((cta == first) != (at == item_at) || cta < first || cta > last) return 15;
+        const int first = kv_first_cta(p), last = kv_last_cta(p);
+        parts[{b, h, tile}].push_back({cta, at == p.item_at ? 1 : 0});
+        if ((cta == first) != (at == p.item_at) || cta < first || cta > last) return 15;
         ++arrivals[first];
         needed[first] = last - first + 1;
       }
-      at = seg_end;
-      if (at < end) {
-        item_at = item_end;
-        if (++tile == w.tiles) {
-          tile = 0;
-          if (++h == c.kv_heads) {
-            h = 0;
-            do {
-              if (++b >= s.seqs) return 16;
-              w = kv_rows(s, c.page, group, rt, b, err);
-            } while (w.tiles == 0);
-          }
+      if (p.alone || item_end >= p.end) break;
+      p.at = p.item_at = item_end;
+      if (++p.tile == p.w.tiles) {
+        p.tile = 0;
+        if (++p.h == c.kv_heads) {
+          p.h = 0;
+          do {
+            if (++p.b >= s.seqs) return 16;
+            p.w = rows_of(p.b);
+          } while (p.w.tiles == 0);
         }
-        units = kv_run_units(w, tile / w.parts, unit);
       }
+      p.units = kv_run_units(p.w, p.tile / p.w.parts, unit);
     }
   }
   for (auto& a : arrivals)
@@ -152,7 +168,7 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int rt, int warps, int gr
   }
   // every item once, every key of it that has a page once
   for (int b = 0; b < s.seqs; ++b) {
-    const KvRows w = kv_rows(s, c.page, group, rt, b, err);
+    const KvRows w = rows_of(b);
     int covered = 0;
     for (int h = 0; h < c.kv_heads; ++h)
       for (int tile = 0; tile < w.tiles; ++tile) {
