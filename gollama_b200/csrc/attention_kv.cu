@@ -51,18 +51,19 @@ struct AttnKv {
   uint32_t k1024, less72;  // pairs of halves: 1024, -72
 };
 
-// NQ: query tiles of 8 rows of an item; W: warps.
+// NQ: query tiles of 8 rows of an item, or 0: one tile of 4 rows, whose hi and lo
+// are its 8 columns; W: warps.
 template <int HD, int NQ, int W>
 struct Shape {
   using Tile = KvTile<HD>;
   static constexpr int NB = Tile::NB;
-  static constexpr int RT = 8 * NQ;  // query rows of an item
+  static constexpr int RT = NQ ? 8 * NQ : 4;  // query rows of an item
   static constexpr int STAGES = HD >= 96 ? 2 : 3;
   // CTAs of an SM: 16 warps of 128 registers or 20 of 96, or 12 of 168 with more rows
   static constexpr int PER_SM = W == 16 ? 1 : (NQ > 1 ? 12 : HD >= 96 ? 16 : 20) / W;
   static constexpr int SCALES = WK * NB * 6;  // a tile's scales as the products take them
   static constexpr int WARP = STAGES * Tile::BYTES + SCALES;
-  static constexpr int QUERIES = NQ * NB * 1024;  // the queries as operands
+  static constexpr int QUERIES = NQ ? NQ * NB * 1024 : NB * 512;  // the queries as operands
   static constexpr int JOIN = W * RT * (HD + 2) * 4;  // the warps' (o, m, l), in the place of all this
   static constexpr int SMEM = QUERIES + W * WARP > JOIN ? QUERIES + W * WARP : JOIN;
   static_assert(WARP % 16 == 0, "rings start on 16 bytes");
@@ -194,6 +195,8 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
   using S = Shape<HD, NQ, W>;
   using Tile = KvTile<HD>;
   constexpr int NB = S::NB, RT = S::RT, STAGES = S::STAGES, UNIT = W * WK;
+  constexpr bool PAIRED = NQ == 0;        // columns 2r and 2r + 1 are hi and lo of row r
+  constexpr int TILES = NQ ? NQ : 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ KvPlace place;
   __shared__ int sum_s[2][W];
@@ -268,7 +271,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     if (place.b < 0) return;  // not reached, were the lengths left alone meanwhile
   }
 
-  uint4* queries = reinterpret_cast<uint4*>(smem);  // [query tile][block][half of it][lane]: hi, hi, lo, lo
+  uint4* queries = reinterpret_cast<uint4*>(smem);  // [query tile][block][half of it][lane]: hi, hi, lo, lo; paired: [block][lane]: the halves' column
   uint8_t* ring = smem + S::QUERIES + warp * S::WARP;
   float* kscale = reinterpret_cast<float*>(ring + STAGES * Tile::BYTES);                   // [block][key % 8][key / 8]
   __half* vscale = reinterpret_cast<__half*>(ring + STAGES * Tile::BYTES + WK * NB * 4);  // [block][pair % 4][key / 8][2]
@@ -312,10 +315,10 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     auto row_last = [&](int r) { return edge_key + (r < rows ? r : 0) / width; };
 
     // the queries' values are on their way while the table's are looked up
-    static_assert(NQ <= W, "a warp per query tile");
+    static_assert(TILES <= W, "a warp per query tile");
     float x[NB][8];
-    if (warp < NQ) {
-      const int r = 8 * warp + g < rows ? 8 * warp + g : 0, token = tok0 + r / width, hh = head0 + r % width;
+    if (warp < TILES) {
+      const int mine = PAIRED ? g >> 1 : 8 * warp + g, r = mine < rows ? mine : 0, token = tok0 + r / width, hh = head0 + r % width;
       const float* qp =
           a.q + static_cast<size_t>(place.w.first + token) * a.q_ld + static_cast<size_t>(place.h * a.group + hh) * HD;
 #pragma unroll
@@ -363,7 +366,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     // ---- the queries as operands, a tile of 8 rows per warp: lane (g, t) has
     // elements 8t .. 8t + 7 of each block of row g, in the order in which the codes
     // of 8 elements come apart: (0,4), (1,5); (2,6), (3,7)
-    if (warp < NQ) {
+    if (warp < TILES) {
       const int n = warp;
       float top = 0.f;
 #pragma unroll
@@ -376,28 +379,30 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
       int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
       e = e < -100 ? -100 : e > 126 ? 126 : e;
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
-      if (t == 0) rs_s[8 * n + g] = a.scale2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * 0.0001220703125f;  // 2^(e - 13)
+      if (t == 0) rs_s[PAIRED ? g >> 1 : 8 * n + g] = a.scale2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * 0.0001220703125f;  // 2^(e - 13)
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[i][j] *= up;
+        uint4 q[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          uint4 q;
-          split2(x[i][2 * j], x[i][2 * j + 4], &q.x, &q.z);
-          split2(x[i][2 * j + 1], x[i][2 * j + 5], &q.y, &q.w);
-          queries[((n * NB + i) * 2 + j) * 32 + lane] = q;
+          split2(x[i][2 * j], x[i][2 * j + 4], &q[j].x, &q[j].z);
+          split2(x[i][2 * j + 1], x[i][2 * j + 5], &q[j].y, &q[j].w);
+          if (!PAIRED) queries[((n * NB + i) * 2 + j) * 32 + lane] = q[j];
         }
+        if (PAIRED)
+          queries[i * 32 + lane] = g & 1 ? make_uint4(q[0].z, q[0].w, q[1].z, q[1].w) : make_uint4(q[0].x, q[0].y, q[1].x, q[1].y);
       }
     }
     __syncthreads();
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 
     // rows: elements 4g + e of a block, columns: queries; [..][j][0..1] is e = 2j, [2..3] e = 2j + 1
-    float acc[NQ][NB][2][4];
-    float m[NQ][2], l[NQ][2];  // of queries 8n + 2t and 8n + 2t + 1
+    float acc[TILES][NB][2][4];
+    float m[TILES][2], l[TILES][2];  // of queries 8n + 2t and 8n + 2t + 1; paired: [0][0], of query t
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
+    for (int n = 0; n < TILES; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
@@ -450,7 +455,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
           const int now = 4 - e;
           const float by = vtop ? __uint_as_float(static_cast<uint32_t>(127 + now - vexp) << 23) : 0.f;
 #pragma unroll
-          for (int n = 0; n < NQ; ++n)
+          for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -474,8 +479,9 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
       }
       __syncwarp();
 
-      // ---- s of keys 16 j + g (x = 0, 1: queries 2t, 2t + 1) and 16 j + 8 + g (x = 2, 3)
-      float s[NQ][2][4];
+      // ---- s of keys 16 j + g (x = 0, 1: queries 2t, 2t + 1) and 16 j + 8 + g (x = 2, 3);
+      // paired: x = 0 and 1, of query t
+      float s[TILES][2][4];
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         uint32_t kw[4];  // codes of elements 8t .. 8t + 7 of the block, keys 8x + g
@@ -487,6 +493,21 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
           const uint32_t x = kw[2 * j], y = kw[2 * j + 1], xs = x >> 8, ys = y >> 8;
           ka[j][0] = unpack.low(x), ka[j][1] = unpack.low(y), ka[j][2] = unpack.next(x), ka[j][3] = unpack.next(y);
           ka[j][4] = unpack.low(xs), ka[j][5] = unpack.low(ys), ka[j][6] = unpack.next(xs), ka[j][7] = unpack.next(ys);
+        }
+        if constexpr (PAIRED) {
+          const uint4 q = queries[i * 32 + lane];
+          float c[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mma16816(c[j], ka[j][0], ka[j][1], ka[j][2], ka[j][3], q.x, q.y, zero);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mma16816(c[j], ka[j][4], ka[j][5], ka[j][6], ka[j][7], q.z, q.w, c[j]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const float dd = j ? (z ? d.w : d.z) : (z ? d.y : d.x), y = c[j][2 * z] + c[j][2 * z + 1];
+              s[0][j][z] = i ? fmaf(dd, y, s[0][j][z]) : dd * y;
+            }
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -512,8 +533,51 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 
       // ---- the running softmax of queries 8n + 2t and 8n + 2t + 1
       const bool edge = key + WK > key1 || key + WK - 1 > edge_key;
-      // probabilities as halves, turned so that lane (g, t) has query 8n + g and keys 2t, 2t + 1 of each 8
-      uint32_t hi[NQ][4], lo[NQ][4];
+      // probabilities as halves, turned so that lane (g, t) has column g and keys 2t, 2t + 1 of each 8
+      uint32_t hi[TILES][4], lo[TILES][4];
+      uint32_t own[4];  // paired: what the lane's column is, hi or lo; hi is 0 where it is hi
+      if constexpr (PAIRED) {
+        const float rs = rs_s[t];
+        if (edge) {
+          const int last = row_last(t);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const int k = key + 16 * j + 8 * z + g;
+              if (k > last || k >= key1) s[0][j][z] = -INFINITY;
+            }
+        }
+        float top = fmaxf(fmaxf(s[0][0][0], s[0][0][1]), fmaxf(s[0][1][0], s[0][1][1]));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 16)) * rs;
+        if (__any_sync(~0u, top > m[0][0] + SLACK)) {
+          const float now = fmaxf(m[0][0], top), by = now == -INFINITY ? 0.f : exp2_fast(m[0][0] - now);
+          m[0][0] = now;
+          l[0][0] *= by;
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) acc[0][i][j][x] *= by;
+        }
+        const float ms = m[0][0] == -INFINITY ? 0.f : m[0][0] - PEXP;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float p = exp2_fast(fmaf(s[0][j][i], rs, -ms));
+            l[0][0] += p;
+            uint32_t ph, pl;
+            split2(p, p, &ph, &pl);
+            ph = transposed(ph);
+            pl = transposed(pl);
+            own[2 * j + i] = g & 1 ? pl : ph;
+            hi[0][2 * j + i] = g & 1 ? ph : 0u;
+          }
+      }
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         const float2 rs = *reinterpret_cast<const float2*>(rs_s + 8 * n + 2 * t);
@@ -582,6 +646,25 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
           va[j][0] = unpack.low(u), va[j][1] = unpack.next(u), va[j][2] = unpack.low(v), va[j][3] = unpack.next(v);
           va[j][4] = unpack.low(us), va[j][5] = unpack.next(us), va[j][6] = unpack.low(vs), va[j][7] = unpack.next(vs);
         }
+        if constexpr (PAIRED) {
+          uint32_t p[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) p[x] = fma2(own[x], dw[x], fma2(hi[0][x], dw[x], neg2(mul2(hi[0][x], dw[x]))));
+          if (fix) {  // a key that a row does not see counts nothing, whatever its scale is
+            const int last = row_last(g >> 1);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int k = key + 8 * x + 2 * t;
+              p[x] &= (k <= last ? 0x0000ffffu : 0u) | (k + 1 <= last ? 0xffff0000u : 0u);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              mma16816(acc[0][i][e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], p[2 * j],
+                       p[2 * j + 1], acc[0][i][e]);
+        }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           uint32_t ph[4], pl[4];
@@ -622,6 +705,20 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     __syncthreads();  // the rings are free
     float* jo = reinterpret_cast<float*>(smem) + warp * RT * HD;
     float* jm = reinterpret_cast<float*>(smem) + W * RT * HD;  // [W][RT] m, then l
+    if constexpr (PAIRED) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const float(*y)[4] = acc[0][i];
+        *reinterpret_cast<float4*>(jo + t * HD + 32 * i + 4 * g) = make_float4(
+            (y[0][0] + y[0][1]) * down, (y[0][2] + y[0][3]) * down, (y[1][0] + y[1][1]) * down, (y[1][2] + y[1][3]) * down);
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[0][0] += __shfl_xor_sync(~0u, l[0][0], o);
+      if (g == 0) {
+        jm[warp * RT + t] = m[0][0];
+        jm[W * RT + warp * RT + t] = l[0][0] * (1.f / (1 << PEXP));
+      }
+    }
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
 #pragma unroll
@@ -790,7 +887,9 @@ int launch_for(Context* ctx, const AttnKv& a, cudaStream_t s) {
   // join; of many items a CTA has several, and small CTAs overlap one's joins
   // with another's copies.
   const long long items = static_cast<long long>(a.s.rows) * ((a.group + 7) / 8) * a.c.kv_heads;
-  return items >= ctx->num_sms / 2 ? launch<HD, 1, 4>(ctx, a, s) : launch<HD, 1, 16>(ctx, a, s);
+  const bool many = items >= ctx->num_sms / 2;
+  if (rows <= 4) return many ? launch<HD, 0, 4>(ctx, a, s) : launch<HD, 0, 16>(ctx, a, s);
+  return many ? launch<HD, 1, 4>(ctx, a, s) : launch<HD, 1, 16>(ctx, a, s);
 }
 
 }  // namespace
