@@ -60,7 +60,7 @@ struct Shape {
   static constexpr int RT = NQ ? 8 * NQ : 4;  // query rows of an item
   static constexpr int STAGES = HD >= 96 ? 2 : 3;
   // CTAs of an SM: 16 warps of 128 registers or 20 of 96, or 12 of 168 with more rows
-  static constexpr int PER_SM = W == 16 ? 1 : (NQ > 1 ? 12 : HD >= 96 ? 16 : 20) / W;
+  static constexpr int PER_SM = W == 16 ? 1 : (NQ > 2 && HD >= 96 ? 8 : NQ > 1 ? 12 : HD >= 96 ? 16 : 20) / W;
   static constexpr int SCALES = WK * NB * 6;  // a tile's scales as the products take them
   static constexpr int WARP = STAGES * Tile::BYTES + SCALES;
   static constexpr int QUERIES = NQ ? NQ * NB * 1024 : NB * 512;  // the queries as operands
@@ -882,6 +882,9 @@ int launch_for(Context* ctx, const AttnKv& a, cudaStream_t s) {
   // an item as they fill, since an item unpacks its keys and values once.
   const long long rows = static_cast<long long>(a.s.rows) * a.group / a.s.seqs;
   if (HD <= 64 && rows > 24) return launch<HD, HD <= 64 ? 4 : 2, 4>(ctx, a, s);
+  if constexpr (HD >= 96) {
+    if (rows > 16 && rows <= 24) return launch<HD, 3, 4>(ctx, a, s);
+  }
   if (rows > 8) return launch<HD, 2, 4>(ctx, a, s);
   // Few items are cut between many CTAs, and few large CTAs leave fewer parts to
   // join; of many items a CTA has several, and small CTAs overlap one's joins
