@@ -101,6 +101,16 @@ __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uin
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
+// (x0, x1) += (y0, y1), each rounded to nearest
+__device__ __forceinline__ void add_pair(float* x, const float* y) {
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%0, %1};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x[0]), "+f"(x[1])
+      : "f"(y[0]), "f"(y[1]));
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -632,7 +642,9 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
       }
       const bool fix = odd_scale && edge;
 
-      // ---- o
+      // ---- o: a tile's sum from zero, then added.  (The products cut their sums
+      // off, each by up to 2^-24 of what is there: a long row summed in them alone
+      // came out 2e-6 too small after 4096 keys.)
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         uint32_t vw[4];  // codes of elements 4g .. 4g + 3, keys 8x + 2t and 8x + 2t + 1
@@ -658,12 +670,15 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
               p[x] &= (k <= last ? 0x0000ffffu : 0u) | (k + 1 <= last ? 0xffff0000u : 0u);
             }
           }
+          float y[2][4];
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              mma16816(acc[0][i][e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], p[2 * j],
-                       p[2 * j + 1], acc[0][i][e]);
+              mma16816(y[e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], p[2 * j], p[2 * j + 1],
+                       j ? y[e] : zero);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) add_pair(acc[0][i][e], y[e]), add_pair(acc[0][i][e] + 2, y[e] + 2);
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -683,17 +698,19 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
               pl[x] &= keep;
             }
           }
+          float y[2][4];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              mma16816(acc[n][i][e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], ph[2 * j],
-                       ph[2 * j + 1], acc[n][i][e]);
+              mma16816(y[e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], ph[2 * j], ph[2 * j + 1],
+                       j ? y[e] : zero);
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              mma16816(acc[n][i][e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], pl[2 * j],
-                       pl[2 * j + 1], acc[n][i][e]);
+              mma16816(y[e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], pl[2 * j], pl[2 * j + 1], y[e]);
           }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) add_pair(acc[n][i][e], y[e]), add_pair(acc[n][i][e] + 2, y[e] + 2);
         }
       }
       stage = stage == STAGES - 1 ? 0 : stage + 1;
