@@ -749,11 +749,10 @@ extern "C" int glc_sample(glc_ctx* ctx, const float* logits, int ld, int rows, i
     return no("a pointer is not aligned to its elements");
   if (rows > 0x7fffffff / glc::MAX_CLUSTER) return no("too many rows");
   glc::DeviceScope on(c);
-  // CTAs of a row: until the device is full, and as its slice needs
+  // CTAs of a row: as its slices need, and more while all of them run at once
   int ctas = 1;
-  while (ctas < glc::MAX_CLUSTER &&
-         (static_cast<long long>(rows) * ctas < 2 * c->num_sms || (vocab + ctas - 1) / ctas > 16400) &&
-         vocab / ctas > 1024)
+  while (ctas < glc::MAX_CLUSTER && vocab / ctas > 1024 &&
+         ((vocab + ctas - 1) / ctas > 16400 || static_cast<long long>(rows) * ctas <= c->num_sms))
     ctas *= 2;
   glc::Sample a{logits, static_cast<size_t>(ld), vocab, ((vocab + ctas - 1) / ctas + 3) & ~3, temperature, top_k,
                 top_p, min_p, uniform, tokens, logp};

@@ -256,11 +256,13 @@ def attend(ctx, cache, batch, q, heads, pad=0, lse=True):
 
 def check(cache, batch, q, heads, o, lse):
     """Per element, with s the sum of |q_i k_i| / sqrt(hd) of the largest key:
-    a score is off by at most s (2^-22 from q's two halves + 2^-24 for each of the
-    ~20 roundings of its sums), ~2^-19.4 s; an exponential of it by that times
-    itself and 2^-22 more; the probabilities' halves add 2^-22, the sums over up to
-    2^7 tiles of a warp and the joins 2^7 2^-24 at most; numerator and denominator
-    both.  Hence 2 (2^-19.4 s + 2^-16.5), relative to the largest value (8 scales)."""
+    a score is off by at most s (2^-22 from q's two halves, 2^-24 for each of the ~20
+    roundings and cut-off sums of its products), ~2^-19.4 s; an exponential by that
+    times itself and 2^-22 more; the probabilities' halves and their products with
+    the scales add 2^-21, a tile's 8 cut-off sums 2^-21, and the at most 2^9 additions
+    of tiles and parts, to nearest, 2^-24 each, of either sign, 2^-19.5; numerator and
+    denominator both.  Hence 2 (2^-19.4 s + 2^-18.5), relative to the largest value
+    (8 scales)."""
     p = cache.pools
     want, want_lse, s = ref.attend(p, batch.table, batch.lens, batch.starts, q, heads)
     none = np.isnan(want_lse).any(1)
@@ -269,7 +271,7 @@ def check(cache, batch, q, heads, o, lse):
     o = o[:, : heads * hd]
     assert (o[none] == CANARY).all() and (lse[none] == CANARY).all()
     o, want, lse, want_lse, s = o[~none], want[~none], lse[~none], want_lse[~none], s[~none]
-    tol = 2 * (2**-19.4 * s + 2**-16.5)
+    tol = 2 * (2**-19.4 * s + 2**-18.5)
     big = float(np.abs(p.scales[1].astype(np.float64))[np.isfinite(p.scales[1])].max() * 8)
     err = np.abs(o - want).reshape(len(o), heads, hd).max(-1)
     assert (err <= tol * big).all(), (err / (tol * big)).max()
@@ -347,14 +349,17 @@ def test_value_scales_that_grow_along_the_sequence(ctx):
     check(cache, batch, q, 4, *attend(ctx, cache, batch, q, 4))
 
 
-def test_what_a_row_does_not_see_does_not_count(ctx):
+@pytest.mark.parametrize("kv_heads,group,hd", [(2, 2, 64), (1, 1, 32), (2, 8, 128), (1, 20, 64), (1, 1, 96)])
+@pytest.mark.parametrize("news", [[9, 1], [3, 2]])
+def test_what_a_row_does_not_see_does_not_count(ctx, kv_heads, group, hd, news):
     """NaN and infinite scales behind the end of a sequence, in unused pages, and
     in tokens that only later rows see; a visible NaN reaches the rows that see it."""
     r = np.random.default_rng(12)
-    cache, batch = make(ctx, r, [40, 21], [9, 1], 2, 64, 16)
-    q = 2 * r.standard_normal((10, 4 * 64), dtype=np.float32)
-    clean, clean_lse = attend(ctx, cache, batch, q, 4)
-    check(cache, batch, q, 4, clean, clean_lse)
+    heads, rows = kv_heads * group, sum(news)
+    cache, batch = make(ctx, r, [40, 21], news, kv_heads, hd, 16)
+    q = 2 * r.standard_normal((rows, heads * hd), dtype=np.float32)
+    clean, clean_lse = attend(ctx, cache, batch, q, heads)
+    check(cache, batch, q, heads, clean, clean_lse)
     p = cache.pools
     used = np.zeros((p.pages, 16), bool)
     for b, n in enumerate(batch.lens):
@@ -364,20 +369,52 @@ def test_what_a_row_does_not_see_does_not_count(ctx):
         s = p.scales[side].transpose(0, 2, 1, 3)
         s[~used] = np.array([np.nan, np.inf, -np.inf, np.nan], np.float16)[r.integers(0, 4, s[~used].shape)]
         p.scales[side] = s.transpose(0, 2, 1, 3)
-    o, lse = attend(ctx, Cache(ctx, p), batch, q, 4)
+    o, lse = attend(ctx, Cache(ctx, p), batch, q, heads)
     assert same_bits(o, clean) and same_bits(lse, clean_lse)
-    # position 36 of the first sequence is new: rows 31..35 are before it
+    # the first sequence's last-but-one token: of its new rows the last two see it
+    at = 38
+    sees = np.array([b == 0 and pos >= at for b, pos in batch.positions()])
+    assert sees.sum() == 2
     for side in (0, 1):
         keep = p.raw.copy()
-        p.scales[side, batch.table[0, 2], :, 4] = np.nan
-        o, lse = attend(ctx, Cache(ctx, p), batch, q, 4)
+        p.scales[side, batch.table[0, at // 16], :, at % 16] = np.nan
+        o, lse = attend(ctx, Cache(ctx, p), batch, q, heads)
         p.raw = keep
-        assert np.isnan(o[5:9]).all()  # (the row's own position is 36, and all after it)
-        seen = np.array([0, 1, 2, 3, 4, 9])
-        assert np.isfinite(o[seen]).all()
-        np.testing.assert_allclose(o[seen], clean[seen], rtol=0, atol=2**-13)
+        assert np.isnan(o[sees]).all()
+        assert np.isfinite(o[~sees]).all()
+        np.testing.assert_allclose(o[~sees], clean[~sees], rtol=0, atol=2**-13)
         if side == 0:
-            assert same_bits(np.ascontiguousarray(lse[seen]), np.ascontiguousarray(clean_lse[seen]))
+            assert same_bits(np.ascontiguousarray(lse[~sees]), np.ascontiguousarray(clean_lse[~sees]))
+
+
+def test_long_rows_do_not_drift(ctx):
+    """Many keys for each warp: sums of hundreds of tiles stay within 2^-19 of the mean square."""
+    r = np.random.default_rng(16)
+    n, B = 16000, 40
+    cache, batch = make(ctx, r, [n], None, 1, 32, 64)
+    batch = Batch(ctx, np.repeat(batch.table, B, 0), [n] * B)
+    q = np.repeat(2 * r.standard_normal((1, 8 * 32), dtype=np.float32), B, 0)
+    o, lse = attend(ctx, cache, batch, q, 8)
+    want, want_lse, _ = ref.attend(cache.pools, batch.table[:1], [n], None, q[:1], 8)
+    for row in range(B):
+        assert np.linalg.norm(o[row] - want[0]) <= 2**-19 * np.linalg.norm(want[0])
+        assert np.abs(lse[row] - want_lse[0]).max() <= 2**-19
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 3e38])
+def test_a_bad_query_spoils_its_own_row_alone(ctx, bad):
+    r = np.random.default_rng(17)
+    for heads, news in ((8, None), (2, None), (8, [5, 1])):
+        cache, batch = make(ctx, r, [90, 33], news, 2, 64, 16)
+        q = 2 * r.standard_normal((batch.rows, heads * 64), dtype=np.float32)
+        clean, clean_lse = attend(ctx, cache, batch, q, heads)
+        q[0, 64 + 5] = bad
+        o, lse = attend(ctx, cache, batch, q, heads)
+        keep = np.ones_like(o, bool)
+        keep[0, 64:128] = False
+        assert same_bits(o[keep], clean[keep])
+        if not bad == 3e38:  # (a score beyond fp32's range, or not)
+            assert np.isnan(o[0, 64:128]).all()
 
 
 def test_attention_reports_bad_tables_and_goes_on(ctx):
