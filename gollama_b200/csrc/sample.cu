@@ -36,7 +36,7 @@ namespace {
 
 constexpr int NT = 512, NW = NT / 32;
 constexpr int BINS = 8192;
-constexpr int CAP = NT;          // tokens that are ranked at once, one per thread
+constexpr int CAP = 512;         // tokens that are ranked at once, one per thread
 constexpr int POWERS = 256;      // bins, and table entries, per factor of two of the weight
 constexpr int DIGIT = 10;        // bits of the order per step of narrowing
 constexpr int MAX_CLUSTER = 8;
@@ -44,8 +44,8 @@ constexpr int SLICE_MAX = 43008; // tokens of a CTA: 168 KB of its shared memory
 constexpr uint32_t ONE = 1u << 31;  // the largest weight
 constexpr int GROUPS = BINS / 32;
 static_assert(2 << DIGIT <= BINS && 32 * POWERS == BINS, "digits (two sums each) and weights have a bin");
-static_assert(CAP == NT && GROUPS % 32 == 0, "a thread per listed token, a lane per group of bins");
-static_assert(BINS == 16 * NT && GROUPS <= NT && 32 * MAX_CLUSTER <= NT, "a thread per group, and per bin of a group and CTA");
+static_assert(CAP <= NT && GROUPS % 32 == 0, "a thread per listed token, a lane per group of bins");
+static_assert(BINS <= 16 * NT && GROUPS <= NT && 32 * MAX_CLUSTER <= NT, "a thread per group, and per bin of a group and CTA");
 static_assert(SLICE_MAX < (1 << 16), "sums of 16-bit numbers over a slice have 32 bits");
 
 struct Sample {
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
         if (i < ctas && tid >= end) peer = i + 1, at = tid - end;
       }
       const u64 order = tid < m ? cluster.map_shared_rank(&s, peer)->list[at] : 0;
-      s.pulled[tid] = order;
+      if (tid < CAP) s.pulled[tid] = order;
       __syncthreads();
       if (tid < m) {
         int r = 0;
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
         }
       }
       tell(more, [](Shared& o) -> u64* { return o.bases; });
-      if (tid < s.listed[round & 1]) {  // (tell's barrier: the places are there)
+      if (tid < CAP && tid < s.listed[round & 1]) {  // (tell's barrier: the places are there)
         const int i = static_cast<int>(s.list[tid]);
         s.list[tid] = order_of(plain(src[i]), first + i);
       }
