@@ -44,9 +44,8 @@ __device__ __forceinline__ RowAt row_at(const KvPools& c, const KvSeqs& s, int t
 // magnitude is three shuffles.  blockIdx.x covers the heads of a row (queries,
 // keys, values, in that order), blockIdx.y the rows, `step` in a row for a block.
 __global__ void __launch_bounds__(256)
-    kv_append_kernel(KvPools c, KvSeqs s, const float* __restrict__ q, size_t q_ld, float* __restrict__ q_out,
-                     size_t q_out_ld, int heads, const float* __restrict__ k, size_t k_ld,
-                     const float* __restrict__ v, size_t v_ld, const float* __restrict__ cos_t,
+    kv_append_kernel(KvPools c, KvSeqs s, const float* q, size_t q_ld, float* q_out, size_t q_out_ld, int heads,
+                     const float* k, size_t k_ld, const float* v, size_t v_ld, const float* __restrict__ cos_t,
                      const float* __restrict__ sin_t, int table_rows, int step, int* __restrict__ err) {
   GLC_PDL_ENTRY();
   __shared__ RowAt at_s[ROWS];
@@ -248,8 +247,8 @@ int kv_check(Context* ctx, const char* what, const glc_kv_cache* cache, const gl
   if (batch->num_seqs > 0 && (!batch->page_table || !batch->lens)) return no("page_table and lens must be given");
   if (!batch->starts && batch->num_rows < batch->num_seqs)
     return no("without starts, num_rows must be at least num_seqs");
-  if (static_cast<long long>(batch->max_pages) * cache->page_size > 0x7fffffff)
-    return no("max_pages * page_size must stay below 2^31");
+  if (static_cast<long long>(batch->max_pages) * cache->page_size > 0x40000000)
+    return no("max_pages * page_size must be at most 2^30");
   return GLC_OK;
 }
 
@@ -280,7 +279,7 @@ int glc_kv_append(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* b
   if (rc) return rc;
   auto no = [&](const char* why) { return c->fail(GLC_ERR_INVALID, std::string("kv_append: ") + why); };
   const long long kv_width = static_cast<long long>(cache->num_kv_heads) * cache->head_dim;
-  const long long q_width = static_cast<long long>(num_heads) * cache->head_dim;
+  const long long q_width = q ? static_cast<long long>(num_heads) * cache->head_dim : 0;
   if ((q == nullptr) != (q_out == nullptr)) return no("q and q_out must both be given, or neither");
   if (q && num_heads <= 0) return no("num_heads must be positive");
   if ((cos_t == nullptr) != (sin_t == nullptr)) return no("cos_t and sin_t must both be given, or neither");
@@ -298,7 +297,7 @@ int glc_kv_append(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* b
   const int heads = q ? num_heads : 0;
   const int units = (heads + 2 * cache->num_kv_heads) * (cache->head_dim / 4);
   const double moved = static_cast<double>(batch->num_rows) *
-                       (8.0 * (q ? q_width : 0) + (8.0 + 9.0 / 8.0) * kv_width);
+                       (8.0 * q_width + (8.0 + 9.0 / 8.0) * kv_width);
   glc::ProfScope prof(c, glc::PROF_OTHER, moved, c->stream);
   const glc::RowGrid g = glc::row_grid(c, units, batch->num_rows, glc::MOST);
   glc::launch_pdl(c, glc::kv_append_kernel, g.grid, 256, 0, c->stream,

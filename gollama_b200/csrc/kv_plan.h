@@ -67,7 +67,7 @@ struct KvSpan {
 KV_HD KvSpan kv_span(const KvSeqs& s, int page, int b, int* err) {
   KvSpan r;
   r.len = s.lens[b];
-  const int most = s.max_pages * page;  // below 2^31, checked by the host
+  const int most = s.max_pages * page;  // at most 2^30, checked by the host
   if (r.len < 0 || r.len > most) {
     kv_bad(err);
     r.len = r.len < 0 ? 0 : most;

@@ -403,7 +403,7 @@ typedef struct glc_kv_batch {
   const int* lens;       /* [num_seqs] */
   const int* starts;     /* [num_seqs + 1], ascending, or NULL */
   int num_seqs;
-  int max_pages;
+  int max_pages;         /* max_pages * page_size at most 2^30 */
   int num_rows;          /* rows of the operands */
 } glc_kv_batch;
 

@@ -169,7 +169,7 @@ CACHES = [("cache", None, INVALID), ("cache", cache_of(num_pages=0), INVALID), (
           ("cache", cache_of(hd=256), UNSUPPORTED), ("cache", cache_of(k=0), INVALID), ("cache", cache_of(v=8), INVALID),
           ("batch", None, INVALID), ("batch", good_batch(rows=-1), INVALID), ("batch", good_batch(seqs=-1), INVALID),
           ("batch", good_batch(max_pages=0), INVALID), ("batch", good_batch(rows=3), INVALID),
-          ("batch", good_batch(max_pages=1 << 28), INVALID), ("batch", KVBatchC(num_seqs=2, max_pages=2, num_rows=2), INVALID)]
+          ("batch", good_batch(max_pages=(1 << 26) + 1), INVALID), ("batch", KVBatchC(num_seqs=2, max_pages=2, num_rows=2), INVALID)]
 
 
 def refused(call, name, base, field, value, code):
