@@ -187,6 +187,11 @@ struct Unpack {
   }
 };
 
+__device__ __forceinline__ int arrive(int* count) {
+  int before;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+  return before;
+}
 // (M, L, o) += the part (m, l, y)
 __device__ __forceinline__ void add_part(float m, float l, float4 y, float* M, float* L, float4* o) {
   const float now = fmaxf(*M, m), ns = now == -INFINITY ? 0.f : now;
@@ -216,11 +221,14 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
   const int g = lane >> 2, t = lane & 3;
 
   // ---- the share of this CTA: thread i counts the units of its run of
-  // sequences, a scan over the threads finds the run that the share begins in
+  // sequences, a scan over the threads finds the run that the share begins in; of
+  // up to 32 sequences each warp counts by itself, without barriers
   {
     if (tid == 0) place.b = -1;
+    const bool few = a.s.seqs <= 32;
+    const int me = few ? lane : tid;
     const int run = a.s.seqs <= W * 32 ? 1 : (a.s.seqs + W * 32 - 1) / (W * 32);
-    const int b0 = tid * run < a.s.seqs ? tid * run : a.s.seqs;
+    const int b0 = me * run < a.s.seqs ? me * run : a.s.seqs;
     const int b1 = b0 + run < a.s.seqs ? b0 + run : a.s.seqs;
     KvRows w = {};
     if (b0 < b1) w = kv_rows(a.s, a.c.page, a.toks, a.parts, b0, a.err);
@@ -236,11 +244,15 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
         const int v = __shfl_up_sync(~0u, upto, o);
         if (lane >= o) upto += v;
       }
+      *mine = y;
+      *before = upto - y;
+      if (few) {
+        *total = __shfl_sync(~0u, upto, 31);
+        return;
+      }
       int* sums = sum_s[calls++ & 1];
       if (lane == 31) sums[warp] = upto;
       __syncthreads();
-      *mine = y;
-      *before = upto - y;
       *total = 0;
 #pragma unroll
       for (int i = 0; i < W; ++i) {
@@ -264,6 +276,8 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
         break;
       }
     }
+    if (few && warp) mine = 0;  // the first warp says
+    __syncwarp();               // (place.b is -1)
     if (before <= begin && begin < before + mine) {
       place.total = total;
       place.ctas = ctas;
@@ -799,47 +813,58 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     if (!whole) {
       // ---- the last of the item's CTAs to arrive joins the parts
       const int first_cta = kv_first_cta(p), last_cta = kv_last_cta(p);
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
-        last_s = atomicAdd(a.count + first_cta, 1) == last_cta - first_cta;
+        // releases the CTA's part (its writes are before the barrier) and acquires the others'
+        last_s = arrive(a.count + first_cta) == last_cta - first_cta;
         if (last_s) a.count[first_cta] = 0;
       }
       __syncthreads();
       if (last_s) {
-        __threadfence();
-        // groups of threads take every GROUPSth part, and join through shared memory
+        // a thread has PER elements of every part; where there are more threads than
+        // elements, groups of them take every GROUPSth part and join in shared memory
         constexpr int ELEMS = RT * HD / 4, GROUPS = ELEMS < W * 32 ? W * 32 / ELEMS : 1;
-        float4* so = reinterpret_cast<float4*>(smem);
-        float2* sm = reinterpret_cast<float2*>(smem + GROUPS * ELEMS * 16);
-        for (int i0 = 0; i0 < ELEMS; i0 += W * 32) {
-          const int group = GROUPS > 1 ? tid / ELEMS : 0, i = GROUPS > 1 ? tid - group * ELEMS : i0 + tid;
-          const int r = i / (HD / 4), c4 = i - r * (HD / 4);
-          float M = -INFINITY, L = 0.f;
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (group < GROUPS && i < ELEMS) {
-#pragma unroll 8
-            for (int x = first_cta + group; x <= last_cta; x += GROUPS) {
-              const float* y0 = a.part + static_cast<size_t>(2 * x + (x == first_cta ? 1 : 0)) * RT * (HD + 2);
-              add_part(__ldcg(y0 + RT * HD + r), __ldcg(y0 + RT * HD + RT + r),
-                       __ldcg(reinterpret_cast<const float4*>(y0) + i), &M, &L, &o);
-            }
-          }
-          if constexpr (GROUPS > 1) {
-            if (group < GROUPS) {
-              so[group * ELEMS + i] = o;
-              if (c4 == 0) sm[group * RT + r] = make_float2(M, L);
-            }
-            __syncthreads();
-            if (group == 0) {
+        constexpr int PER = (ELEMS + W * 32 - 1) / (W * 32);
+        const int group = GROUPS > 1 ? tid / ELEMS : 0, i0 = GROUPS > 1 ? tid - group * ELEMS : tid;
+        float M[PER], L[PER];
+        float4 o[PER];
 #pragma unroll
-              for (int x = 1; x < GROUPS; ++x) {
-                const float2 ml = sm[x * RT + r];
-                add_part(ml.x, ml.y, so[x * ELEMS + i], &M, &L, &o);
-              }
+        for (int k = 0; k < PER; ++k) M[k] = -INFINITY, L[k] = 0.f, o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (group < GROUPS) {
+#pragma unroll(PER > 2 ? 2 : 8 / PER)
+          for (int x = first_cta + group; x <= last_cta; x += GROUPS) {
+            const float* y = a.part + static_cast<size_t>(2 * x + (x == first_cta ? 1 : 0)) * RT * (HD + 2);
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+              const int i = i0 + k * W * 32, r = i / (HD / 4);
+              if (i < ELEMS)
+                add_part(__ldcg(y + RT * HD + r), __ldcg(y + RT * HD + RT + r), __ldcg(reinterpret_cast<const float4*>(y) + i),
+                         &M[k], &L[k], &o[k]);
             }
           }
-          if (group == 0 && i < ELEMS && r < rows) write(r, c4, M, L, o);
+        }
+        if constexpr (GROUPS > 1) {
+          float4* so = reinterpret_cast<float4*>(smem);
+          float2* sm = reinterpret_cast<float2*>(smem + GROUPS * ELEMS * 16);
+          if (group < GROUPS) {
+            so[group * ELEMS + i0] = o[0];
+            if (i0 % (HD / 4) == 0) sm[group * RT + i0 / (HD / 4)] = make_float2(M[0], L[0]);
+          }
+          __syncthreads();
+          if (group == 0) {
+#pragma unroll
+            for (int x = 1; x < GROUPS; ++x) {
+              const float2 ml = sm[x * RT + i0 / (HD / 4)];
+              add_part(ml.x, ml.y, so[x * ELEMS + i0], &M[0], &L[0], &o[0]);
+            }
+          }
+        }
+        if (group == 0) {
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            const int i = i0 + k * W * 32, r = i / (HD / 4);
+            if (i < ELEMS && r < rows) write(r, i - r * (HD / 4), M[k], L[k], o[k]);
+          }
         }
       }
     }

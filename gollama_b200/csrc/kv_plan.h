@@ -235,8 +235,13 @@ KV_HD void kv_place(KvPlace* p, const KvRows& w, int b, int unit, int per, int a
   p->b = b;
   p->w = w;
   p->alone = alone;
-  int first;
-  p->tile = kv_find_tile(w, unit, per, at - p->h * per_head, &first, &p->units);
+  int first = 0;
+  if (w.tiles == 1) {
+    p->tile = 0;
+    p->units = kv_run_units(w, 0, unit);
+  } else {
+    p->tile = kv_find_tile(w, unit, per, at - p->h * per_head, &first, &p->units);
+  }
   const int piece = at - p->h * per_head - first;  // of the tile
   if (alone) {
     p->item_at = 0;
