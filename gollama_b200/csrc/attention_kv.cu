@@ -101,16 +101,6 @@ __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uin
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-// (x0, x1) += (y0, y1), each rounded to nearest
-__device__ __forceinline__ void add_pair(float* x, const float* y) {
-  asm("{\n\t.reg .b64 a, b;\n\t"
-      "mov.b64 a, {%0, %1};\n\t"
-      "mov.b64 b, {%2, %3};\n\t"
-      "add.rn.f32x2 a, a, b;\n\t"
-      "mov.b64 {%0, %1}, a;\n\t}"
-      : "+f"(x[0]), "+f"(x[1])
-      : "f"(y[0]), "f"(y[1]));
-}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -309,7 +299,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
   for (int j = 0; j < 4; ++j) swizzled[j] = codes_to + ((lane8 * 16) ^ Tile::swizzle(j));
   // a warp's tiles lie UNIT keys apart
-  const int scales_from = a.c.scales_at;
+  const uint32_t scales_from = a.c.scales_at;
   const int step_pages = (UNIT / 16) / page16, step_slot = (UNIT / 16) % page16;
 
   const Unpack unpack{a.k1024, a.less72};
@@ -353,39 +343,45 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
         x[i][4] = v.x, x[i][5] = v.y, x[i][6] = v.z, x[i][7] = v.w;
       }
     }
-    auto table_page = [&](int index) {
-      const int p = table[index];
-      if (static_cast<unsigned>(p) < static_cast<unsigned>(a.c.num_pages)) return p;
-      kv_bad(a.err);
-      return -1;
-    };
-    // the lane's group of 16 tokens in the warp's next tile, and its page
+    // The lane's group of 16 tokens in the warp's next tile: its page (-1: none), and
+    // where its codes and scales are in that.  An index that is no page is noted, and
+    // said at the end.
     int next = key0 + warp * WK;
     KvWalk walk;
     walk.start(next + 16 * grp, page16);
-    int page = next + 16 * grp < key1 ? table_page(walk.index) : -1;
+    bool bad = false;
+    auto table_page = [&] {
+      int p = -1;
+      if (next + 16 * grp < key1) {
+        p = table[walk.index];
+        bad |= static_cast<unsigned>(p) >= static_cast<unsigned>(a.c.num_pages);
+      }
+      return static_cast<unsigned>(p) < static_cast<unsigned>(a.c.num_pages) ? p : -1;
+    };
+    int page = table_page();
 
-    // copies the tile at `next` to a stage and looks the following one's page up.
-    // A group has whole pages of 16 slots, so the slots behind the last key are
-    // copied too: their codes are numbers, their scales are not used.
-    auto fetch = [&](int stage) {
+    // copies the tile at `next` to the stage at `to` and looks the following one's
+    // page up.  A group has whole pages of 16 slots, so the slots behind the last key
+    // are copied too: their codes are numbers, their scales are not used.
+    uint32_t to = 0;
+    auto fetch = [&] {
       if (next < key1) {
         const uint8_t* from = head + static_cast<uint64_t>(page < 0 ? 0 : page) * page_bytes;
-        const uint8_t* codes = from + walk.slot * (16 * Tile::ROW);
-        const uint8_t* scales = from + walk.slot * (32 * NB);
+        const uint8_t* codes = from + static_cast<uint32_t>(walk.slot) * (16 * Tile::ROW);
+        const uint8_t* scales = from + (static_cast<uint32_t>(walk.slot) * (32 * NB) + scales_from);
         const int size = page < 0 ? 0 : 16;  // 0: zeros are stored, nothing is read
-        const uint32_t to = stage * Tile::BYTES;
 #pragma unroll
         for (int j = 0; j < Tile::LANE_PIECES; ++j) copy16(swizzled[j & 3] + to + 128 * j, codes + 128 * j, size);
-        if (lane8 < Tile::GROUP_SCALES) copy16(scales_to + to, scales + scales_from, size);
+        if (lane8 < Tile::GROUP_SCALES) copy16(scales_to + to, scales, size);
+        to = to == (STAGES - 1) * Tile::BYTES ? 0 : to + Tile::BYTES;
         next += UNIT;
         walk.advance(step_pages, step_slot, page16);
-        page = next + 16 * grp < key1 ? table_page(walk.index) : -1;
+        page = table_page();
       }
       copies_close();
     };
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+    for (int i = 0; i < STAGES - 1; ++i) fetch();
 
     // ---- the queries as operands, a tile of 8 rows per warp: lane (g, t) has
     // elements 8t .. 8t + 7 of each block of row g, in the order in which the codes
@@ -446,12 +442,12 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     uint32_t vtop = 0;  // largest scale (bits) that vexp allows
     uint32_t up1 = 0x3c003c00u, up2 = 0x3c003c00u;  // 2^vexp, in pairs of halves
 
-    int stage = 0;
+    uint32_t stage = 0;  // bytes
     for (int key = key0 + warp * WK; key < key1; key += UNIT) {
       copies_wait<STAGES - 2>();
       __syncwarp();  // the tile is there for all lanes, and all are done with the last one's stage
-      fetch(stage == 0 ? STAGES - 1 : stage - 1);
-      const uint32_t from = ring_u + stage * Tile::BYTES;
+      fetch();
+      const uint32_t from = ring_u + stage;
       bool odd_scale;  // some value scale is infinite or not a number
       {
         // lane = key: its scales, zero behind the last key
@@ -563,6 +559,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
       if constexpr (PAIRED) {
         const float rs = rs_s[t];
         if (edge) {
+          __syncwarp();  // (a branch, not selects)
           const int last = row_last(t);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
@@ -606,6 +603,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
       for (int n = 0; n < NQ; ++n) {
         const float2 rs = *reinterpret_cast<const float2*>(rs_s + 8 * n + 2 * t);
         if (edge) {
+          __syncwarp();  // (a branch, not selects)
           const int last0 = row_last(8 * n + 2 * t), last1 = row_last(8 * n + 2 * t + 1);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
@@ -692,7 +690,9 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
               mma16816(y[e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], p[2 * j], p[2 * j + 1],
                        j ? y[e] : zero);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) add_pair(acc[0][i][e], y[e]), add_pair(acc[0][i][e] + 2, y[e] + 2);
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) acc[0][i][e][z] += y[e][z];
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -724,12 +724,15 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
               mma16816(y[e], va[j][4 * e], va[j][4 * e + 1], va[j][4 * e + 2], va[j][4 * e + 3], pl[2 * j], pl[2 * j + 1], y[e]);
           }
 #pragma unroll
-          for (int e = 0; e < 2; ++e) add_pair(acc[n][i][e], y[e]), add_pair(acc[n][i][e] + 2, y[e] + 2);
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) acc[n][i][e][z] += y[e][z];
         }
       }
-      stage = stage == STAGES - 1 ? 0 : stage + 1;
+      stage = stage == (STAGES - 1) * Tile::BYTES ? 0 : stage + Tile::BYTES;
     }
     copies_wait<0>();
+    if (bad) kv_bad(a.err);
 
     // ---- the warps' parts of the segment joined through shared memory
     const float down = __uint_as_float(static_cast<uint32_t>(127 - PEXP - vexp) << 23);
