@@ -59,8 +59,13 @@ struct Shape {
   static constexpr int NB = Tile::NB;
   static constexpr int RT = NQ ? 8 * NQ : 4;  // query rows of an item
   static constexpr int STAGES = HD >= 96 ? 2 : 3;
-  // CTAs of an SM: 16 warps of 128 registers or 20 of 96, or 12 of 168 with more rows
-  static constexpr int PER_SM = W == 16 ? 1 : (NQ > 2 && HD >= 96 ? 8 : NQ > 1 ? 12 : HD >= 96 ? 16 : 20) / W;
+  // CTAs of an SM: 12 warps of 168 registers, of narrow heads 16 of 128.  More warps
+  // with fewer registers compute addresses again and again: at 128 a tile of 128
+  // elements takes 757 instructions, at 168 680 (64 x 8192 tokens, 32/8 heads of
+  // 128: 114.5 and 111.7 us); a tile of 64 at 96, 128 and 168 takes 560, 513 and 464
+  // (128 x 4096 tokens, 32/4 heads of 64: 49.2, 45.8 and 48.0 us).
+  static constexpr int WIDE = HD >= 96;
+  static constexpr int PER_SM = W >= 12 ? 1 : (NQ > 2 && WIDE ? 8 : NQ > 1 || WIDE ? 12 : 16) / W;
   static constexpr int SCALES = WK * NB * 6;  // a tile's scales as the products take them
   static constexpr int WARP = STAGES * Tile::BYTES + SCALES;
   static constexpr int QUERIES = NQ ? NQ * NB * 1024 : NB * 512;  // the queries as operands
