@@ -39,6 +39,24 @@ __device__ __forceinline__ RowAt row_at(const KvPools& c, const KvSeqs& s, int t
   return r;
 }
 
+// Codes of 4 elements where x (1 / d) may lie to the wrong side of a half: the
+// residual x - n d is exact (n d has 15 bits, and the difference lies on x's grid
+// and below d), and is held against d / 2.
+__device__ __noinline__ unsigned nearest_codes(const float* x, float d, float rd) {
+  const float edge = 0.5f * fabsf(d);
+  unsigned bits = 0;
+  for (int i = 0; i < 4; ++i) {
+    float n = rintf(__fmul_rn(x[i], rd));
+    n = fminf(fmaxf(n, -16.f), 16.f);
+    const float rest = fmaf(-n, d, x[i]);
+    const float by = (rest < 0.f) == (d < 0.f) ? 1.f : -1.f;
+    if (fabsf(rest) > edge || (fabsf(rest) == edge && (static_cast<int>(n) & 1))) n += by;
+    n = fminf(fmaxf(n, -8.f), 7.f);
+    bits |= static_cast<unsigned>(static_cast<int>(n) + 8) << (4 * i);
+  }
+  return bits;
+}
+
 // A thread holds 4 consecutive elements (two rotation pairs) of one head of
 // one row; 8 neighbouring lanes hold the 32 that share a scale, so the largest
 // magnitude is three shuffles.  blockIdx.x covers the heads of a row (queries,
@@ -122,21 +140,21 @@ __global__ void __launch_bounds__(256)
         const float d = __half2float(d16);
         unsigned bits = 0x8888u;
         if (!nan && d != 0.f) {
-          // the whole number nearest to the exact x / d: a first guess by the
-          // reciprocal, then its residual x - n d, which is exact (n d has 15 bits,
-          // and the difference lies on x's grid and below d), against d / 2
-          const float rd = __frcp_rn(d), edge = 0.5f * fabsf(d);
+          // the whole number nearest to the exact x / d: x (1 / d) is off by 2^-24 of
+          // itself, so below 12 it rounds to the same one unless it is within 10^-6 of
+          // a half (or d was held to the largest half)
+          const float rd = __frcp_rn(d);
+          constexpr float ROUND = 12582912.f;  // 1.5 2^23: the nearest whole number in the low bits of a sum
+          float off = fabsf(m) <= 524032.f ? 0.f : 1.f;
           bits = 0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float n = rintf(__fmul_rn(x[i], rd));
-            n = fminf(fmaxf(n, -16.f), 16.f);
-            const float rest = fmaf(-n, d, x[i]);
-            const float by = (rest < 0.f) == (d < 0.f) ? 1.f : -1.f;
-            if (fabsf(rest) > edge || (fabsf(rest) == edge && (static_cast<int>(n) & 1))) n += by;
-            n = fminf(fmaxf(n, -8.f), 7.f);
-            bits |= static_cast<unsigned>(static_cast<int>(n) + 8) << (4 * i);
+            const float sum = fmaf(x[i], rd, ROUND);
+            off = fmaxf(off, fabsf(fmaf(x[i], rd, ROUND - sum)));
+            const int n = static_cast<int>(__float_as_uint(sum)) - 0x4b400000 + 8;
+            bits |= static_cast<unsigned>(n < 0 ? 0 : n > 15 ? 15 : n) << (4 * i);
           }
+          if (off > 0.499998f) bits = nearest_codes(x, d, rd);
         }
         uint8_t* to = (is_k ? c.k : c.v) + (static_cast<size_t>(place.page) * c.kv_heads + h) * c.chunk;
         reinterpret_cast<uint16_t*>(to + static_cast<size_t>(place.slot) * half)[at] = static_cast<uint16_t>(bits);
