@@ -229,10 +229,14 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     if (b0 < b1) w = kv_rows(a.s, a.c.page, a.toks, a.parts, b0, a.err);
     // pieces of `per` units of the run, those of all before it, and of all
     int calls = 0;
+    bool bad = false;  // starts that do not ascend: nothing is done
     auto count = [&](int per, int* mine, int* before, int* total) {
       int y = 0;
-      for (int b = b0; b < b1; ++b)
-        y += kv_head_pieces(run == 1 ? w : kv_rows(a.s, a.c.page, a.toks, a.parts, b, a.err), UNIT, per) * a.c.kv_heads;
+      for (int b = b0; b < b1; ++b) {
+        if (run > 1) w = kv_rows(a.s, a.c.page, a.toks, a.parts, b, a.err);
+        bad |= w.bad;
+        y += kv_head_pieces(w, UNIT, per) * a.c.kv_heads;
+      }
       int upto = y;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -243,11 +247,12 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
       *before = upto - y;
       if (few) {
         *total = __shfl_sync(~0u, upto, 31);
+        bad = __any_sync(~0u, bad);
         return;
       }
       int* sums = sum_s[calls++ & 1];
       if (lane == 31) sums[warp] = upto;
-      __syncthreads();
+      bad = __syncthreads_or(bad);
       *total = 0;
 #pragma unroll
       for (int i = 0; i < W; ++i) {
@@ -257,6 +262,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     };
     int mine, before, total;
     count(1, &mine, &before, &total);
+    if (bad) return;  // the same for the whole CTA, and for all of them
     const int ctas = total < static_cast<int>(gridDim.x) ? total : static_cast<int>(gridDim.x);
     if (static_cast<int>(blockIdx.x) >= ctas) return;
     // one piece of one item for each CTA, where pieces come out even enough
@@ -789,7 +795,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
           make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
       if (a.lse && c4 == 0)
         a.lse[static_cast<size_t>(tk) * a.c.kv_heads * a.group + hh] =
-            M == -INFINITY ? -INFINITY : M * 0.69314718055994531f + logf(L);
+            M == -INFINITY ? (L == 0.f ? -INFINITY : L) : M * 0.69314718055994531f + logf(L);  // (L: or NaN)
     };
     for (int i = tid; i < RT * HD / 4; i += W * 32) {
       const int r = i / (HD / 4), c4 = i - r * (HD / 4);
@@ -967,10 +973,8 @@ extern "C" int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const g
   const int group = num_heads / cache->num_kv_heads;
   if (static_cast<long long>(batch->num_rows) * group > 0x40000000) return no("too many query rows");
   if (glc::kv_pools(*cache).chunk * cache->num_kv_heads > 0xffffffffu) return no("a page must stay below 4 GB");
-  // units of the smallest tiles and units, at most: they are counted in 32 bits
-  const double units = (static_cast<double>(batch->num_rows) * ((group + 7) / 8) + batch->num_seqs) * cache->num_kv_heads *
-                       (static_cast<double>(batch->max_pages) * cache->page_size / 128 + 1);
-  if (units > 2147483647.0) return no("num_rows, num_kv_heads and max_pages are too large together");
+  if (glc::kv_most_units(batch->num_rows, batch->num_seqs, group, cache->num_kv_heads, batch->max_pages, cache->page_size) >
+      2147483647.0) return no("num_rows, num_kv_heads and max_pages are too large together");
   if (batch->num_rows == 0 || batch->num_seqs == 0) return GLC_OK;
   glc::DeviceScope on(c);
   glc::AttnKv a;

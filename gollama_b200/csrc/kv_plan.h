@@ -63,6 +63,7 @@ KV_HD void kv_bad(int* err) {
 // where they go beyond it.
 struct KvSpan {
   int first, n, len;
+  bool bad;  // its starts do not ascend within the operands' rows
 };
 KV_HD KvSpan kv_span(const KvSeqs& s, int page, int b, int* err) {
   KvSpan r;
@@ -74,6 +75,7 @@ KV_HD KvSpan kv_span(const KvSeqs& s, int page, int b, int* err) {
   }
   r.first = b;
   r.n = 1;
+  r.bad = false;
   if (s.starts) {
     r.first = s.starts[b];
     const int end = s.starts[b + 1];
@@ -81,6 +83,7 @@ KV_HD KvSpan kv_span(const KvSeqs& s, int page, int b, int* err) {
       kv_bad(err);
       r.first = 0;
       r.n = 0;
+      r.bad = true;
     } else {
       r.n = end - r.first;
     }
@@ -126,6 +129,9 @@ KV_HD int kv_page(const KvSeqs& s, int num_pages, int b, int index, int* err) {
 
 constexpr int KV_WK = 32;  // keys of a warp's tile
 
+// The sequences' rows are disjoint only if every one's starts ascend: only then is the
+// sum of their units what the host allowed for, so one bad pair ends the whole call.
+
 // The items of one KV head of a sequence.  A tile of `rt` query rows holds the
 // heads of `toks` whole tokens, or, where a group has more heads than that, up to
 // rt heads of one token (`parts` tiles per token).  Tile i sees the keys of its
@@ -133,6 +139,7 @@ constexpr int KV_WK = 32;  // keys of a warp's tile
 // writes its rows).
 struct KvRows {
   int first, n, len, toks, parts, tiles;
+  bool bad;
 };
 KV_HD KvRows kv_rows(const KvSeqs& s, int page, int toks, int parts, int b, int* err) {
   const KvSpan r = kv_span(s, page, b, err);
@@ -140,6 +147,7 @@ KV_HD KvRows kv_rows(const KvSeqs& s, int page, int toks, int parts, int b, int*
   w.first = r.first;
   w.n = r.n;
   w.len = r.len;
+  w.bad = r.bad;
   w.toks = toks;
   w.parts = parts;
   w.tiles = r.n <= toks ? (r.n ? parts : 0) : (r.n + toks - 1) / toks * parts;
@@ -198,6 +206,13 @@ KV_HD int kv_find_tile(const KvRows& w, int unit, int per, int at, int* first, i
   *first = sum;
   *units = 1;
   return 0;
+}
+
+// Units that a call may have, at most: they are counted in 32 bits.  Of all variants
+// the tiles of 4 rows and the units of 128 keys make the most.
+inline double kv_most_units(double rows, double seqs, double group, double kv_heads, double max_pages, double page) {
+  const double parts = static_cast<double>((static_cast<long long>(group) + 3) / 4);
+  return (rows * parts + seqs) * kv_heads * (max_pages * page / (4 * KV_WK) + 1);
 }
 
 // Of `total` units, CTA c of `ctas` (at most total) has a run of total / ctas, the

@@ -31,6 +31,14 @@ int walk(const KvPools& c, const KvSeqs& s, int group, int rt, int warps, int gr
   const int unit = warps * KV_WK;
   const int toks = group < rt ? rt / group : 1, parts_of = (group + rt - 1) / rt;
   auto rows_of = [&](int b) { return kv_rows(s, c.page, toks, parts_of, b, err); };
+  for (int b = 0; b < s.seqs; ++b)
+    if (rows_of(b).bad) {  // the kernel's CTAs all return
+      for (int i = b; i < s.seqs; ++i) rows_of(i);
+      return 0;
+    }
+  long long all = 0;
+  for (int b = 0; b < s.seqs; ++b) all += static_cast<long long>(kv_head_pieces(rows_of(b), unit, 1)) * c.kv_heads;
+  if (all > kv_most_units(s.rows, s.seqs, group, c.kv_heads, s.max_pages, c.page)) return 100;
   auto pieces_of = [&](int per) {
     int sum = 0;
     for (int b = 0; b < s.seqs; ++b) sum += kv_head_pieces(rows_of(b), unit, per) * c.kv_heads;

@@ -94,6 +94,25 @@ def test_bad_pages_lengths_and_rows_are_neither_read_nor_silent(host):
         assert walk(host, cache, batch_of(ok, [9, 9], starts, rows=6), 2, 4) == (0, BAD)
 
 
+def test_starts_that_do_not_ascend_end_the_whole_call(host):
+    """Sequences that each claim all rows would have more units than the host allowed
+    for: nothing is walked, wherever the bad pair lies."""
+    ok = np.zeros((6, 4), np.int32)
+    for starts in ([0, 40, 0, 40, 0, 40, 0], [0, 1, 2, 3, 4, 5, 4], [3, 2, 3, 4, 5, 6, 7], [0, 40, 40, 0, 40, 40, 40]):
+        got = walk(host, cache_of(8, 16, 1, 64), batch_of(ok, [64] * 6, starts, rows=40), 8, 148, 4, 4)
+        assert got == (0, BAD)
+
+
+def test_units_stay_within_what_the_host_allows_for(host):
+    """Groups of 5 to 8 heads in tiles of 4 rows, idle sequences beside one of many rows
+    (the walk compares its units with the bound)."""
+    for group in (1, 3, 4, 5, 8, 9, 17):
+        for lens, news in (([600, 0, 0, 0, 0], [90, 0, 0, 0, 0]), ([700, 700], [700, 1]), ([0] * 8, [1] * 8), ([512] * 3, [1] * 3)):
+            batch = batch_of(table_for(lens, 16, 8, 2), lens, np.concatenate([[0], np.cumsum(news)]))
+            for rt in (4, 8, 32):
+                assert walk(host, cache_of(8, 16, 2, 32), batch, group, 148, rt, 4) == (0, 0), (group, news, rt)
+
+
 def test_rows_find_their_sequence_and_position(host):
     cache = cache_of(8, 16, 2, 64)
     table = np.zeros((4, 4), np.int32)
@@ -201,6 +220,12 @@ def test_read_refuses_no_output(call):
     ("o_ld", 257, INVALID), ("o", P + 4, INVALID), ("lse", P + 1, INVALID)])
 def test_attention_refuses(call, field, value, code):
     refused(call, "glc_attention_kv", ATTEND, field, value, code)
+
+
+def test_attention_refuses_more_units_than_are_counted(call):
+    # 8 heads in tiles of 4: two tiles a token, 8193 units each
+    batch = KVBatchC(page_table=P, lens=P, starts=P, num_seqs=1, max_pages=65536, num_rows=200000)
+    refused(call, "glc_attention_kv", {**ATTEND, "cache": cache_of(kv_heads=1), "heads": 8, "q_ld": 512, "o_ld": 512}, "batch", batch, INVALID)
 
 
 @pytest.mark.parametrize("field,value,code", [
