@@ -25,6 +25,13 @@
 // own tiles of 32 keys with its own ring of asynchronous copies; the warps of
 // a CTA join at the end of an item.  Items cut between CTAs leave partial
 // (m, l, o); the CTA that arrives last joins them in the order of their keys.
+//
+// It is bound by instructions: a tile of 32 keys of 128 elements takes a warp 680 for
+// 4 query rows (issue slots 0.56 used, the matrix pipe 19 %).  64 sequences of up to
+// 8192 tokens, 32/8 heads of 128, take 112 to 120 us, 0.59 to 0.63 of a plain copy's
+// rate for the 455 MB of cache; 512 new tokens on 4096, 32/4 heads of 64: 0.38 of the
+// matrix pipe.  Small batches are bound by latency: the share of the work, the page
+// table, the copy, the join.
 #include <cfloat>
 
 #include "kv_cache.cuh"
@@ -936,6 +943,13 @@ template <int HD>
 int launch_for(Context* ctx, const AttnKv& a, cudaStream_t s) {
   // Rows that share a KV head of a sequence, on average: as many query tiles in
   // an item as they fill, since an item unpacks its keys and values once.
+  //   up to 4 rows: hi and lo as neighbouring columns of one product, 145 -> 123 us (64
+  //     x 8192 tokens, 32/8 heads of 128);
+  //   narrow heads, more than 24 rows: four tiles (items of 8 rows took 522 us for a
+  //     512-token chunk on 4096, 32/4 heads of 64, items of up to 32 take 409);
+  //   wide heads, 17 to 24 rows: three tiles, 60.5 -> 53.8 us (5 tokens each, 32/8 heads
+  //     of 128).  For longer chunks two (785 us, three 845), and for 24 rows of narrow
+  //     heads two (23.4 us, three 25.0): fewer registers, more warps.
   const long long rows = static_cast<long long>(a.s.rows) * a.group / a.s.seqs;
   if (HD <= 64 && rows > 24) return launch<HD, HD <= 64 ? 4 : 2, 4>(ctx, a, s);
   if constexpr (HD >= 96) {
@@ -943,8 +957,10 @@ int launch_for(Context* ctx, const AttnKv& a, cudaStream_t s) {
   }
   if (rows > 8) return launch<HD, 2, 4>(ctx, a, s);
   // Few items are cut between many CTAs, and few large CTAs leave fewer parts to
-  // join; of many items a CTA has several, and small CTAs overlap one's joins
-  // with another's copies.
+  // join: one sequence of 131072 tokens (32/4 heads of 64) 23.6 us against 39.5 with
+  // CTAs of 4 warps, of 16384 11.0 against 22.2.  Of many items a CTA has several, and
+  // small CTAs overlap one's joins with another's copies: 32 sequences of 2048 take
+  // 14.4 and 14.5 us.
   const long long items = static_cast<long long>(a.s.rows) * ((a.group + 7) / 8) * a.c.kv_heads;
   const bool many = items >= ctx->num_sms / 2;
   if (rows <= 4) return many ? launch<HD, 0, 4>(ctx, a, s) : launch<HD, 0, 16>(ctx, a, s);

@@ -418,7 +418,7 @@ GLC_API int glc_kv_cache_bytes(const glc_kv_cache* cache, size_t* bytes);
  * in floats (multiples of 4), so the operands may be columns of one fused
  * projection; pointers are 16-byte aligned.  cos_t/sin_t: [table_rows]
  * [head_dim/2] of glc_rope_table on the device (both NULL: no rotation; q is
- * copied).  The rotation is glc_rope's, bit for bit.  Of 32 elements x, e the
+ * copied).  Where q_out is q, their strides are equal.  The rotation is glc_rope's, bit for bit.  Of 32 elements x, e the
  * one of largest magnitude (the first of equals): scale = half(e / -8), held
  * to +-65504, and code = 8 + the whole number nearest to x / scale (ties to
  * even) held to [-8, 7]; a scale of zero has codes 8; an infinity or a NaN
@@ -438,7 +438,8 @@ GLC_API int glc_kv_read(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_ba
  * h / (num_heads / num_kv_heads).  q, o: [num_rows][num_heads * head_dim] with
  * row strides in floats (multiples of 4); lse (nullable): [num_rows]
  * [num_heads], the natural logarithm of the softmax's sum.  A token with no
- * visible position (lens[b] == 0) gets o = 0 and lse = -infinity.  The
+ * visible position (lens[b] == 0) gets o = 0 and lse = -infinity.  Starts that
+ * do not ascend within [0, num_rows] end the whole call, with nothing written.  The
  * products use the cache's exact values and q and the probabilities to 22
  * bits, the sums are float32.  Deterministic.  Uses the context workspace. */
 GLC_API int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* batch, const float* q,
@@ -452,9 +453,9 @@ GLC_API int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const glc_
  * order, the first token whose running sum of probability exceeds uniform *
  * the kept sum.  Settings are one value per row in device memory; uniform in
  * [0, 1).  A temperature that is not positive takes the largest logit; top_k
- * <= 0, top_p >= 1 and min_p <= 0 keep all; top_p <= 0 and min_p >= 1 keep
- * the first, and the equals of the first; any of top_k, top_p and min_p may be NULL.  A NaN
- * counts as -infinity; -infinity is never drawn; where a row has nothing else
+ * <= 0, top_p >= 1 and min_p <= 0 keep all; top_p <= 0 keeps the first token
+ * alone, min_p >= 1 the largest logit and its equals; any of top_k, top_p and
+ * min_p may be NULL.  A NaN logit counts as -infinity; -infinity is never drawn; where a row has nothing else
  * its token is -1 and its logp -infinity.  logp (nullable): the natural
  * logarithm of the drawn token's share of the kept probability.  Weights are
  * whole numbers of 2^-31 of the largest, so that sums do not depend on their

@@ -415,6 +415,8 @@ def test_a_bad_query_spoils_its_own_row_alone(ctx, bad):
         assert same_bits(o[keep], clean[keep])
         if not bad == 3e38:  # (a score beyond fp32's range, or not)
             assert np.isnan(o[0, 64:128]).all()
+        if np.isnan(bad):  # every score is NaN, and so is the sum
+            assert np.isnan(lse[0, 1]) and np.isfinite(np.delete(lse.ravel(), 1)).all()
 
 
 def test_attention_reports_bad_tables_and_goes_on(ctx):
@@ -437,6 +439,43 @@ def test_attention_reports_bad_tables_and_goes_on(ctx):
     batch.d[1].upload(np.array([100, 50], np.int32))
     o, _ = attend(ctx, cache, batch, q, 4)
     assert same_bits(o, clean)
+
+
+@pytest.mark.parametrize("seqs", [3, 40])
+def test_starts_that_do_not_ascend_end_the_attention(ctx, seqs):
+    """Reported, and no row is written; the next call is whole."""
+    r = np.random.default_rng(18)
+    lens, news = [20 + i for i in range(seqs)], [2] * seqs
+    cache, batch = make(ctx, r, lens, news, 2, 64, 16)
+    heads = 4
+    q = 2 * r.standard_normal((batch.rows, heads * 64), dtype=np.float32)
+    clean, _ = attend(ctx, cache, batch, q, heads)
+    good = np.array(batch.starts, np.int32)
+    for at, value in ((1, 5), (seqs, 1), (0, -1), (seqs, 2 * seqs + 1)):
+        bad = good.copy()
+        bad[at] = value
+        batch.d[2].upload(bad)
+        dq, o = ctx.from_numpy(q), ctx.from_numpy(np.full(q.shape, CANARY))
+        ctx.call("glc_attention_kv", C.byref(cache.c), C.byref(batch.c), dq.addr, q.shape[1], heads, o.addr, q.shape[1], 0)
+        with pytest.raises(GlcError, match="out of range"):
+            ctx.sync()
+        assert (o.numpy() == CANARY).all(), (at, value)
+    batch.d[2].upload(good)
+    o, _ = attend(ctx, cache, batch, q, heads)
+    assert same_bits(o, clean)
+
+
+def test_attention_in_place_and_on_cut_items(ctx):
+    """o in the place of q, for an item that many CTAs share."""
+    r = np.random.default_rng(19)
+    for lens, heads in (([9000], 8), ([300, 20, 0], 4)):
+        cache, batch = make(ctx, r, lens, None, 1, 64, 64)
+        q = 2 * r.standard_normal((batch.rows, heads * 64), dtype=np.float32)
+        clean, _ = attend(ctx, cache, batch, q, heads)
+        d = ctx.from_numpy(q)
+        ctx.call("glc_attention_kv", C.byref(cache.c), C.byref(batch.c), d.addr, q.shape[1], heads, d.addr, q.shape[1], 0)
+        ctx.sync()
+        assert same_bits(d.numpy(), clean)
 
 
 def test_pools_beyond_32_bits(ctx):
@@ -622,6 +661,19 @@ def test_sample_at_the_ends_of_the_random_number(ctx):
     # the first token of all, or the last with any weight
     assert tok[0] == 0 and tok[3] == 0 and tok[4] == 0
     assert all(tok[i] >= 1990 for i in (1, 2, 5))
+
+
+@pytest.mark.parametrize("t", [1e-45, 1e-30, 1e30, np.inf])
+def test_sample_at_the_ends_of_the_temperature(ctx, t):
+    """Next to none: the largest's equals share all; without bound: all are equal."""
+    r = np.random.default_rng(27)
+    x = (2 * r.standard_normal((4, 2000))).astype(np.float32)
+    x[1, [5, 9]] = x[1].max()
+    if t < 1e38:  # (infinity over infinity has no value)
+        x[2, 7] = np.inf
+    x[3, ::2] = -np.inf
+    u = np.array([0.5, 0.75, 0.5, 0.25], np.float32)
+    check_sample(x, t, None, None, None, u, *sample(ctx, x, t, None, None, None, u))
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 131072), (2, 262145), (1, 344064)])

@@ -205,6 +205,10 @@ def test_append_refuses(call, field, value, code):
     refused(call, "glc_kv_append", APPEND, field, value, code)
 
 
+def test_append_refuses_queries_in_place_of_another_stride(call):
+    refused(call, "glc_kv_append", {**APPEND, "q_out": P}, "q_out_ld", 260, INVALID)
+
+
 @pytest.mark.parametrize("field,value,code", CACHES + [
     ("k_ld", 127, INVALID), ("v_ld", 130, INVALID), ("k", P + 4, INVALID), ("v", P + 2, INVALID)])
 def test_read_refuses(call, field, value, code):
