@@ -59,8 +59,9 @@ KV_HD void kv_bad(int* err) {
 }
 
 // The rows [first, first + n) of sequence b that hold its new tokens, and its
-// length, held to what the operands and the table have; the error word is set
-// where they go beyond it.
+// length.  Where the length is not within the table or the rows are not within the
+// operands the error word is set and there are no rows: a length cut to the table's
+// would put the new tokens on the slots of its last ones.
 struct KvSpan {
   int first, n, len;
   bool bad;  // its starts do not ascend within the operands' rows
@@ -69,9 +70,10 @@ KV_HD KvSpan kv_span(const KvSeqs& s, int page, int b, int* err) {
   KvSpan r;
   r.len = s.lens[b];
   const int most = s.max_pages * page;  // at most 2^30, checked by the host
-  if (r.len < 0 || r.len > most) {
+  const bool fits = r.len >= 0 && r.len <= most;
+  if (!fits) {
     kv_bad(err);
-    r.len = r.len < 0 ? 0 : most;
+    r.len = 0;
   }
   r.first = b;
   r.n = 1;
@@ -88,6 +90,7 @@ KV_HD KvSpan kv_span(const KvSeqs& s, int page, int b, int* err) {
       r.n = end - r.first;
     }
   }
+  if (!fits) r.n = 0;
   return r;
 }
 

@@ -395,9 +395,11 @@ typedef struct glc_kv_cache {
  * sequences may share pages that no call writes.
  *
  * Values that only the device sees are checked there: a page index outside
- * the pools, a length beyond max_pages * page_size, rows outside
- * [0, num_rows) or a position beyond the rotation tables is neither read nor
- * written, and the next glc_sync returns GLC_ERR_DEVICE. */
+ * the pools, a length that is negative or beyond max_pages * page_size, rows
+ * outside [0, num_rows) or a position beyond the rotation tables is neither
+ * read nor written, and the next glc_sync returns GLC_ERR_DEVICE.  A sequence
+ * of such a length has no rows in the call: its pages, and its rows of every
+ * output, keep what they held. */
 typedef struct glc_kv_batch {
   const int* page_table; /* [num_seqs][max_pages] */
   const int* lens;       /* [num_seqs] */
