@@ -32,6 +32,7 @@
 #include <cooperative_groups.h>
 
 #include "kv_cache.cuh"
+#include "sample_plan.h"
 
 namespace cg = cooperative_groups;
 
@@ -308,8 +309,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   auto enough = [&](uint32_t w, auto logit) { return w >= least && (!only_top || logit() == top); };
   // the random number and p as 64-bit fractions; a goal is the high word of a product
   const u64 u64th = !(u > 0.f) ? 0 : u >= 1.f ? ~0ull : static_cast<u64>(static_cast<double>(u) * 18446744073709551616.0);
-  const u64 p64 = by_p ? static_cast<u64>(static_cast<double>(fmaxf(p_set, 0.f)) * 18446744073709551616.0) : 0;
-  auto p_goal = [&](u64 all) { return __umul64hi(all, p64) + (all * p64 != 0); };  // the least whole number not below p * all
+  const u64 p64 = by_p ? sample_share(p_set) : 0;
+  auto p_goal = [&](u64 all) -> u64 { return sample_goal(all, p64); };
 
   // a token of the order up to `cut` (all but NaN and -infinity where it is 0)
   auto before_cut = [&](float l, int i, u64 cut) {
@@ -362,6 +363,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
       const u64 upto = warp_scan(sum_y, lane);
       goal = goal_of(__shfl_sync(~0u, upto, 31));
       u64 before = base + upto - sum_y;
+      if (lane == 0) s.bin = 0, s.base = base, s.in_bin = 0;  // a goal that no bin reaches finds the first one
+      __syncwarp();
 #pragma unroll
       for (int j = 0; j < GROUPS / 32; ++j) {
         if (before < goal && goal <= before + y[j]) {
