@@ -40,15 +40,15 @@ namespace glc {
 namespace {
 
 constexpr int NT = 512, NW = NT / 32;
-constexpr int BINS = 8192;
+constexpr int BINS = SAMPLE_BINS;
 constexpr int CAP = 512;         // tokens that are ranked at once, one per thread
-constexpr int POWERS = 256;      // bins, and table entries, per factor of two of the weight
+constexpr int POWERS = SAMPLE_POWERS;
 constexpr int DIGIT = 10;        // bits of the order per step of narrowing
 constexpr int MAX_CLUSTER = 8;
 constexpr int SLICE_MAX = 43008; // tokens of a CTA: 168 KB of its shared memory
 constexpr uint32_t ONE = 1u << 31;  // the largest weight
 constexpr int GROUPS = BINS / 32;
-static_assert(2 << DIGIT <= BINS && 32 * POWERS == BINS, "digits (two sums each) and weights have a bin");
+static_assert(2 << DIGIT <= BINS, "digits (two sums each) have a bin");
 static_assert(CAP <= NT && GROUPS % 32 == 0, "a thread per listed token, a lane per group of bins");
 static_assert(BINS <= 16 * NT && GROUPS <= NT && 32 * MAX_CLUSTER <= NT, "a thread per group, and per bin of a group and CTA");
 static_assert(SLICE_MAX < (1 << 16), "sums of 16-bit numbers over a slice have 32 bits");
@@ -79,44 +79,6 @@ __device__ __forceinline__ float logit_of(u64 order) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 __device__ __forceinline__ int index_of(u64 order) { return static_cast<int>(~static_cast<uint32_t>(order)); }
-
-// 2^(31 - j / 256), as the whole number less the bits of ROUND, and as a float.
-struct Power {
-  uint32_t whole;
-  float power;
-};
-constexpr float ROUND = 12582912.f;  // 1.5 2^23: added to a number below 2^22, the nearest whole one in the low bits
-
-struct Weights {
-  float top, c;         // c: 1 / temperature, for what needs no more than 24 bits
-  double dtop, scale;   // 256 log2(e) / temperature
-  const Power* powers;
-  // (top - l) / temperature = (256 q + j + f) ln2 / 256, |f| <= 1/2, f exact to 2^-40:
-  // 2^-q by a shift, 2^(-j/256) from the table, 1 - exp(-f ln2 / 256) by three terms
-  // of its series (the fourth is below 2^-41), rounded to units before it is taken
-  // off.  *bin: 256 q + j; *lead: the weight's first 16 bits, before the shift.
-  // A logit that is -infinity or not a number has weight 0.
-  __device__ __forceinline__ uint32_t operator()(float l, int* bin, uint32_t* lead) const {
-    const bool some = (top - l) * c < 22.17f;  // else it rounds to 0 or 1, and bins stay below 8192
-    const double d = dtop - static_cast<double>(l);
-    const double k = fma(d, scale, 6755399441055744.0);  // 1.5 2^52: the whole number in the low bits
-    const float f = static_cast<float>(fma(d, scale, 6755399441055744.0 - k));
-    const int n = some ? __double2loint(k) : 32 * POWERS - 1;
-    constexpr float L = static_cast<float>(0.6931471805599453 / POWERS);
-    const float y = f * fmaf(f, fmaf(f, L * L * L / 6, -L * L / 2), L);
-    const Power p = powers[n & (POWERS - 1)];
-    const uint32_t w = p.whole - __float_as_uint(fmaf(p.power, y, ROUND));
-    const int q = n / POWERS;
-    *bin = n;
-    *lead = some ? w >> 15 : 0;
-    return some ? (w + ((1u << q) >> 1)) >> q : 0;
-  }
-  __device__ __forceinline__ uint32_t operator()(float l) const {
-    int bin;
-    uint32_t lead;
-    return (*this)(l, &bin, &lead);
-  }
-};
 
 __device__ __forceinline__ u64 warp_sum(u64 x) {
 #pragma unroll
@@ -151,7 +113,7 @@ struct Shared {
   u64 totals[2][MAX_CLUSTER], bases[MAX_CLUSTER];
   // a CTA's own
   u64 groups[GROUPS], parts[MAX_CLUSTER][32];
-  Power powers[POWERS];
+  SamplePower powers[POWERS];
   u64 warp_a[NW], warp_b[NW];
   float warp_f[NW], warp_top[NW];
   int warp_n[NW];
@@ -236,10 +198,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     }
   }
   if (n + tid < 4 * n4) x[n + tid] = __uint_as_float(0x7fc00000u);  // the last 4 tokens are whole
-  if (tid < POWERS) {
-    const double y = exp2(31.0 - tid * (1.0 / POWERS));
-    s.powers[tid] = {static_cast<uint32_t>(y + 0.5) + __float_as_uint(ROUND), static_cast<float>(y)};
-  }
+  if (tid < POWERS) s.powers[tid] = sample_power(tid);
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
@@ -296,12 +255,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     // (src is read again through plain)
   }
 
-  Weights weight;
+  SampleWeights weight;
   weight.top = top;
-  weight.dtop = top;
   const double inv = 1.0 / static_cast<double>(temp);
   weight.scale = inv * (POWERS * 1.4426950408889634);
-  weight.c = static_cast<float>(fmin(inv, static_cast<double>(FLT_MAX)));
   weight.powers = s.powers;
   // a token counts from this weight on; min_p >= 1 keeps the largest logit's equals
   const bool only_top = min_set >= 1.f;
@@ -553,7 +510,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
         u64 lower = 0;
         for (int i = 0; i < kept; ++i) lower += index_of(s.ranked[i]) < index ? s.weights[i] : 0;
         if (lower <= at && at < lower + w)
-          finish(index, static_cast<float>((static_cast<double>(logit_of(s.ranked[tid])) - weight.dtop) * inv -
+          finish(index, static_cast<float>((static_cast<double>(logit_of(s.ranked[tid])) - weight.top) * inv -
                                            log(static_cast<double>(all) * (1.0 / ONE))));
       }
       return;
@@ -724,7 +681,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
         const u64 upto = at + warp_scan(mine, lane);
         if (upto - mine <= goal && goal < upto)
           finish(first + i + lane,
-                 static_cast<float>((static_cast<double>(plain(src[i + lane])) - weight.dtop) * inv -
+                 static_cast<float>((static_cast<double>(plain(src[i + lane])) - weight.top) * inv -
                                     log(static_cast<double>(all) * (1.0 / ONE))));
         at = __shfl_sync(~0u, upto, 31);
         if (goal < at) break;

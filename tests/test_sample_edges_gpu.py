@@ -19,3 +19,13 @@ def test_the_smallest_nucleus_is_the_first_token(ctx, p, k, rows, vocab):
         tok, logp = sample(ctx, x, t, k, p, None, u)
         assert np.array_equal(tok, x.argmax(1)) and (logp == 0).all()
         check_sample(x, t, k, p, None, u, tok, logp)
+
+
+@pytest.mark.parametrize("t,size", [(1e-45, 1e-42), (1e-42, 1e-39), (2e-39, 3e-38), (1e-40, 1e-44), (3e-39, 1e-38), (1e-38, 1e-30)])
+@pytest.mark.parametrize("k,p,m", [(None, None, None), (None, 0.9, None), (40, 0.9, None), (700, None, 0.01), (None, 0.999, 0.05)])
+@pytest.mark.parametrize("rows,vocab", [(3, 1000), (2, 32000)])
+def test_temperatures_whose_inverse_no_float_holds(ctx, rows, vocab, k, p, m, t, size):
+    r = np.random.default_rng(vocab)
+    x = (size * r.standard_normal((rows, vocab))).astype(np.float32)
+    u = r.random(rows, dtype=np.float32)
+    check_sample(x, t, k, p, m, u, *sample(ctx, x, t, k, p, m, u))

@@ -31,3 +31,27 @@ def test_a_share_of_a_sum_is_reached_by_some_token(host, p, all_):
     assert 1 <= goal <= all_
     exact = math.ceil(Fraction(float(np.float32(p))) * all_)
     assert goal == max(exact, 1)
+
+
+def weights(host, top, t, x):
+    x = np.ascontiguousarray(x, np.float32)
+    w, bins, lead = np.zeros(len(x), np.uint32), np.zeros(len(x), np.int32), np.zeros(len(x), np.uint32)
+    p = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
+    host.sample_weights_of(C.c_float(top), C.c_float(t), p(x), len(x), p(w), p(bins), p(lead))
+    return w, bins, lead
+
+
+# a temperature whose inverse no float holds makes many bins of differences that are next to nothing
+@pytest.mark.parametrize("t", [1e-45, 1e-42, 1e-40, 2.9e-39, 3e-39, 1e-30, 0.01, 1.0, 1e30, np.inf])
+@pytest.mark.parametrize("size", [1e-44, 1e-41, 1e-39, 6e-38, 1e-20, 1.0, 1e5, 3e38])
+def test_every_weight_has_a_bin_and_is_that_of_its_logit(host, t, size):
+    r = np.random.default_rng(1)
+    far = np.concatenate([r.random(4000), [0.0, 1.0], 10.0 ** r.uniform(-8, 0, 1000)])
+    x = (-far * size).astype(np.float32)
+    top = float(x.max())
+    x = np.concatenate([x, np.array([np.nan, -np.inf], np.float32)])
+    w, bins, lead = weights(host, top, t, x)
+    assert (bins >= 0).all() and (bins < host.sample_bins()).all()
+    assert (w[-2:] == 0).all() and (lead[-2:] == 0).all()
+    d = (np.float64(top) - x[:-2].astype(np.float64)) / np.float64(np.float32(t))
+    assert (np.abs(w[:-2] - 2.0**31 * np.exp(-d)) <= 1.5 + 2.0**-9).all()  # half a unit of the table's entry, the correction, the shift
