@@ -154,6 +154,9 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   const int n = a.vocab - first < a.slice ? (a.vocab - first > 0 ? a.vocab - first : 0) : a.slice;
   const int n4 = (n + 3) >> 2;
   Shared& lead = *cluster.map_shared_rank(&s, 0);
+  // A CTA's shared memory may be written to once all of the cluster have started:
+  // they say so here and wait for it behind the logits' load.
+  cluster.barrier_arrive();
 
   // ---- the row's settings
   const float temp = a.temperature[row];
@@ -207,6 +210,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   }
   if (lane == 0) s.warp_top[warp] = top, s.warp_f[warp] = sum, s.warp_n[warp] = finite;
   __syncthreads();
+  cluster.barrier_wait();
   if (tid < ctas) {  // to each CTA of the row
     top = s.warp_top[0], sum = s.warp_f[0], finite = s.warp_n[0];
 #pragma unroll

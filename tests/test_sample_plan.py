@@ -55,3 +55,17 @@ def test_every_weight_has_a_bin_and_is_that_of_its_logit(host, t, size):
     assert (w[-2:] == 0).all() and (lead[-2:] == 0).all()
     d = (np.float64(top) - x[:-2].astype(np.float64)) / np.float64(np.float32(t))
     assert (np.abs(w[:-2] - 2.0**31 * np.exp(-d)) <= 1.5 + 2.0**-9).all()  # half a unit of the table's entry, the correction, the shift
+
+
+def test_no_store_to_another_cta_before_the_cluster_has_started():
+    """Every thread arrives at the cluster's barrier first thing and waits for it before the first store to the
+    shared memory of the row's other CTAs; each barrier is arrived at once and waited for once."""
+    text = (HERE.parent / "gollama_b200" / "csrc" / "sample.cu").read_text()
+    kernel = text[text.index("sample_kernel(const Sample a) {"):text.index('extern "C"')]
+    arrive, wait = kernel.index("cluster.barrier_arrive();"), kernel.index("cluster.barrier_wait();")
+    stores = [kernel.index(x) for x in ("o.tops[rank] =", "o.sums[rank] =", "o.finites[rank] =")]
+    assert arrive < kernel.index("const float* src") < wait < min(stores)
+    assert kernel.count("barrier_arrive") == kernel.count("barrier_wait") == 1
+    # before the wait nothing goes through a peer's address, returns, or uses the barrier for itself
+    before = kernel[:wait]
+    assert before.count("map_shared_rank") == 1 and "lead." not in before and "return" not in before and "cluster.sync" not in before
