@@ -1,13 +1,14 @@
 // Drawing the next token: temperature, top-k, top-p, min-p, and the inverse of
 // the kept tokens' running sum at a given random number.
 //
-// A token's weight is exp((l - max) / temperature) as a whole number of 2^-31,
-// so sums of weights are exact and every order of summation gives the same one.
-// The exponent is reduced in 64 bits and the weight is right to about one unit:
-// with tens of thousands of tokens kept, sums of float32 exponentials are off by
-// about 2^-25 of themselves, which moves past a token's edge about once in a
-// thousand rows, and that token is then another; units of 2^-31 of the largest
-// weight do so about once in 10^5.
+// A token's weight is exp((l - max) / temperature) to 27 bits, in whole numbers of
+// 2^-45 (sample_plan.h), so sums of weights are exact and every order of
+// summation gives the same one.  The exponent is reduced in 64 bits and the weight is
+// right to 2^-27 of itself and 2^-45 of the largest, so the sum of V tokens to V 2^-45
+// and 2^-27 of itself where all errors are of one sign, as in a tail of equal logits,
+// and to a small part of that in an ordinary row.  Sums of float32 exponentials are
+// off by about 2^-25 of themselves: with tens of thousands of tokens kept that moves
+// past a token's edge about once in a thousand rows, and that token is then another.
 //
 // Tokens are ordered by (logit falling, index rising), a total order; the kept
 // ones of top-k and of top-p are each a prefix of it, so each filter is a cut:
@@ -46,12 +47,12 @@ constexpr int POWERS = SAMPLE_POWERS;
 constexpr int DIGIT = 10;        // bits of the order per step of narrowing
 constexpr int MAX_CLUSTER = 8;
 constexpr int SLICE_MAX = 43008; // tokens of a CTA: 168 KB of its shared memory
-constexpr uint32_t ONE = 1u << 31;  // the largest weight
 constexpr int GROUPS = BINS / 32;
-static_assert(2 << DIGIT <= BINS, "digits (two sums each) have a bin");
+static_assert(3 << DIGIT <= BINS, "digits (three sums each) have a bin");
 static_assert(CAP <= NT && GROUPS % 32 == 0, "a thread per listed token, a lane per group of bins");
 static_assert(BINS <= 16 * NT && GROUPS <= NT && 32 * MAX_CLUSTER <= NT, "a thread per group, and per bin of a group and CTA");
 static_assert(SLICE_MAX < (1 << 16), "sums of 16-bit numbers over a slice have 32 bits");
+static_assert(SLICE_MAX / NT + 4 <= 127, "a thread's sum of weights");
 
 struct Sample {
   const float* logits;
@@ -266,7 +267,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   weight.powers = s.powers;
   // a token counts from this weight on; min_p >= 1 keeps the largest logit's equals
   const bool only_top = min_set >= 1.f;
-  const uint32_t least = only_top ? ONE : min_set > 0.f ? static_cast<uint32_t>(ceil(static_cast<double>(min_set) * ONE)) : 1u;
+  const double least_units = static_cast<double>(min_set) * SAMPLE_UNITS;
+  const uint32_t least = only_top ? SAMPLE_ONE : least_units > 1.0 ? sample_code(least_units) : SAMPLE_LEAST;
   auto enough = [&](uint32_t w, auto logit) { return w >= least && (!only_top || logit() == top); };
   // the random number and p as 64-bit fractions; a goal is the high word of a product
   const u64 u64th = !(u > 0.f) ? 0 : u >= 1.f ? ~0ull : static_cast<u64>(static_cast<double>(u) * 18446744073709551616.0);
@@ -400,7 +402,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   auto cut_of = [&](bool mass, int m, u64 base, u64 goal) {
     if (mass) {
       u64 all;
-      const u64 w = tid < m ? s.weights[tid] : 0;
+      const u64 w = tid < m ? sample_weight(s.weights[tid]) : 0;
       const u64 before = base + block_before(w, s.warp_a, &all, lane, warp);
       if (tid < m && before < goal && (tid == m - 1 || before + w >= goal)) s.cut = s.ranked[tid];
       __syncthreads();
@@ -429,12 +431,16 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
         const float l = plain(src[i]);
         const int d = digit_of(l, i);
         if (d < 0) continue;
-        const uint32_t w = mass ? wt[i] : 1;
-        atomicAdd(&s.hist[d], w & 0xffffu);
-        if (w >> 16) atomicAdd(&s.hist[DIGITS + d], w >> 16);
+        const u64 w = mass ? sample_weight(wt[i]) : 1;  // three numbers of 16 bits
+        atomicAdd(&s.hist[d], static_cast<uint32_t>(w) & 0xffffu);
+        if (w >> 16) {
+          atomicAdd(&s.hist[DIGITS + d], static_cast<uint32_t>(w >> 16) & 0xffffu);
+          atomicAdd(&s.hist[2 * DIGITS + d], static_cast<uint32_t>(w >> 32));
+        }
       }
-      locate(DIGITS, base, [](const Shared& o, int i) { return o.hist[i] + (static_cast<u64>(o.hist[DIGITS + i]) << 16); },
-             [&](u64) { return goal; });
+      locate(DIGITS, base, [](const Shared& o, int i) {
+        return o.hist[i] + (static_cast<u64>(o.hist[DIGITS + i]) << 16) + (static_cast<u64>(o.hist[2 * DIGITS + i]) << 32);
+      }, [&](u64) { return goal; });
       const int want = s.bin;
       base = s.base;
       for (int i = tid; i < n; i += NT) {
@@ -502,20 +508,20 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
       const int kept = static_cast<int>(goal);
       u64 all;
       uint32_t w = tid < kept ? s.weights[tid] : 0;
-      const u64 before = block_before(w, s.warp_a, &all, lane, warp);
+      const u64 before = block_before(sample_weight(w), s.warp_a, &all, lane, warp);
       if (by_p && before >= p_goal(all)) w = 0;
       if (w && !enough(w, [&] { return logit_of(s.ranked[tid]); })) w = 0;
-      block_before(w, s.warp_a, &all, lane, warp);
+      block_before(sample_weight(w), s.warp_a, &all, lane, warp);
       const int index = tid < kept ? index_of(s.ranked[tid]) : INT_MAX;
-      if (tid < kept) s.weights[tid] = w;
+      if (tid < kept) s.pulled[tid] = sample_weight(w);
       __syncthreads();
       const u64 at = __umul64hi(all, u64th);
       if (w) {  // in index order: the token whose interval has the goal
         u64 lower = 0;
-        for (int i = 0; i < kept; ++i) lower += index_of(s.ranked[i]) < index ? s.weights[i] : 0;
-        if (lower <= at && at < lower + w)
+        for (int i = 0; i < kept; ++i) lower += index_of(s.ranked[i]) < index ? s.pulled[i] : 0;
+        if (lower <= at && at < lower + sample_weight(w))
           finish(index, static_cast<float>((static_cast<double>(logit_of(s.ranked[tid])) - weight.top) * inv -
-                                           log(static_cast<double>(all) * (1.0 / ONE))));
+                                           log(static_cast<double>(all) * (1.0 / SAMPLE_UNITS))));
       }
       return;
     }
@@ -528,7 +534,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   // ---- the weights, in the logits' place; of top-p, their histogram: sums of
   // their first 16 bits by bin, which is to say nearly where the cut is
   if (by_p) clear();
-  u64 mine = 0;
+  SampleSum mine;
 #pragma unroll 1
   for (int i = tid; i < n4; i += NT) {
     const float4 v = reinterpret_cast<const float4*>(x)[i];
@@ -546,8 +552,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (lead16[j]) atomicAdd(&s.hist[bin[j]], lead16[j]);
-      mine += static_cast<u64>(w[0]) + w[1];
-      mine += static_cast<u64>(w[2]) + w[3];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mine.add(w[j]);
     }
     reinterpret_cast<uint4*>(wt)[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -568,29 +574,28 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     for (int i = 0; i < ctas; ++i) all += from[i];
     return all;
   };
-  uint32_t cut_w = 1;
+  uint32_t cut_w = SAMPLE_LEAST;
   if (by_p) {
-    tell(mine, [](Shared& o) -> u64* { return o.totals[0]; });
+    tell(mine.value(), [](Shared& o) -> u64* { return o.totals[0]; });
     locate(BINS, 0, [](const Shared& o, int i) { return (static_cast<u64>(o.hist[i]) << 15) >> (i / POWERS); },
            [&](u64 all) { return p_goal(all); });
     int bin = s.bin;
     const u64 goal = p_goal(told(s.totals[0]));
     for (;;) {
       // the region of that bin in whole weights: exactly what is before it and in it
-      const uint32_t high = bin == 0 ? ONE : static_cast<uint32_t>(exp2(31.0 - (bin - 0.5) * (1.0 / POWERS)));
-      const uint32_t low = bin == BINS - 1 ? 0 : static_cast<uint32_t>(exp2(31.0 - (bin + 0.5) * (1.0 / POWERS)));
-      u64 more = 0;
+      const uint32_t high = sample_bin_top(bin), low = sample_bin_top(bin + 1);
+      SampleSum more;
 #pragma unroll 2
       for (int i = tid; i < n4; i += NT) {
         const uint4 v = reinterpret_cast<const uint4*>(wt)[i];
         const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (ws[j] > high) more += ws[j];
+          if (ws[j] > high) more.add(ws[j]);
           else if (ws[j] > low) list_place(4 * i + j);
         }
       }
-      tell(more, [](Shared& o) -> u64* { return o.bases; });
+      tell(more.value(), [](Shared& o) -> u64* { return o.bases; });
       if (tid < CAP && tid < s.listed[round & 1]) {  // (tell's barrier: the places are there)
         const int i = static_cast<int>(s.list[tid]);
         s.list[tid] = order_of(plain(src[i]), first + i);
@@ -601,11 +606,12 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
       // what the region has; of more tokens than can be ranked, summed in each CTA
       u64 inside = 0;
       if (m <= CAP) {
-        block_before(tid < m ? s.weights[tid] : 0, s.warp_a, &inside, lane, warp);
+        block_before(tid < m ? sample_weight(s.weights[tid]) : 0, s.warp_a, &inside, lane, warp);
       } else {
-        u64 y = 0;
-        for (int i = tid; i < n; i += NT) y += wt[i] > low && wt[i] <= high ? wt[i] : 0;
-        tell(y, [](Shared& o) -> u64* { return o.totals[1]; });
+        SampleSum y;
+        for (int i = tid; i < n; i += NT)
+          if (wt[i] > low && wt[i] <= high) y.add(wt[i]);
+        tell(y.value(), [](Shared& o) -> u64* { return o.totals[1]; });
         cluster.sync();
         inside = told(s.totals[1]);
       }
@@ -631,9 +637,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   // token with more than the cut's weight is before it, near that weight its logit
   // says (weights are not monotone to the last unit; those of top-k's dropped
   // tokens are 0)
-  constexpr uint32_t NEAR = 4;
-  const uint32_t near_cut = by_p ? cut_w + NEAR : 0;
-  const uint32_t from_cut = cut_w > NEAR ? cut_w - NEAR : 1;
+  const uint32_t near_cut = by_p ? cut_w + SAMPLE_NEAR : 0;
+  const uint32_t from_cut = cut_w > SAMPLE_NEAR + SAMPLE_LEAST ? cut_w - SAMPLE_NEAR : SAMPLE_LEAST;
   const uint32_t floor_w = from_cut > least ? from_cut : least;
   auto kept = [&](uint32_t w, int i) -> uint32_t {
     if (w < floor_w) return 0;
@@ -645,15 +650,17 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
   };
   const int chunk = ((n + NW - 1) / NW + 127) & ~127;
   {
-    u64 w = 0;
+    SampleSum sum_w;
     const int end = (warp + 1) * chunk < n ? (warp + 1) * chunk : n;
 #pragma unroll 2
     for (int i = warp * chunk + 4 * lane; i < end; i += 128) {
       const uint4 v = *reinterpret_cast<const uint4*>(wt + i);
-      w += static_cast<u64>(kept(v.x, i)) + kept(v.y, i + 1);
-      w += static_cast<u64>(kept(v.z, i + 2)) + kept(v.w, i + 3);
+      sum_w.add(kept(v.x, i));
+      sum_w.add(kept(v.y, i + 1));
+      sum_w.add(kept(v.z, i + 2));
+      sum_w.add(kept(v.w, i + 3));
     }
-    w = warp_sum(w);
+    const u64 w = warp_sum(sum_w.value());
     if (lane == 0) s.warp_a[warp] = w;
     tell(lane == 0 ? w : 0, [](Shared& o) -> u64* { return o.totals[1]; });
   }
@@ -672,21 +679,21 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
     const int part = ((chunk + NW - 1) / NW + 31) & ~31;
     const int run0 = w0 * chunk, run1 = run0 + chunk < n ? run0 + chunk : n;
     const int p0 = run0 + warp * part, p1 = p0 + part < run1 ? p0 + part : run1;
-    u64 w = 0;
-    for (int i = p0 + lane; i < p1; i += 32) w += kept(wt[i], i);
-    w = warp_sum(w);
+    SampleSum sum_w;
+    for (int i = p0 + lane; i < p1; i += 32) sum_w.add(kept(wt[i], i));
+    const u64 w = warp_sum(sum_w.value());
     if (lane == 0) s.warp_b[warp] = w;
     __syncthreads();
     u64 at = 0;
     for (int i = 0; i < warp; ++i) at += s.warp_b[i];
     if (at <= goal && goal < at + w) {
       for (int i = p0; i < p1; i += 32) {
-        const u64 mine = i + lane < p1 ? kept(wt[i + lane], i + lane) : 0;
+        const u64 mine = i + lane < p1 ? sample_weight(kept(wt[i + lane], i + lane)) : 0;
         const u64 upto = at + warp_scan(mine, lane);
         if (upto - mine <= goal && goal < upto)
           finish(first + i + lane,
                  static_cast<float>((static_cast<double>(plain(src[i + lane])) - weight.top) * inv -
-                                    log(static_cast<double>(all) * (1.0 / ONE))));
+                                    log(static_cast<double>(all) * (1.0 / SAMPLE_UNITS))));
         at = __shfl_sync(~0u, upto, 31);
         if (goal < at) break;
       }

@@ -459,9 +459,9 @@ GLC_API int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const glc_
  * alone, min_p >= 1 the largest logit and its equals; any of top_k, top_p and
  * min_p may be NULL.  A NaN logit counts as -infinity; -infinity is never drawn; where a row has nothing else
  * its token is -1 and its logp -infinity.  logp (nullable): the natural
- * logarithm of the drawn token's share of the kept probability.  Weights are
- * whole numbers of 2^-31 of the largest, so that sums do not depend on their
- * order.  vocab at most 344064. */
+ * logarithm of the drawn token's share of the kept probability.  A weight is
+ * right to 2^-27 of itself and 2^-45 of the largest, and sums of weights are
+ * exact, so that they do not depend on their order.  vocab at most 344064. */
 GLC_API int glc_sample(glc_ctx* ctx, const float* logits, int ld, int rows, int vocab, const float* temperature,
                        const int* top_k, const float* top_p, const float* min_p, const float* uniform,
                        int64_t* tokens, float* logp);
