@@ -66,13 +66,7 @@ struct Shape {
   static constexpr int NB = Tile::NB;
   static constexpr int RT = NQ ? 8 * NQ : 4;  // query rows of an item
   static constexpr int STAGES = HD >= 96 ? 2 : 3;
-  // CTAs of an SM: 12 warps of 168 registers, of narrow heads 16 of 128.  More warps
-  // with fewer registers compute addresses again and again: at 128 a tile of 128
-  // elements takes 757 instructions, at 168 680 (64 x 8192 tokens, 32/8 heads of
-  // 128: 114.5 and 111.7 us); a tile of 64 at 96, 128 and 168 takes 560, 513 and 464
-  // (128 x 4096 tokens, 32/4 heads of 64: 49.2, 45.8 and 48.0 us).
-  static constexpr int WIDE = HD >= 96;
-  static constexpr int PER_SM = W >= 12 ? 1 : (NQ > 2 && WIDE ? 8 : NQ > 1 || WIDE ? 12 : 16) / W;
+  static constexpr int PER_SM = kv_per_sm(HD, NQ, W);
   static constexpr int SCALES = WK * NB * 6;  // a tile's scales as the products take them
   static constexpr int WARP = STAGES * Tile::BYTES + SCALES;
   static constexpr int QUERIES = NQ ? NQ * NB * 1024 : NB * 512;  // the queries as operands
@@ -941,30 +935,15 @@ int launch(Context* ctx, const AttnKv& a, cudaStream_t s) {
 
 template <int HD>
 int launch_for(Context* ctx, const AttnKv& a, cudaStream_t s) {
-  // Rows that share a KV head of a sequence, on average: as many query tiles in
-  // an item as they fill, since an item unpacks its keys and values once.
-  //   up to 4 rows: hi and lo as neighbouring columns of one product, 145 -> 123 us (64
-  //     x 8192 tokens, 32/8 heads of 128);
-  //   narrow heads, more than 24 rows: four tiles (items of 8 rows took 522 us for a
-  //     512-token chunk on 4096, 32/4 heads of 64, items of up to 32 take 409);
-  //   wide heads, 17 to 24 rows: three tiles, 60.5 -> 53.8 us (5 tokens each, 32/8 heads
-  //     of 128).  For longer chunks two (785 us, three 845), and for 24 rows of narrow
-  //     heads two (23.4 us, three 25.0): fewer registers, more warps.
-  const long long rows = static_cast<long long>(a.s.rows) * a.group / a.s.seqs;
-  if (HD <= 64 && rows > 24) return launch<HD, HD <= 64 ? 4 : 2, 4>(ctx, a, s);
-  if constexpr (HD >= 96) {
-    if (rows > 16 && rows <= 24) return launch<HD, 3, 4>(ctx, a, s);
+  const KvVariant v = kv_variant(HD, a.s.rows, a.s.seqs, a.group, a.c.kv_heads, ctx->num_sms);
+  if constexpr (HD <= 64) {
+    if (v.tiles == 4) return launch<HD, 4, 4>(ctx, a, s);
+  } else {
+    if (v.tiles == 3) return launch<HD, 3, 4>(ctx, a, s);
   }
-  if (rows > 8) return launch<HD, 2, 4>(ctx, a, s);
-  // Few items are cut between many CTAs, and few large CTAs leave fewer parts to
-  // join: one sequence of 131072 tokens (32/4 heads of 64) 23.6 us against 39.5 with
-  // CTAs of 4 warps, of 16384 11.0 against 22.2.  Of many items a CTA has several, and
-  // small CTAs overlap one's joins with another's copies: 32 sequences of 2048 take
-  // 14.4 and 14.5 us.
-  const long long items = static_cast<long long>(a.s.rows) * ((a.group + 7) / 8) * a.c.kv_heads;
-  const bool many = items >= ctx->num_sms / 2;
-  if (rows <= 4) return many ? launch<HD, 0, 4>(ctx, a, s) : launch<HD, 0, 16>(ctx, a, s);
-  return many ? launch<HD, 1, 4>(ctx, a, s) : launch<HD, 1, 16>(ctx, a, s);
+  if (v.tiles == 2) return launch<HD, 2, 4>(ctx, a, s);
+  if (v.tiles == 0) return v.warps == 4 ? launch<HD, 0, 4>(ctx, a, s) : launch<HD, 0, 16>(ctx, a, s);
+  return v.warps == 4 ? launch<HD, 1, 4>(ctx, a, s) : launch<HD, 1, 16>(ctx, a, s);
 }
 
 }  // namespace

@@ -211,6 +211,41 @@ KV_HD int kv_find_tile(const KvRows& w, int unit, int per, int at, int* first, i
   return 0;
 }
 
+// The kernel that a call takes: query tiles of 8 rows of an item (0: one tile of 4 rows)
+// and warps of a CTA.  By the rows that share a KV head of a sequence, on average: as many
+// query tiles in an item as they fill, since an item unpacks its keys and values once.
+//   up to 4 rows: hi and lo as neighbouring columns of one product, 145 -> 123 us (64
+//     x 8192 tokens, 32/8 heads of 128);
+//   narrow heads, more than 24 rows: four tiles (items of 8 rows took 522 us for a
+//     512-token chunk on 4096, 32/4 heads of 64, items of up to 32 take 409);
+//   wide heads, 17 to 24 rows: three tiles, 60.5 -> 53.8 us (5 tokens each, 32/8 heads
+//     of 128).  For longer chunks two (785 us, three 845), and for 24 rows of narrow
+//     heads two (23.4 us, three 25.0): fewer registers, more warps.
+// Few items are cut between many CTAs, and few large CTAs leave fewer parts to
+// join: one sequence of 131072 tokens (32/4 heads of 64) 23.6 us against 39.5 with
+// CTAs of 4 warps, of 16384 11.0 against 22.2.  Of many items a CTA has several, and
+// small CTAs overlap one's joins with another's copies: 32 sequences of 2048 take
+// 14.4 and 14.5 us.
+struct KvVariant {
+  int tiles, warps;
+};
+inline KvVariant kv_variant(int head_dim, long long rows, int seqs, int group, int kv_heads, int sms) {
+  const long long shared = rows * group / seqs;
+  if (head_dim <= 64 && shared > 24) return {4, 4};
+  if (head_dim >= 96 && shared > 16 && shared <= 24) return {3, 4};
+  if (shared > 8) return {2, 4};
+  const bool many = rows * ((group + 7) / 8) * kv_heads >= sms / 2;
+  return {shared <= 4 ? 0 : 1, many ? 4 : 16};
+}
+// Its CTAs of an SM: 12 warps of 168 registers, of narrow heads 16 of 128.  More warps
+// with fewer registers compute addresses again and again: at 128 a tile of 128
+// elements takes 757 instructions, at 168 680 (64 x 8192 tokens, 32/8 heads of
+// 128: 114.5 and 111.7 us); a tile of 64 at 96, 128 and 168 takes 560, 513 and 464
+// (128 x 4096 tokens, 32/4 heads of 64: 49.2, 45.8 and 48.0 us).
+constexpr int kv_per_sm(int head_dim, int tiles, int warps) {
+  return warps >= 12 ? 1 : (tiles > 2 && head_dim >= 96 ? 8 : tiles > 1 || head_dim >= 96 ? 12 : 16) / warps;
+}
+
 // Units that a call may have, at most: they are counted in 32 bits.  Of all variants
 // the tiles of 4 rows and the units of 128 keys make the most.
 inline double kv_most_units(double rows, double seqs, double group, double kv_heads, double max_pages, double page) {
