@@ -4,7 +4,8 @@
 // codes, d one scale per 32 elements), the running form of the softmax over
 // tiles of keys:
 //   s_j = q . k_j * log2(e) / sqrt(hd),  m' = max(m, max s_j),
-//   p_j = 2^(s_j - m'),  l = l 2^(m - m') + sum p_j,  o = o 2^(m - m') + sum p_j v_j.
+//   p_j = 2^(s_j - max s_j),  w = 2^(max s_j - m'),
+//   l = l 2^(m - m') + w sum p_j,  o = o 2^(m - m') + w sum p_j v_j.
 //
 // Codes become matrix operands without being scaled: two of them OR'ed into the
 // mantissas of two halves are 1024 + n (or 1024 + 16 n), and one packed addition
@@ -16,7 +17,9 @@
 // into two halves (hi + lo, 22 bits) and goes through in two products with one
 // accumulator.  The scales enter outside the products: a key's in float32 after
 // the product over its 32 elements, a value's before it, on the probabilities'
-// halves (hi' = hi d, lo' = lo d + the exact rest fma(hi, d, -hi')).
+// halves (hi' = hi d, lo' = lo d + the exact rest fma(hi, d, -hi')).  Each tile's
+// probabilities are relative to its own maximum, so that what lies beside a key
+// with nearly all of the weight keeps its bits.
 //
 // A work item is a sequence, a KV head and 8 to 32 query rows ((new token, head of
 // the KV head's group) pairs); its keys are cut into units, the units of all
@@ -432,10 +435,11 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 
     // rows: elements 4g + e of a block, columns: queries; [..][j][0..1] is e = 2j, [2..3] e = 2j + 1
     float acc[TILES][NB][2][4];
+    constexpr float NONE = -FLT_MAX;  // the maximum of no score: differences of two are numbers
     float m[TILES][2], l[TILES][2];  // of queries 8n + 2t and 8n + 2t + 1; paired: [0][0], of query t
 #pragma unroll
     for (int n = 0; n < TILES; ++n) {
-      m[n][0] = m[n][1] = -INFINITY;
+      m[n][0] = m[n][1] = NONE;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
@@ -444,15 +448,18 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
           for (int x = 0; x < 4; ++x) acc[n][i][j][x] = 0.f;
     }
-    // m is raised only when a score passes it by more than 2^SLACK, so that the
-    // sums are seldom rescaled; probabilities are held at 2^PEXP and value scales
-    // at 2^vexp times their size: their products stay below 2^15, and lo and lo'
-    // are normal halves where they matter
+    // A tile's probabilities are taken relative to its own largest score and held at
+    // 2^pexp times their size, value scales at 2^vexp times theirs: products stay below
+    // 2^15, and hi and lo are normal halves for all probabilities down to 2^-15 of the
+    // tile's largest (2^4 times, relative to the running maximum, gave errors of 3e-5 in
+    // keys beside one that has nearly all of the weight and a small value).  The tile's
+    // sum is then added at 2^(its maximum - m - pexp).  m is raised only when a score
+    // passes it by more than 2^SLACK, so that the sums are seldom rescaled.
     constexpr float SLACK = 4.f;
-    constexpr int PEXP = 4;
+    float pexp = 12.f;
     int vexp = 0;
-    uint32_t vtop = 0;  // largest scale (bits) that vexp allows
-    uint32_t up1 = 0x3c003c00u, up2 = 0x3c003c00u;  // 2^vexp, in pairs of halves
+    uint32_t vtop = 0;  // largest scale (bits) that they allow
+    uint32_t up = 0x3c003c00u;  // 2^vexp, in pairs of halves
 
     uint32_t stage = 0;  // bytes
     for (int key = key0 + warp * WK; key < key1; key += UNIT) {
@@ -480,11 +487,22 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
         }
         big = __reduce_max_sync(~0u, big);
         odd_scale = big > 0x7bffu;
+        if (odd_scale) {  // (the finite ones' sizes count)
+          big = 0;
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const uint32_t mag = (i & 1 ? vd[i / 2] >> 16 : vd[i / 2]) & 0x7fffu;
+            if (mag <= 0x7bffu) big = big > mag ? big : mag;
+          }
+          big = __reduce_max_sync(~0u, big);
+        }
         if (big > vtop) {  // the same for the whole warp
-          if (odd_scale) big = 0x7bffu;
-          // the largest scale to [2^4, 2^5): room for scales four times as large
+          // the largest scale to [1, 2): room for scales four times as large.  Scales made
+          // larger lose nothing; made smaller, by 2^-6 at most, those below 2^-8 lose bits,
+          // so beyond that the probabilities make way: to 2^3 for the largest scales.
           const int e = big < 0x400u ? -15 : static_cast<int>(big >> 10) - 15;
-          const int now = 4 - e;
+          const int now = e > 6 ? -6 : -e;
+          pexp = static_cast<float>(12 - (e + now));
           const float by = vtop ? __uint_as_float(static_cast<uint32_t>(127 + now - vexp) << 23) : 0.f;
 #pragma unroll
           for (int n = 0; n < TILES; ++n)
@@ -496,14 +514,11 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
                 for (int x = 0; x < 4; ++x) acc[n][i][j][x] *= by;
           vexp = now;
           vtop = e + 3 > 15 ? 0x7fffu : (static_cast<uint32_t>(e + 3 + 15) << 10) - 1;
-          // 2^vexp as two halves, since 2^19 is none
-          const int first = vexp > 15 ? 15 : vexp, second = vexp - first;
-          up1 = static_cast<uint32_t>(15 + first) * 0x04000400u;
-          up2 = static_cast<uint32_t>(15 + second) * 0x04000400u;
+          up = static_cast<uint32_t>(15 + vexp) * 0x04000400u;
         }
 #pragma unroll
         for (int i = 0; i < (NB + 1) / 2; ++i) {
-          const uint32_t d = mul2(mul2(vd[i], up1), up2);
+          const uint32_t d = mul2(vd[i], up);
           __half* to = vscale + (((lane >> 1) & 3) * 4 + (lane >> 3)) * 2 + (lane & 1);
           to[(2 * i) * 32] = __ushort_as_half(static_cast<unsigned short>(d));
           if (2 * i + 1 < NB) to[(2 * i + 1) * 32] = __ushort_as_half(static_cast<unsigned short>(d >> 16));
@@ -567,6 +582,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
       const bool edge = key + WK > key1 || key + WK - 1 > edge_key;
       // probabilities as halves, turned so that lane (g, t) has column g and keys 2t, 2t + 1 of each 8
       uint32_t hi[TILES][4], lo[TILES][4];
+      float by_tile[TILES][2];  // what the tile's sums count
       uint32_t own[4];  // paired: what the lane's column is, hi or lo; hi is 0 where it is hi
       if constexpr (PAIRED) {
         const float rs = rs_s[t];
@@ -586,7 +602,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 16)) * rs;
         if (__any_sync(~0u, top > m[0][0] + SLACK)) {
-          const float now = fmaxf(m[0][0], top), by = now == -INFINITY ? 0.f : exp2_fast(m[0][0] - now);
+          const float now = fmaxf(m[0][0], top), by = exp2_fast(m[0][0] - now);
           m[0][0] = now;
           l[0][0] *= by;
 #pragma unroll
@@ -596,13 +612,15 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
               for (int x = 0; x < 4; ++x) acc[0][i][j][x] *= by;
         }
-        const float ms = m[0][0] == -INFINITY ? 0.f : m[0][0] - PEXP;
+        const float ts = fmaxf(top - pexp, NONE);
+        by_tile[0][0] = exp2_fast(ts - m[0][0]);
+        float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float p = exp2_fast(fmaf(s[0][j][i], rs, -ms));
-            l[0][0] += p;
+            const float p = exp2_fast(fmaf(s[0][j][i], rs, -ts));
+            sum += p;
             uint32_t ph, pl;
             split2(p, p, &ph, &pl);
             ph = transposed(ph);
@@ -610,6 +628,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
             own[2 * j + i] = g & 1 ? pl : ph;
             hi[0][2 * j + i] = g & 1 ? ph : 0u;
           }
+        l[0][0] = fmaf(sum, by_tile[0][0], l[0][0]);
       }
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
@@ -638,7 +657,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float now = fmaxf(m[n][i], top[i]);
-            by[i] = now == -INFINITY ? 0.f : exp2_fast(m[n][i] - now);
+            by[i] = exp2_fast(m[n][i] - now);
             m[n][i] = now;
             l[n][i] *= by[i];
           }
@@ -649,20 +668,27 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
               for (int x = 0; x < 4; ++x) acc[n][i][j][x] *= by[x & 1];
         }
-        const float ms[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0] - PEXP, m[n][1] == -INFINITY ? 0.f : m[n][1] - PEXP};
+        float ts[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ts[i] = fmaxf(top[i] - pexp, NONE);
+          by_tile[n][i] = exp2_fast(ts[i] - m[n][i]);
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float p0 = exp2_fast(fmaf(s[n][j][2 * i], rs.x, -ms[0]));
-            const float p1 = exp2_fast(fmaf(s[n][j][2 * i + 1], rs.y, -ms[1]));
-            l[n][0] += p0;
-            l[n][1] += p1;
+            const float p0 = exp2_fast(fmaf(s[n][j][2 * i], rs.x, -ts[0]));
+            const float p1 = exp2_fast(fmaf(s[n][j][2 * i + 1], rs.y, -ts[1]));
+            sum[0] += p0;
+            sum[1] += p1;
             uint32_t ph, pl;
             split2(p0, p1, &ph, &pl);
             hi[n][2 * j + i] = transposed(ph);
             lo[n][2 * j + i] = transposed(pl);
           }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) l[n][i] = fmaf(sum[i], by_tile[n][i], l[n][i]);
       }
       const bool fix = odd_scale && edge;
 
@@ -704,7 +730,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int z = 0; z < 4; ++z) acc[0][i][e][z] += y[e][z];
+            for (int z = 0; z < 4; ++z) acc[0][i][e][z] = fmaf(y[e][z], by_tile[0][0], acc[0][i][e][z]);
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -738,7 +764,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int z = 0; z < 4; ++z) acc[n][i][e][z] += y[e][z];
+            for (int z = 0; z < 4; ++z) acc[n][i][e][z] = fmaf(y[e][z], by_tile[n][z & 1], acc[n][i][e][z]);
         }
       }
       stage = stage == (STAGES - 1) * Tile::BYTES ? 0 : stage + Tile::BYTES;
@@ -747,7 +773,7 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
     if (bad) kv_bad(a.err);
 
     // ---- the warps' parts of the segment joined through shared memory
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - PEXP - vexp) << 23);
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - vexp) << 23);
     __syncthreads();  // the rings are free
     float* jo = reinterpret_cast<float*>(smem) + warp * RT * HD;
     float* jm = reinterpret_cast<float*>(smem) + W * RT * HD;  // [W][RT] m, then l
@@ -761,8 +787,8 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) l[0][0] += __shfl_xor_sync(~0u, l[0][0], o);
       if (g == 0) {
-        jm[warp * RT + t] = m[0][0];
-        jm[W * RT + warp * RT + t] = l[0][0] * (1.f / (1 << PEXP));
+        jm[warp * RT + t] = m[0][0] == NONE ? -INFINITY : m[0][0];
+        jm[W * RT + warp * RT + t] = l[0][0];
       }
     }
 #pragma unroll
@@ -779,8 +805,8 @@ __global__ void __launch_bounds__(W * 32, Shape<HD, NQ, W>::PER_SM) attention_kv
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[n][x] += __shfl_xor_sync(~0u, l[n][x], o);
         if (g == 0) {
-          jm[warp * RT + 8 * n + 2 * t + x] = m[n][x];
-          jm[W * RT + warp * RT + 8 * n + 2 * t + x] = l[n][x] * (1.f / (1 << PEXP));
+          jm[warp * RT + 8 * n + 2 * t + x] = m[n][x] == NONE ? -INFINITY : m[n][x];
+          jm[W * RT + warp * RT + 8 * n + 2 * t + x] = l[n][x];
         }
       }
     }

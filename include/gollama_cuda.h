@@ -442,8 +442,11 @@ GLC_API int glc_kv_read(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_ba
  * [num_heads], the natural logarithm of the softmax's sum.  A token with no
  * visible position (lens[b] == 0) gets o = 0 and lse = -infinity.  Starts that
  * do not ascend within [0, num_rows] end the whole call, with nothing written.  The
- * products use the cache's exact values and q and the probabilities to 22
- * bits, the sums are float32.  Deterministic.  Uses the context workspace. */
+ * products use the cache's exact values, q to 22 bits, and a probability times
+ * its value's scale to 22 bits or, where that is more, to 2^-36 of the largest
+ * value scale in the sequence times the largest probability among the 32 keys
+ * of its tile; the sums are float32.  Deterministic.  Uses the context
+ * workspace. */
 GLC_API int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* batch, const float* q,
                              int q_ld, int num_heads, float* o, int o_ld, float* lse);
 /* Draws one token per row of logits [rows][ld], the first vocab columns
