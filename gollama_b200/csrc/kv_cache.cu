@@ -59,6 +59,15 @@ __device__ __noinline__ unsigned nearest_codes(const float* x, float d, float rd
   return bits;
 }
 
+// The call's sequences, dealt out over the threads of the first `lookers` rows of blocks.
+// The last thing of a kernel: as the first it took the append to 74 registers, and the
+// ragged batch above 179 us for 165.
+__device__ __forceinline__ void look_at_all(const KvPools& c, const KvSeqs& s, int lookers, int* err) {
+  if (blockIdx.y >= lookers) return;
+  const long long block = static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x;
+  kv_look(s, c.page, block * blockDim.x + threadIdx.x, static_cast<long long>(lookers) * gridDim.x * blockDim.x, err);
+}
+
 // A thread holds 4 consecutive elements (two rotation pairs) of one head of
 // one row; 8 neighbouring lanes hold the 32 that share a scale, so the largest
 // magnitude is three shuffles.  blockIdx.x covers the heads of a row (queries,
@@ -66,7 +75,8 @@ __device__ __noinline__ unsigned nearest_codes(const float* x, float d, float rd
 __global__ void __launch_bounds__(256)
     kv_append_kernel(KvPools c, KvSeqs s, const float* q, size_t q_ld, float* q_out, size_t q_out_ld, int heads,
                      const float* k, size_t k_ld, const float* v, size_t v_ld, const float* __restrict__ cos_t,
-                     const float* __restrict__ sin_t, int table_rows, int step, int* __restrict__ err) {
+                     const float* __restrict__ sin_t, int table_rows, int step, int lookers,
+                     int* __restrict__ err) {
   GLC_PDL_ENTRY();
   __shared__ RowAt at_s[ROWS];
   const int quads = c.head_dim >> 2;
@@ -165,12 +175,13 @@ __global__ void __launch_bounds__(256)
       }
     }
   }
+  look_at_all(c, s, lookers, err);
 }
 
 // A thread reads 4 codes (2 bytes) and their scale and writes 4 floats; rows as above.
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 8)
     kv_read_kernel(KvPools c, KvSeqs s, float* __restrict__ k, size_t k_ld, float* __restrict__ v, size_t v_ld,
-                   int step, int* __restrict__ err) {
+                   int step, int lookers, int* __restrict__ err) {
   GLC_PDL_ENTRY();
   __shared__ RowAt at_s[ROWS];
   const int quads = c.head_dim >> 2;
@@ -217,6 +228,7 @@ __global__ void __launch_bounds__(256)
       }
     }
   }
+  look_at_all(c, s, lookers, err);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -228,14 +240,16 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 struct RowGrid {
   dim3 grid;
   int step;
+  int lookers;  // rows of blocks that look at the sequences
 };
-RowGrid row_grid(const Context* ctx, int units, int rows, int most) {
+RowGrid row_grid(const Context* ctx, int units, int rows, int seqs, int most) {
   const int bx = (units + 255) / 256;
   const long long blocks = static_cast<long long>(bx) * rows, full = 8LL * ctx->num_sms;
   int step = 1;
   while (step < most && blocks > full * step) step *= 2;
   while ((rows + step - 1) / step > 65535) step *= 2;
-  return {dim3(bx, (rows + step - 1) / step), step};
+  const int by = (rows + step - 1) / step, look = (seqs + 256 * bx - 1) / (256 * bx);
+  return {dim3(bx, by), step, look < by ? look : by};
 }
 
 int cache_check(const char* what, const glc_kv_cache* c, std::string* msg) {
@@ -321,11 +335,11 @@ int glc_kv_append(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* b
   const double moved = static_cast<double>(batch->num_rows) *
                        (8.0 * q_width + (8.0 + 9.0 / 8.0) * kv_width);
   glc::ProfScope prof(c, glc::PROF_OTHER, moved, c->stream);
-  const glc::RowGrid g = glc::row_grid(c, units, batch->num_rows, glc::MOST);
+  const glc::RowGrid g = glc::row_grid(c, units, batch->num_rows, batch->num_seqs, glc::MOST);
   glc::launch_pdl(c, glc::kv_append_kernel, g.grid, 256, 0, c->stream,
                   glc::kv_pools(*cache), glc::kv_seqs(*batch), q, static_cast<size_t>(q_ld), q_out,
                   static_cast<size_t>(q_out_ld), heads, k, static_cast<size_t>(k_ld), v, static_cast<size_t>(v_ld),
-                  cos_t, sin_t, table_rows, g.step, c->d_err);
+                  cos_t, sin_t, table_rows, g.step, g.lookers, c->d_err);
   GLC_LAUNCH_CHECK(c, "kv_append");
   return GLC_OK;
 }
@@ -349,10 +363,10 @@ int glc_kv_read(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_batch* bat
   const int units = sides * cache->num_kv_heads * (cache->head_dim / 4);
   glc::ProfScope prof(c, glc::PROF_OTHER, static_cast<double>(batch->num_rows) * sides * width * (4.0 + 9.0 / 16.0),
                       c->stream);
-  const glc::RowGrid g = glc::row_grid(c, units, batch->num_rows, glc::MOST);
+  const glc::RowGrid g = glc::row_grid(c, units, batch->num_rows, batch->num_seqs, glc::MOST);
   glc::launch_pdl(c, glc::kv_read_kernel, g.grid, 256, 0, c->stream,
                   glc::kv_pools(*cache), glc::kv_seqs(*batch), k, static_cast<size_t>(k_ld), v,
-                  static_cast<size_t>(v_ld), g.step, c->d_err);
+                  static_cast<size_t>(v_ld), g.step, g.lookers, c->d_err);
   GLC_LAUNCH_CHECK(c, "kv_read");
   return GLC_OK;
 }

@@ -118,6 +118,13 @@ KV_HD bool kv_row(const KvSeqs& s, int page, int t, int* err, int* seq, int* pos
   return *pos >= 0;
 }
 
+// Every step-th sequence from `first` on is looked at for its rows and length alone:
+// where starts do not ascend, a row's search may pass by the pair that is wrong.
+KV_HD void kv_look(const KvSeqs& s, int page, long long first, long long step, int* err) {
+  if (!s.starts) return;  // a row is a sequence
+  for (long long b = first; b < s.seqs; b += step) kv_span(s, page, static_cast<int>(b), err);
+}
+
 // Page `index` of sequence b; -1 (and the error word) where the table has none.
 KV_HD int kv_page(const KvSeqs& s, int num_pages, int b, int index, int* err) {
   const int p = s.table[static_cast<size_t>(b) * s.max_pages + index];

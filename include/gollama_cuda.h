@@ -399,7 +399,9 @@ typedef struct glc_kv_cache {
  * outside [0, num_rows) or a position beyond the rotation tables is neither
  * read nor written, and the next glc_sync returns GLC_ERR_DEVICE.  A sequence
  * of such a length has no rows in the call: its pages, and its rows of every
- * output, keep what they held. */
+ * output, keep what they held.  A pair of starts that does not ascend within
+ * [0, num_rows] has no rows in glc_kv_append and glc_kv_read either, and a row
+ * that several of the other pairs claim is that of one of them. */
 typedef struct glc_kv_batch {
   const int* page_table; /* [num_seqs][max_pages] */
   const int* lens;       /* [num_seqs] */
