@@ -280,6 +280,9 @@ int kv_check(Context* ctx, const char* what, const glc_kv_cache* cache, const gl
   if (!batch) return no("no batch given");
   if (batch->num_seqs < 0 || batch->num_rows < 0 || batch->max_pages <= 0) return no("bad batch sizes");
   if (batch->num_seqs > 0 && (!batch->page_table || !batch->lens)) return no("page_table and lens must be given");
+  if ((reinterpret_cast<uintptr_t>(batch->page_table) | reinterpret_cast<uintptr_t>(batch->lens) |
+       reinterpret_cast<uintptr_t>(batch->starts)) & 3)
+    return no("page_table, lens and starts must be 4-byte aligned");
   if (!batch->starts && batch->num_rows < batch->num_seqs)
     return no("without starts, num_rows must be at least num_seqs");
   if (static_cast<long long>(batch->max_pages) * cache->page_size > 0x40000000)

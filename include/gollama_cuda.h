@@ -383,7 +383,7 @@ typedef struct glc_kv_cache {
   int head_dim;     /* 32, 64, 96 or 128 */
 } glc_kv_cache;
 
-/* The sequences of one call, in device memory (int32).  Sequence b has
+/* The sequences of one call, in device memory (int32, 4-byte aligned).  Sequence b has
  * lens[b] tokens in the cache, the new ones included; its tokens p * page_size
  * to (p + 1) * page_size - 1 are in page page_table[b * max_pages + p].  Its
  * new tokens are its last ones: rows starts[b] to starts[b + 1] - 1 of the
