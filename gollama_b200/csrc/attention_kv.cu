@@ -989,6 +989,7 @@ extern "C" int glc_attention_kv(glc_ctx* ctx, const glc_kv_cache* cache, const g
   const long long width = static_cast<long long>(num_heads) * cache->head_dim;
   if (q_ld < width || o_ld < width || ((q_ld | o_ld) & 3))
     return no("row strides must be multiples of 4 and at least num_heads * head_dim");
+  if (q == o && q_ld != o_ld) return no("o may be q where their strides are equal");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) & 15) return no("q and o must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(lse) & 3) return no("lse must be 4-byte aligned");
   const int group = num_heads / cache->num_kv_heads;

@@ -440,8 +440,8 @@ GLC_API int glc_kv_read(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_ba
  * pkg/model/attention.go:113-206): o = softmax(q . k / sqrt(head_dim)) v over
  * positions 0 to the token's own, query head h on KV head
  * h / (num_heads / num_kv_heads).  q, o: [num_rows][num_heads * head_dim] with
- * row strides in floats (multiples of 4); lse (nullable): [num_rows]
- * [num_heads], the natural logarithm of the softmax's sum.  A token with no
+ * row strides in floats (multiples of 4), o may be q where these are equal; lse
+ * (nullable): [num_rows][num_heads], the natural logarithm of the softmax's sum.  A token with no
  * visible position (lens[b] == 0) gets o = 0 and lse = -infinity.  Starts that
  * do not ascend within [0, num_rows] end the whole call, with nothing written.  The
  * products use the cache's exact values, q to 22 bits, and a probability times
