@@ -265,6 +265,9 @@ int cache_check(const char* what, const glc_kv_cache* c, std::string* msg) {
     *msg = std::string(what) + ": head_dim must be 32, 64, 96 or 128";
     return GLC_ERR_UNSUPPORTED;
   }
+  // sizes and offsets are counted in 64 bits
+  if (static_cast<double>(c->num_pages) * c->num_kv_heads * static_cast<double>(kv_pools(*c).chunk) > 4e18)
+    return no("num_pages, num_kv_heads and page_size are too large together");
   return GLC_OK;
 }
 
