@@ -21,7 +21,7 @@
 // probabilities are relative to its own maximum, so that what lies beside a key
 // with nearly all of the weight keeps its bits.
 //
-// A work item is a sequence, a KV head and 8 to 32 query rows ((new token, head of
+// A work item is a sequence, a KV head and 4 to 32 query rows ((new token, head of
 // the KV head's group) pairs); its keys are cut into units, the units of all
 // items laid end to end and dealt out evenly over the CTAs, so that lengths
 // may differ and a single long sequence fills the device.  Each warp walks its
@@ -29,10 +29,10 @@
 // a CTA join at the end of an item.  Items cut between CTAs leave partial
 // (m, l, o); the CTA that arrives last joins them in the order of their keys.
 //
-// It is bound by instructions: a tile of 32 keys of 128 elements takes a warp 680 for
-// 4 query rows (issue slots 0.56 used, the matrix pipe 19 %).  64 sequences of up to
-// 8192 tokens, 32/8 heads of 128, take 112 to 120 us, 0.59 to 0.63 of a plain copy's
-// rate for the 455 MB of cache; 512 new tokens on 4096, 32/4 heads of 64: 0.38 of the
+// It is bound by instructions: a tile of 32 keys of 128 elements takes a warp 692 for
+// 4 query rows (issue slots 0.57 used, the matrix pipe 19 %).  64 sequences of up to
+// 8192 tokens, 32/8 heads of 128, take 117 to 123 us, 0.57 to 0.60 of a plain copy's
+// rate for the 455 MB of cache; 512 new tokens on 4096, 32/4 heads of 64: 0.36 of the
 // matrix pipe.  Small batches are bound by latency: the share of the work, the page
 // table, the copy, the join.
 #include <cfloat>

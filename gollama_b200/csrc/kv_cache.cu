@@ -4,7 +4,7 @@
 // Both are one pass over their operands: a stored token moves (num_heads + 2
 // num_kv_heads) * head_dim floats in, num_heads * head_dim floats and
 // 2 num_kv_heads * head_dim * 9/16 bytes out.  13916 tokens of 32/8 heads of 128
-// with their read-back take 154 to 165 us, 0.67 to 0.72 of a plain copy's rate; looking each
+// with their read-back take 164 to 168 us, 0.66 to 0.68 of a plain copy's rate; looking each
 // row up on its own and reading none ahead took 281.
 #include <cfloat>
 #include <climits>

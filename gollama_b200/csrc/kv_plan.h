@@ -245,7 +245,8 @@ inline KvVariant kv_variant(int head_dim, long long rows, int seqs, int group, i
   return {shared <= 4 ? 0 : 1, many ? 4 : 16};
 }
 // Its CTAs of an SM: 12 warps of 168 registers, of narrow heads 16 of 128.  More warps
-// with fewer registers compute addresses again and again: at 128 a tile of 128
+// with fewer registers compute addresses again and again (measured before tiles took
+// their own maximum, 12 instructions more): at 128 a tile of 128
 // elements takes 757 instructions, at 168 680 (64 x 8192 tokens, 32/8 heads of
 // 128: 114.5 and 111.7 us); a tile of 64 at 96, 128 and 168 takes 560, 513 and 464
 // (128 x 4096 tokens, 32/4 heads of 64: 49.2, 45.8 and 48.0 us).

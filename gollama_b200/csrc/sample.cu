@@ -24,10 +24,10 @@
 // their place, the weights, so each is read and computed once; the histograms,
 // the gathered tokens and the partial sums meet through distributed shared
 // memory.  Only what is near a cut reads a logit again.  256 rows of 131075 at
-// top_p 0.95 take 231 us, a tenth of a plain copy's rate: a CTA's phases are 3.3 us
+// top_p 0.95 take 237 us, a tenth of a plain copy's rate: a CTA's phases were 3.3 us
 // for the logits, 5.1 for weights and histogram, 3.9 for the draw, and the rest of 27
-// exchanges between the CTAs of a row and what they wait for.  128 rows of 32000 with
-// mixed settings take 27 us, one row 9.7.
+// exchanges between the CTAs of a row and what they wait for (with weights of 2^-31,
+// 231 us in all).  128 rows of 32000 with mixed settings take 28 us, one row 9.9.
 #include <cfloat>
 #include <climits>
 #include <cooperative_groups.h>
@@ -621,7 +621,9 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const Sample a) {
                        : narrow(true, base, goal, [&](float, int i) { return wt[i] > low && wt[i] <= high; });
         break;
       }
-      // the first 16 bits said a neighbour: once more
+      // the first 16 bits said a neighbour: once more.  (Close to 1 the cut is where a few
+      // 10^-6 of the sum are many bins: 256 rows of 131075 take 237 us at top_p 0.95, 241 at
+      // 0.999, 276 at 0.99999, 663 at 0.9999999.)
       bin += step;
       ++round;
       cluster.sync();
@@ -726,7 +728,9 @@ extern "C" int glc_sample(glc_ctx* ctx, const float* logits, int ld, int rows, i
   glc::DeviceScope on(c);
   // CTAs of a row: as its slices need, and more while all of them run at once (128 rows
   // of 32000: 27 us with 2, 33 with 4); slices stay small enough for two CTAs on an SM
-  // (256 rows of 131075: 231 us with 8, 250 with 4 and slices of 33000)
+  // (256 rows of 131075: 231 us with 8, 250 with 4 and slices of 33000).  Above 139000
+  // tokens one of 8 leaves no room for a second one: 256 rows of 139000 take 242 us, of
+  // 141000 369, of 151936 395 and of 256000 542
   int ctas = 1;
   while (ctas < glc::MAX_CLUSTER && vocab / ctas > 1024 &&
          ((vocab + ctas - 1) / ctas > 16400 || static_cast<long long>(rows) * ctas <= c->num_sms))

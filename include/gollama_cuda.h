@@ -443,7 +443,10 @@ GLC_API int glc_kv_read(glc_ctx* ctx, const glc_kv_cache* cache, const glc_kv_ba
  * row strides in floats (multiples of 4), o may be q where these are equal; lse
  * (nullable): [num_rows][num_heads], the natural logarithm of the softmax's sum.  A token with no
  * visible position (lens[b] == 0) gets o = 0 and lse = -infinity.  Starts that
- * do not ascend within [0, num_rows] end the whole call, with nothing written.  The
+ * do not ascend within [0, num_rows] end the whole call, with nothing written.
+ * (num_rows * ceil(group / 4) + num_seqs) * num_kv_heads * (max_pages *
+ * page_size / 128 + 1), for groups of num_heads / num_kv_heads heads, stays
+ * below 2^31.  The
  * products use the cache's exact values, q to 22 bits, and a probability times
  * its value's scale to 22 bits or, where that is more, to 2^-36 of the largest
  * value scale in the sequence times the largest probability among the 32 keys
